@@ -173,7 +173,7 @@ def prepare(case, seed):
 
 def _scale(x):
     """Power of two per row ``[..., 1]``, fp32."""
-    m, e = torch.frexp(x.abs().amax(-1, keepdim=True).clamp(max=448.0 * 128) / 448.0)
+    m, e = torch.frexp(x.abs().amax(-1, keepdim=True).clamp(2.0 ** -24, 448.0 * 128) / 448.0)
     return torch.ldexp(torch.ones_like(m), (e - (m == 0.5).int()).clamp(-15, 7))
 
 
