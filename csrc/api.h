@@ -147,6 +147,20 @@ int b200_qkv_split_norm_rope_cache(void* q_out, const void* qkv, const int64_t* 
 int b200_rope(void* q, void* k, const int64_t* positions, const float* cos_sin, int64_t T, int Hq, int Hk, int D,
               int rot_dim, int neox, int64_t max_pos, int64_t q_stride, int64_t k_stride, const int64_t* positions3,
               int sec0, int sec1, int interleaved, int dtype, cudaStream_t st);
+// ---- 8-bit key / value cache: uint8 [num_blocks][2][Hkv] pages of block_size rows of D e4m3 codes and block_size fp32 scales
+// (common/kv8.cuh).  D a multiple of 16 up to 512, block_size a multiple of 4, cache 16-byte aligned; 2 = arguments it does not take.
+int b200_kv8_put(const void* k, const void* v, void* cache, const int64_t* slots, int64_t T, int Hkv, int D, int block_size,
+                 int64_t num_blocks, int64_t k_stride, int64_t v_stride, int dtype, cudaStream_t st);
+int b200_kv8_qkv(void* q_out, const void* qkv, const int64_t* positions, const float* cos_sin, const void* q_w, const void* k_w,
+                 float eps, int64_t T, int Hq, int Hkv, int D, int rot_dim, int neox, int gemma, void* cache, const int64_t* slots,
+                 int block_size, int64_t num_blocks, int64_t max_pos, int64_t qkv_stride, int dtype, cudaStream_t st);
+// rows of either cache (eight = 0: one in the type of `dtype`, [num_blocks][2][Hkv][block_size][D]) to k, v [M, Hkv, D]
+int b200_kv_gather(void* k, void* v, const void* cache, const int64_t* slots, int64_t M, int Hkv, int D, int block_size,
+                   int64_t num_blocks, int eight, int dtype, cudaStream_t st);
+int b200_kv8_attention_generic(void* out, const void* q, const void* cache, const int* block_tables, const int* seq_lens,
+                               const int* qsl, const float* sinks, int64_t T, int B, int Hq, int Hkv, int D, int block_size,
+                               int max_blocks, int64_t bt_stride, int64_t num_blocks, int window, float scale, int64_t q_stride,
+                               int dtype, cudaStream_t st);
 int b200_reshape_and_cache(const void* k, const void* v, void* kv_cache, const int64_t* slots, int64_t T, int Hkv,
                            int D, int block_size, int64_t num_blocks, int64_t k_stride, int64_t v_stride, int dtype,
                            cudaStream_t st);

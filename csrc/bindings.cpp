@@ -911,6 +911,73 @@ void reshape_and_cache(const at::Tensor& k, const at::Tensor& v, at::Tensor kv_c
                                k2.size(0), Hkv, D, kv_cache.size(3), kv_cache.size(0), k2.stride(0), v2.stride(0),
                                dtype_code(k), stream()), "reshape_and_cache");
 }
+// ---- 8-bit key / value cache (uint8 [blocks, 2, Hkv, block_size, D + 4], see common/kv8.cuh)
+void check_kv8(const at::Tensor& cache, int64_t Hkv, int64_t D, const at::Tensor& other) {
+  TORCH_CHECK(cache.is_cuda() && cache.device() == other.device(), "8-bit cache: ", cache.device(), " and ", other.device());
+  TORCH_CHECK(cache.scalar_type() == at::kByte && cache.dim() == 5 && cache.is_contiguous() && cache.size(1) == 2,
+              "8-bit cache: a contiguous uint8 tensor [blocks, 2, kv_heads, block_size, head_dim + 4]");
+  TORCH_CHECK(cache.size(2) == Hkv && cache.size(4) == D + 4, "8-bit cache of shape ", cache.sizes(), " for ", Hkv,
+              " key / value heads of ", D);
+  TORCH_CHECK(D >= 16 && D <= 512 && D % 16 == 0, "8-bit cache: head sizes are multiples of 16 up to 512, not ", D);
+  TORCH_CHECK(cache.size(3) >= 4 && cache.size(3) % 4 == 0, "8-bit cache: block sizes are multiples of 4, not ", cache.size(3));
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(cache.data_ptr()) % 16 == 0, "8-bit cache: not 16-byte aligned");
+}
+void check_slots(const at::Tensor& slots, int64_t n, const at::Tensor& other) {
+  TORCH_CHECK(slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.is_contiguous() && slots.size(0) >= n &&
+                  slots.device() == other.device(),
+              "slots: contiguous int64 [", n, "] on the cache's device");
+}
+void kv8_put(const at::Tensor& k, const at::Tensor& v, at::Tensor cache, const at::Tensor& slots) {
+  TORCH_CHECK(k.dim() == 3 && v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type() && v.device() == k.device(),
+              "keys and values: [T, kv_heads, head_dim] of one type");
+  const int64_t T = k.size(0), Hkv = k.size(1), D = k.size(2);
+  check_kv8(cache, Hkv, D, k);
+  check_slots(slots, T, cache);
+  TORCH_CHECK((k.stride(2) == 1 && k.stride(1) == D && v.stride(2) == 1 && v.stride(1) == D) || T == 0,
+              "keys and values: the heads of a token are contiguous");
+  c10::cuda::CUDAGuard guard(k.device());
+  check(b200_kv8_put(k.data_ptr(), v.data_ptr(), cache.data_ptr(), slots.data_ptr<int64_t>(), T, (int)Hkv, (int)D,
+                     (int)cache.size(3), cache.size(0), k.stride(0), v.stride(0), dtype_code(k), stream()), "kv8_put");
+}
+void kv8_qkv(at::Tensor q_out, const at::Tensor& qkv, const at::Tensor& positions, const at::Tensor& cos_sin,
+             const c10::optional<at::Tensor>& q_w, const c10::optional<at::Tensor>& k_w, double eps, int64_t Hq, int64_t Hkv,
+             int64_t D, bool neox, bool gemma, at::Tensor cache, const at::Tensor& slots) {
+  const int64_t T = qkv.size(0);
+  check_kv8(cache, Hkv, D, qkv);
+  check_slots(slots, T, cache);
+  TORCH_CHECK(qkv.dim() == 2 && qkv.stride(1) == 1 && qkv.size(1) == (Hq + 2 * Hkv) * D, "qkv: [T, (heads + 2 * kv_heads) * head_dim]");
+  TORCH_CHECK(q_out.is_contiguous() && q_out.numel() == T * Hq * D && q_out.scalar_type() == qkv.scalar_type() &&
+              q_out.device() == qkv.device());
+  TORCH_CHECK(cos_sin.scalar_type() == at::kFloat && cos_sin.is_contiguous() && cos_sin.dim() == 2 && cos_sin.size(1) <= D &&
+                  cos_sin.size(1) % 2 == 0 && cos_sin.device() == qkv.device(), "cos_sin: contiguous fp32 [positions, rotary dim]");
+  TORCH_CHECK(positions.scalar_type() == at::kLong && positions.is_contiguous() && positions.numel() >= T &&
+                  positions.device() == qkv.device(), "positions: contiguous int64 [T]");
+  for (const auto* w : {&q_w, &k_w})
+    TORCH_CHECK(!w->has_value() || ((*w)->is_contiguous() && (*w)->numel() == D && (*w)->scalar_type() == qkv.scalar_type() &&
+                                    (*w)->device() == qkv.device()), "norm weights: contiguous [head_dim] of qkv's type");
+  c10::cuda::CUDAGuard guard(qkv.device());
+  check(b200_kv8_qkv(q_out.data_ptr(), qkv.data_ptr(), positions.data_ptr<int64_t>(), cos_sin.data_ptr<float>(), opt_ptr(q_w),
+                     opt_ptr(k_w), (float)eps, T, (int)Hq, (int)Hkv, (int)D, (int)cos_sin.size(1), neox, gemma, cache.data_ptr(),
+                     slots.data_ptr<int64_t>(), (int)cache.size(3), cache.size(0), cos_sin.size(0), qkv.stride(0),
+                     dtype_code(qkv), stream()), "kv8_qkv");
+}
+void kv_gather(at::Tensor k, at::Tensor v, const at::Tensor& cache, const at::Tensor& slots) {
+  TORCH_CHECK(k.dim() == 3 && k.is_contiguous() && v.is_contiguous() && v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type() &&
+              v.device() == k.device());
+  const int64_t M = k.size(0), Hkv = k.size(1), D = k.size(2);
+  const bool eight = cache.scalar_type() == at::kByte;
+  if (eight) {
+    check_kv8(cache, Hkv, D, k);
+  } else {
+    TORCH_CHECK(cache.scalar_type() == k.scalar_type() && cache.dim() == 5 && cache.is_contiguous() && cache.size(1) == 2 &&
+                cache.size(2) == Hkv && cache.size(4) == D && cache.device() == k.device() && D % 16 == 0 &&
+                reinterpret_cast<uintptr_t>(cache.data_ptr()) % 16 == 0);
+  }
+  check_slots(slots, M, cache);
+  c10::cuda::CUDAGuard guard(k.device());
+  check(b200_kv_gather(k.data_ptr(), v.data_ptr(), cache.data_ptr(), slots.data_ptr<int64_t>(), M, (int)Hkv, (int)D,
+                       (int)cache.size(3), cache.size(0), eight, dtype_code(k), stream()), "kv_gather");
+}
 void concat_and_cache_mla(const at::Tensor& kv_c, const at::Tensor& k_pe, at::Tensor cache, const at::Tensor& slots) {
   TORCH_CHECK(cache.is_contiguous() && cache.dim() == 3 && kv_c.stride(-1) == 1 && k_pe.stride(-1) == 1);
   bool fp8 = cache.scalar_type() == at::kByte;
@@ -1011,6 +1078,37 @@ void paged_attention(at::Tensor out, const at::Tensor& q, const at::Tensor& kv_c
                              kv_cache.size(2), q.size(2), kv_cache.size(3), block_tables.stride(0), kv_cache.size(0),
                              max_query_len, num_splits, window, (float)scale, decode_layout, dtype_code(q), stream()),
         "paged_attention", num_splits > 1 ? 2 : 1);
+}
+
+// what every attention call over the 8-bit cache has to bring
+void check_kv8_attention(const at::Tensor& out, const at::Tensor& q, const at::Tensor& cache, const at::Tensor& block_tables,
+                         const at::Tensor& seq_lens, const at::Tensor& qsl, const c10::optional<at::Tensor>& sinks) {
+  TORCH_CHECK(q.dim() == 3 && q.stride(2) == 1 && (q.stride(1) == q.size(2) || q.size(1) == 1), "q: [T, heads, head_dim], the heads of a token contiguous");
+  TORCH_CHECK(out.sizes() == q.sizes() && out.is_contiguous() && out.scalar_type() == q.scalar_type() && out.device() == q.device(),
+              "out: contiguous, shape and type of q");
+  check_kv8(cache, cache.dim() == 5 ? cache.size(2) : 0, q.size(2), q);
+  TORCH_CHECK(cache.size(2) >= 1 && q.size(1) % cache.size(2) == 0, q.size(1), " query heads do not divide over ", cache.size(2), " key / value heads");
+  for (const at::Tensor* t : {&block_tables, &seq_lens, &qsl})
+    TORCH_CHECK(t->scalar_type() == at::kInt && t->device() == q.device(), "block tables and lengths: int32 on q's device");
+  const int64_t B = seq_lens.numel();
+  TORCH_CHECK(seq_lens.dim() == 1 && seq_lens.is_contiguous() && qsl.dim() == 1 && qsl.is_contiguous() && qsl.numel() == B + 1 &&
+                  block_tables.dim() == 2 && block_tables.size(0) == B && (block_tables.stride(1) == 1 || block_tables.size(1) <= 1),
+              "lengths [B], starts [B + 1], block tables [B, blocks]");
+  TORCH_CHECK(cache.size(0) >= 1, "8-bit cache without blocks");
+  if (sinks.has_value())
+    TORCH_CHECK(sinks->scalar_type() == at::kFloat && sinks->is_contiguous() && sinks->numel() == q.size(1) && sinks->device() == q.device(),
+                "sinks: contiguous fp32 [heads]");
+}
+void kv8_attention_generic(at::Tensor out, const at::Tensor& q, const at::Tensor& cache, const at::Tensor& block_tables,
+                           const at::Tensor& seq_lens, const at::Tensor& qsl, const c10::optional<at::Tensor>& sinks, int64_t window,
+                           double scale) {
+  check_kv8_attention(out, q, cache, block_tables, seq_lens, qsl, sinks);
+  c10::cuda::CUDAGuard guard(q.device());
+  check(b200_kv8_attention_generic(out.data_ptr(), q.data_ptr(), cache.data_ptr(), block_tables.data_ptr<int>(),
+                                   seq_lens.data_ptr<int>(), qsl.data_ptr<int>(), sinks.has_value() ? sinks->data_ptr<float>() : nullptr,
+                                   q.size(0), (int)seq_lens.size(0), (int)q.size(1), (int)cache.size(2), (int)q.size(2),
+                                   (int)cache.size(3), (int)block_tables.size(1), block_tables.stride(0), cache.size(0), (int)window,
+                                   (float)scale, q.stride(0), dtype_code(q), stream()), "kv8_attention_generic");
 }
 
 // score bias by distance [Hq, len] fp32 and raw output gates [T, Hq] of an attention call
@@ -2170,6 +2268,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rope", &rope);
   m.def("mrope", &mrope);
   m.def("reshape_and_cache", &reshape_and_cache);
+  m.def("kv8_put", &kv8_put);
+  m.def("kv8_qkv", &kv8_qkv);
+  m.def("kv_gather", &kv_gather);
+  m.def("kv8_attention_generic", &kv8_attention_generic);
   m.def("concat_and_cache_mla", &concat_and_cache_mla);
   m.def("indexer_k_quant_and_cache", &indexer_k_quant_and_cache);
   m.def("convert_req_index_to_global_index", &convert_req_index_to_global_index);

@@ -1,0 +1,309 @@
+// Writing keys and values into the 8-bit paged cache and reading them back (layout and number format: common/kv8.cuh).
+//
+// All three kernels are bound by memory.  A half-warp holds one row: lane l has elements 8 l .. 8 l + 7 of every 128, so that a
+// head of 128 is one 16-byte load a lane, its largest magnitude four shuffles, its codes one 8-byte store.  The two halves of a
+// warp take a token's key and value of the same head, because a NaN in either marks both.
+#include <math.h>
+
+#include "../api.h"
+#include "../common/kv8.cuh"
+#include "../common/launch.cuh"
+
+namespace b200 {
+namespace {
+
+constexpr int kWarps = 8;
+
+// elements 8 l .. 8 l + 7 of every 128 of a row of D; zeros behind its end
+template <typename T, int NI, bool kVec>
+__device__ __forceinline__ void load_row(float (&v)[NI][8], const T* src, int D, int l) {
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int at = i * 128 + l * 8;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+    if (at >= D) continue;          // D is a multiple of 16
+    if constexpr (kVec) {
+      constexpr int N = Vec16<T>::N;
+#pragma unroll
+      for (int p = 0; p < 8; p += N) {
+        const Vec16<T> a = ld_vec(src + at + p);
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[i][p + j] = to_f(a.v[j]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i][j] = to_f(src[at + j]);
+    }
+  }
+}
+
+// Lower half-warp: the key row, upper one: the value row of the same token and head.
+template <int NI>
+__device__ __forceinline__ void put_row(const float (&v)[NI][8], const Kv8Cache& c, int64_t slot, int h, int half, int l) {
+  float amax = 0.f;
+  bool nan = false;
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      amax = fmaxf(amax, fabsf(v[i][j]));
+      nan |= is_nan_bits(v[i][j]);
+    }
+  }
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  nan = __any_sync(0xffffffffu, nan);
+  if (slot < 0 || slot >= c.num_blocks * c.block_size) return;      // padding: the whole warp
+  const float s = kv8_scale(amax), inv = nan ? 0.f : pow2_inv(s);
+  const int off = (int)(slot % c.block_size);
+  uint8_t* page = c.page(slot / c.block_size, half, h);
+  uint8_t* dst = c.codes(page, off);
+#pragma unroll
+  for (int i = 0; i < NI; ++i)
+    if (i * 128 + l * 8 < c.D)
+      *reinterpret_cast<uint2*>(dst + i * 128 + l * 8) = nan ? make_uint2(0, 0) : kv8_pack8(v[i], inv);
+  if (l == 0) *c.scale(page, off) = nan ? __uint_as_float(0x7fffffffu) : s;
+}
+
+// k, v [T, Hkv, D] with strided tokens; a warp = (token, head).
+template <typename T, int NI, bool kVec>
+__global__ void __launch_bounds__(kWarps * 32) kv8_put_kernel(const T* __restrict__ k, const T* __restrict__ v, Kv8Cache c,
+                                                              const int64_t* __restrict__ slots, int64_t rows, int64_t k_stride,
+                                                              int64_t v_stride) {
+  griddep_launch();
+  griddep_wait();
+  const int64_t row = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  const int lane = threadIdx.x & 31, half = lane >> 4, l = lane & 15;
+  const int64_t t = row / c.Hkv;
+  const int h = (int)(row % c.Hkv);
+  float x[NI][8];
+  load_row<T, NI, kVec>(x, (half ? v + t * v_stride : k + t * k_stride) + (int64_t)h * c.D, c.D, l);
+  put_row<NI>(x, c, slots[t], h, half, l);
+}
+
+// A fused qkv row: split, optional RMSNorm of query and key heads, rotation, queries out in T, keys and values into the cache.
+// A warp takes two query heads, or the key and the value of one head; all in fp32 between the load and the one rounding at the
+// end (no rounding to T between norm and rotation, nor in front of the codes).  `kFast`: heads of 128 rotated whole in halves, 16-byte
+// aligned: a column's partner is the lane eight places away.  Otherwise rows meet their partners in shared memory.
+template <typename T, int NI, bool kFast, bool kVec>
+__global__ void __launch_bounds__(kWarps * 32) kv8_qkv_kernel(
+    T* __restrict__ q_out, const T* __restrict__ qkv, const int64_t* __restrict__ positions, const float* __restrict__ cos_sin,
+    const T* __restrict__ q_w, const T* __restrict__ k_w, float eps, int Hq, int rot, int neox, float gemma, Kv8Cache c,
+    const int64_t* __restrict__ slots, int64_t max_pos, int64_t qkv_stride) {
+  extern __shared__ float sm_rows[];
+  griddep_launch();
+  griddep_wait();
+  const int wid = threadIdx.x >> 5, lane = threadIdx.x & 31, half = lane >> 4, l = lane & 15;
+  const int64_t t = blockIdx.x;
+  const int D = c.D, q_units = (Hq + 1) / 2, units = q_units + c.Hkv;
+  int64_t pos = positions[t];
+  pos = pos < 0 ? 0 : (pos >= max_pos ? max_pos - 1 : pos);
+  const float* cs = cos_sin + pos * rot;
+  const int64_t slot = slots[t];
+  float cc[8], ss[8];
+  if constexpr (kFast) {
+    // x' = x c - y s on the first half, y' = y c + x s on the second: own * c + partner * (-s or s)
+#pragma unroll
+    for (int j = 0; j < 8; j += 4) {
+      *reinterpret_cast<float4*>(&cc[j]) = *reinterpret_cast<const float4*>(cs + (l & 7) * 8 + j);
+      *reinterpret_cast<float4*>(&ss[j]) = *reinterpret_cast<const float4*>(cs + 64 + (l & 7) * 8 + j);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ss[j] = l < 8 ? -ss[j] : ss[j];
+  }
+  for (int u = blockIdx.y * kWarps + wid; u < units; u += gridDim.y * kWarps) {
+    const bool is_q = u < q_units;
+    const int head = is_q ? 2 * u + half : Hq + (u - q_units) + half * c.Hkv;
+    const bool in = !is_q || head < Hq, turn = is_q || half == 0;
+    float v[NI][8];
+    load_row<T, NI, kVec>(v, qkv + t * qkv_stride + (int64_t)(in ? head : 0) * D, D, l);
+    const T* w = is_q ? q_w : k_w;
+    if (w != nullptr) {
+      float sq = 0.f;
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sq += v[i][j] * v[i][j];
+      }
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
+      if (turn) {
+        const float inv = rsqrtf(sq / D + eps);
+        float wv[NI][8];
+        load_row<T, NI, kVec>(wv, w, D, l);
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[i][j] = v[i][j] * inv * (wv[i][j] + gemma);
+        }
+      }
+    }
+    if constexpr (kFast) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float other = __shfl_xor_sync(0xffffffffu, v[0][j], 8);
+        if (turn) v[0][j] = v[0][j] * cc[j] + other * ss[j];
+      }
+    } else {
+      float* buf = sm_rows + (wid * 2 + half) * D;
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (i * 128 + l * 8 < D) buf[i * 128 + l * 8 + j] = v[i][j];
+      }
+      __syncwarp();
+      const int hr = rot >> 1;
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int at = i * 128 + l * 8 + j;
+          if (turn && at < 2 * hr) {
+            const bool first = neox ? at < hr : (at & 1) == 0;
+            const int f = neox ? (at < hr ? at : at - hr) : at >> 1;
+            const float other = buf[neox ? (at < hr ? at + hr : at - hr) : at ^ 1];
+            v[i][j] = first ? v[i][j] * cs[f] - other * cs[hr + f] : v[i][j] * cs[f] + other * cs[hr + f];
+          }
+        }
+      }
+      __syncwarp();       // read before the next unit's rows
+    }
+    if (is_q) {
+      if (!in) continue;
+      T* dst = q_out + (t * Hq + head) * (int64_t)D;
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const int at = i * 128 + l * 8;
+        if (at >= D) continue;
+        constexpr int N = Vec16<T>::N;
+#pragma unroll
+        for (int p = 0; p < 8; p += N) {
+          Vec16<T> a;
+#pragma unroll
+          for (int j = 0; j < N; ++j) a.v[j] = from_f<T>(v[i][p + j]);
+          st_vec(dst + at + p, a);
+        }
+      }
+    } else {
+      put_row<NI>(v, c, slot, u - q_units, half, l);
+    }
+  }
+}
+
+// k, v [M, Hkv, D] (contiguous) = rows `slots` of the cache; a slot outside it gives zeros.  A thread takes 16 elements of a row, the
+// grid's y says whether of the key or of the value.  `k8`: the 8-bit cache, otherwise one in T [block][2][kv_head][slot][D].
+template <typename T, bool k8>
+__global__ void __launch_bounds__(256) kv_gather_kernel(T* __restrict__ k, T* __restrict__ v, Kv8Cache c,
+                                                        const int64_t* __restrict__ slots, int64_t chunks) {
+  griddep_launch();
+  griddep_wait();
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= chunks) return;
+  const int per = c.D / 16, which = blockIdx.y;
+  const int64_t row = i / per, m = row / c.Hkv;
+  const int at = (int)(i % per) * 16, h = (int)(row % c.Hkv);
+  const int64_t slot = slots[m];
+  const bool in = slot >= 0 && slot < c.num_blocks * c.block_size;
+  const int64_t blk = in ? slot / c.block_size : 0;
+  const int off = in ? (int)(slot % c.block_size) : 0;
+  T* dst = (which ? v : k) + row * c.D + at;
+  alignas(16) T o[16];
+  if (!in) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) o[j] = from_f<T>(0.f);
+  } else if constexpr (k8) {
+    uint8_t* page = c.page(blk, which, h);
+    const uint4 w = *reinterpret_cast<const uint4*>(c.codes(page, off) + at);
+    const float s = *c.scale(page, off);
+    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float2 f = e4m3x2_to_float2((uint16_t)(x[j / 2] >> (16 * (j & 1))));
+      o[2 * j] = from_f<T>(f.x * s);
+      o[2 * j + 1] = from_f<T>(f.y * s);
+    }
+  } else {
+    const T* src = reinterpret_cast<const T*>(c.base) + (((blk * 2 + which) * c.Hkv + h) * c.block_size + off) * (int64_t)c.D + at;
+#pragma unroll
+    for (int j = 0; j < 16; j += Vec16<T>::N) st_vec(o + j, ld_vec(src + j));
+  }
+#pragma unroll
+  for (int j = 0; j < 16; j += Vec16<T>::N) st_vec(dst + j, ld_vec(o + j));
+}
+
+Kv8Cache cache_of(void* base, int64_t num_blocks, int Hkv, int block_size, int D) {
+  return Kv8Cache{static_cast<uint8_t*>(base), num_blocks, Hkv, block_size, D};
+}
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" int b200_kv8_put(const void* k, const void* v, void* cache, const int64_t* slots, int64_t T_, int Hkv, int D,
+                            int block_size, int64_t num_blocks, int64_t k_stride, int64_t v_stride, int dtype, cudaStream_t st) {
+  if (T_ == 0 || num_blocks == 0) return 0;
+  if (D % 16 || D < 16 || D > 512 || Hkv < 1 || block_size % 4 || block_size < 4) return 2;
+  const int64_t rows = T_ * Hkv, ctas = (rows + kWarps - 1) / kWarps;
+  if (ctas > 0x7fffffff) return 2;
+  const Kv8Cache c = cache_of(cache, num_blocks, Hkv, block_size, D);
+  const int esize = dtype == kF32 ? 4 : 2;
+  const bool vec = aligned16(k) && aligned16(v) && k_stride * esize % 16 == 0 && v_stride * esize % 16 == 0;
+#define B200_KV8_PUT(NI, VEC)                                                                                                  \
+  B200_DISPATCH_DTYPE(dtype, return (int)launch_pdl(kv8_put_kernel<T, NI, VEC>, dim3((unsigned)ctas), dim3(kWarps * 32), 0, st, \
+                                                    (const T*)k, (const T*)v, c, slots, rows, k_stride, v_stride))
+#define B200_KV8_PUT_NI(NI) if (vec) { B200_KV8_PUT(NI, true); } else { B200_KV8_PUT(NI, false); }
+  if (D <= 128) { B200_KV8_PUT_NI(1) }
+  else if (D <= 256) { B200_KV8_PUT_NI(2) }
+  else { B200_KV8_PUT_NI(4) }
+#undef B200_KV8_PUT_NI
+#undef B200_KV8_PUT
+  return 2;
+}
+
+extern "C" int b200_kv8_qkv(void* q_out, const void* qkv, const int64_t* positions, const float* cos_sin, const void* q_w,
+                            const void* k_w, float eps, int64_t T_, int Hq, int Hkv, int D, int rot_dim, int neox, int gemma,
+                            void* cache, const int64_t* slots, int block_size, int64_t num_blocks, int64_t max_pos,
+                            int64_t qkv_stride, int dtype, cudaStream_t st) {
+  if (T_ == 0) return 0;
+  if (D % 16 || D < 16 || D > 512 || Hkv < 1 || Hq < 1 || block_size % 4 || block_size < 4 || rot_dim > D || rot_dim % 2 ||
+      max_pos < 1 || T_ > 0x7fffffff)
+    return 2;
+  const Kv8Cache c = cache_of(cache, num_blocks, Hkv, block_size, D);
+  const int units = (Hq + 1) / 2 + Hkv, esize = dtype == kF32 ? 4 : 2;
+  const bool vec = aligned16(qkv) && qkv_stride * esize % 16 == 0 && aligned16(q_w) && aligned16(k_w);
+  const bool fast = vec && D == 128 && rot_dim == 128 && neox && aligned16(cos_sin);
+  // few tokens: a warp per unit, so that a decode step is one turn deep; otherwise a CTA per token, which reads its angles once
+  const dim3 grid((unsigned)T_, T_ <= 384 ? (unsigned)((units + kWarps - 1) / kWarps) : 1u);
+  const size_t smem = fast ? 0 : (size_t)kWarps * 2 * D * sizeof(float);
+#define B200_KV8_QKV(NI, FAST, VEC)                                                                                            \
+  B200_DISPATCH_DTYPE(dtype, return (int)launch_pdl(kv8_qkv_kernel<T, NI, FAST, VEC>, grid, dim3(kWarps * 32), smem, st,       \
+                                                    (T*)q_out, (const T*)qkv, positions, cos_sin, (const T*)q_w, (const T*)k_w, \
+                                                    eps, Hq, rot_dim, neox, gemma ? 1.f : 0.f, c, slots, max_pos, qkv_stride))
+#define B200_KV8_QKV_NI(NI) if (vec) { B200_KV8_QKV(NI, false, true); } else { B200_KV8_QKV(NI, false, false); }
+  if (fast) { B200_KV8_QKV(1, true, true); }
+  else if (D <= 128) { B200_KV8_QKV_NI(1) }
+  else if (D <= 256) { B200_KV8_QKV_NI(2) }
+  else { B200_KV8_QKV_NI(4) }
+#undef B200_KV8_QKV_NI
+#undef B200_KV8_QKV
+  return 2;
+}
+
+extern "C" int b200_kv_gather(void* k, void* v, const void* cache, const int64_t* slots, int64_t M, int Hkv, int D, int block_size,
+                              int64_t num_blocks, int eight, int dtype, cudaStream_t st) {
+  if (M == 0) return 0;
+  if (D % 16 || D < 16 || Hkv < 1 || block_size < 1 || (eight && block_size % 4)) return 2;
+  const int64_t chunks = M * Hkv * (D / 16), ctas = (chunks + 255) / 256;
+  if (ctas > 0x7fffffff) return 2;
+  const Kv8Cache c = cache_of(const_cast<void*>(cache), num_blocks, Hkv, block_size, D);
+  B200_DISPATCH_DTYPE(dtype, {
+    if (eight) return (int)launch_pdl(kv_gather_kernel<T, true>, dim3((unsigned)ctas, 2), dim3(256), 0, st, (T*)k, (T*)v, c, slots, chunks);
+    return (int)launch_pdl(kv_gather_kernel<T, false>, dim3((unsigned)ctas, 2), dim3(256), 0, st, (T*)k, (T*)v, c, slots, chunks);
+  });
+  return 2;
+}

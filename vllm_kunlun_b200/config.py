@@ -551,7 +551,7 @@ class CacheConfig:
     block_size: int = 16
     num_blocks: Optional[int] = None  # None = derive from memory budget
     gpu_memory_utilization: float = 0.9
-    cache_dtype: str = "auto"  # "auto" | "bfloat16" | "fp8_ds_mla"
+    cache_dtype: str = "auto"  # "auto" | "bfloat16" | "fp8_e4m3" (keys / values per head) | "fp8_ds_mla" (latent rows)
     enable_prefix_caching: bool = False
 
 

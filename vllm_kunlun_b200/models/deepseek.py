@@ -393,6 +393,8 @@ class DeepseekForCausalLM(MoEForCausalLM):
         spec = {}
         # `fp8_ds_mla` (sparse-attention models only): 656-byte rows = 4 x 128 e4m3 | 4 f32 scales | 64 bf16 rope dims
         fp8 = getattr(self, "kv_cache_dtype", "auto") == "fp8_ds_mla"
+        if getattr(self, "kv_cache_dtype", "auto") == "fp8_e4m3":
+            raise ValueError("kv_cache_dtype='fp8_e4m3' keeps keys and values per head; latent attention has neither")
         if fp8 and not cfg.index_topk:
             raise ValueError("kv_cache_dtype='fp8_ds_mla' is served for sparse-attention (indexer) models only")
         for i in range(self.first_layer, self.last_layer):

@@ -259,8 +259,17 @@ class DenseForCausalLM(nn.Module):
         """Per-layer ``(shape_per_block, dtype)`` for layers this stage owns."""
         st = get_state()
         kvh = max(1, self.cfg.num_kv_heads // st.tp_size)
-        return {i: ((2, kvh, block_size, self.cfg.head_dim), self.dtype)
-                for i in range(self.first_layer, self.last_layer)}
+        return {i: self.paged_kv_spec(kvh, block_size, self.cfg.head_dim) for i in range(self.first_layer, self.last_layer)}
+
+    def paged_kv_spec(self, kv_heads: int, block_size: int, head_dim: int):
+        """Keys and values of one layer: in the model's type, or with ``kv_cache_dtype="fp8_e4m3"`` in 8 bits and one fp32 scale per
+        token, head and K or V (:func:`ops.reshape_and_cache`)."""
+        if getattr(self, "kv_cache_dtype", "auto") != "fp8_e4m3":
+            return (2, kv_heads, block_size, head_dim), self.dtype
+        if head_dim % 16 or head_dim > 512 or block_size % 4:
+            raise ValueError(f"kv_cache_dtype='fp8_e4m3' serves head sizes that are multiples of 16 up to 512 and block sizes that are "
+                             f"multiples of 4, not {head_dim} and {block_size}")
+        return (2, kv_heads, block_size, head_dim + 4), torch.uint8
 
     # ---- weights ----
     def init_random(self, seed: int = 0, std: float = 0.02):

@@ -248,7 +248,7 @@ class Gemma4ForCausalLM(MoEForCausalLM):
             if kv_source_layer(self.cfg, i) != i:
                 continue
             lc = layer_attention_config(self.cfg, i)
-            spec[i] = ((2, max(1, lc.num_kv_heads // st.tp_size), block_size, lc.head_dim), self.dtype)
+            spec[i] = self.paged_kv_spec(max(1, lc.num_kv_heads // st.tp_size), block_size, lc.head_dim)
         return spec
 
     def load_weights(self, weights):

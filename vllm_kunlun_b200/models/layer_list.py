@@ -93,6 +93,8 @@ class LayerListForCausalLM(DenseForCausalLM):
 
     # ---- caches
     def kv_cache_spec(self, block_size: int):
+        if getattr(self, "kv_cache_dtype", "auto") == "fp8_e4m3":
+            raise ValueError("kv_cache_dtype='fp8_e4m3': the layers of this design keep caches in the model's type only")
         specs = {i: self.layers[str(i)].mixer.kv_cache_spec(block_size, self.dtype) for i in range(self.last_layer)}
         return {i: s for i, s in specs.items() if s is not None}
 

@@ -213,7 +213,7 @@ class Qwen3NextForCausalLM(MoEForCausalLM):
     def kv_cache_spec(self, block_size: int):
         st = get_state()
         kvh = max(1, self.cfg.num_kv_heads // st.tp_size)
-        return {i: ((2, kvh, block_size, self.cfg.head_dim), self.dtype)
+        return {i: self.paged_kv_spec(kvh, block_size, self.cfg.head_dim)
                 for i in range(self.first_layer, self.last_layer) if not self.cfg.layer_is_linear_attn(i)}
 
     def state_cache_spec(self):

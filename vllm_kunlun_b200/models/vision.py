@@ -384,6 +384,7 @@ class _VLBase(nn.Module):
         return self.language_model.compute_logits(hidden)
 
     def kv_cache_spec(self, block_size: int):
+        self.language_model.kv_cache_dtype = getattr(self, "kv_cache_dtype", "auto")
         return self.language_model.kv_cache_spec(block_size)
 
     def init_random(self, seed: int = 0, std: float = 0.02):

@@ -125,7 +125,15 @@ def mrope(q, k, positions3, cos_sin_cache, head_dim, sections, interleaved=False
 
 
 def reshape_and_cache(k, v, kv_cache, slot_mapping):
-    if k.is_cuda:
+    """Keys and values ``[T, kv_heads, head_dim]`` to their slots; negative slots are padding.  ``kv_cache``: in the type of ``k``,
+    ``[blocks, 2, kv_heads, block_size, head_dim]``, or in 8 bits, ``uint8 [blocks, 2, kv_heads, block_size, head_dim + 4]``
+    (:func:`reference.attention.kv8_rows` says what that holds; 4 more bytes a row for its scale)."""
+    if kv_cache.dtype == torch.uint8:
+        if k.is_cuda:
+            _c().kv8_put(k, v, kv_cache, slot_mapping)
+        else:
+            _ra.reshape_and_cache_kv8(k, v, kv_cache, slot_mapping)
+    elif k.is_cuda:
         _c().reshape_and_cache(k, v, kv_cache, slot_mapping)
     else:
         _ra.reshape_and_cache(k, v, kv_cache, slot_mapping)
@@ -136,19 +144,44 @@ def qkv_split_norm_rope_cache(qkv, positions, cos_sin_cache, q_weight, k_weight,
                               kv_cache, slot_mapping, gemma: bool = False):
     """One pass over a fused qkv row: split, optional per-head q/k RMSNorm, RoPE, and the K/V
     scatter into the paged cache (``_C::split_norm_rope_neox`` + ``reshape_and_cache_flash`` of the
-    reference in a single kernel).  Returns the rotated ``q [T, Hq*D]``."""
+    reference in a single kernel).  Returns the rotated ``q [T, Hq*D]``.  With an 8-bit cache (see :func:`reshape_and_cache`)
+    everything between the projection and the codes is fp32: norm and rotation are not rounded to ``qkv``'s type on the way."""
     T = qkv.shape[0]
+    eight = kv_cache is not None and kv_cache.dtype == torch.uint8
     if qkv.is_cuda:
         q = torch.empty(T, num_heads * head_dim, dtype=qkv.dtype, device=qkv.device)
+        if eight:
+            _c().kv8_qkv(q, qkv, positions, cos_sin_cache, q_weight, k_weight, eps, num_heads, num_kv_heads, head_dim, neox, gemma,
+                         kv_cache, slot_mapping)
+            return q
         _c().qkv_split_norm_rope_cache(q, qkv, positions, cos_sin_cache, q_weight, k_weight, eps,
                                        num_heads, num_kv_heads, head_dim, neox, gemma, kv_cache, slot_mapping)
         return q
-    q, k, v = _rb.split_qknorm_rope(qkv, positions, cos_sin_cache, q_weight, k_weight, eps,
+    q, k, v = _rb.split_qknorm_rope(qkv.float() if eight else qkv, positions, cos_sin_cache, q_weight, k_weight, eps,
                                     num_heads, num_kv_heads, head_dim, neox, gemma)
+    if eight:
+        reshape_and_cache(k.reshape(T, num_kv_heads, head_dim), v.reshape(T, num_kv_heads, head_dim), kv_cache, slot_mapping)
+        return q.to(qkv.dtype)
     if kv_cache is not None:
         _ra.reshape_and_cache(k.reshape(T, num_kv_heads, head_dim), v.reshape(T, num_kv_heads, head_dim),
                               kv_cache, slot_mapping)
     return q
+
+
+def gather_kv_cache(kv_cache, slots, dtype: Optional[torch.dtype] = None):
+    """Rows ``slots [M]`` (int64, as :func:`reshape_and_cache` takes them) of a paged cache: ``k, v [M, kv_heads, head_dim]``; a slot
+    outside the cache gives zeros.  ``dtype``: of the result - any of fp32, bf16, fp16 for an 8-bit cache (bf16 by default; fp16 and
+    bf16 hold its values exactly), the cache's own for the others."""
+    eight = kv_cache.dtype == torch.uint8
+    dtype = dtype or (torch.bfloat16 if eight else kv_cache.dtype)
+    if not eight and dtype != kv_cache.dtype:
+        raise ValueError(f"a cache in {kv_cache.dtype} is read back in its own type, not {dtype}")
+    if kv_cache.is_cuda:
+        shape = (slots.shape[0], kv_cache.shape[2], kv_cache.shape[4] - (4 if eight else 0))
+        k, v = (torch.empty(shape, dtype=dtype, device=kv_cache.device) for _ in range(2))
+        _c().kv_gather(k, v, kv_cache, slots)
+        return k, v
+    return _ra.gather_kv_cache(kv_cache, slots, dtype)
 
 
 def concat_and_cache_mla(kv_c, k_pe, kv_cache, slot_mapping):
@@ -207,7 +240,24 @@ def paged_attention(q, kv_cache, block_tables, seq_lens, query_start_loc, scale:
 
     The batch is decode-first: the first ``num_decodes`` requests have at most ``decode_query_len``
     query tokens each.  On CUDA a mixed batch is served by two launches (decode layout with
-    split-KV, then the prefill layout) over views of the same tensors."""
+    split-KV, then the prefill layout) over views of the same tensors.
+
+    ``kv_cache`` in 8 bits (see :func:`reshape_and_cache`): causal attention with an optional window and sinks; none of ``bias``,
+    ``gate``, ``keep_first``, ``sigmoid``.  A key whose block lies outside the pool is not there, a row that sees no key gives
+    zeros, and rows of no request are left as they are."""
+    if kv_cache.dtype == torch.uint8:
+        if bias is not None or gate is not None or keep_first or sigmoid:
+            raise ValueError("an 8-bit cache serves no score bias, output gate, kept keys or sigmoid weights")
+        if window is not None and window < 0:
+            raise ValueError("an 8-bit cache serves causal attention only")
+        if not q.is_cuda:
+            return _ra.paged_attention_kv8(q, kv_cache, block_tables, seq_lens if seq_lens_cpu is None else seq_lens_cpu,
+                                           query_start_loc if query_start_loc_cpu is None else query_start_loc_cpu, scale, window,
+                                           sinks)
+        from .kv8_cuda import paged_attention_kv8
+        return paged_attention_kv8(out, q, kv_cache, block_tables, seq_lens, query_start_loc, scale, max_query_len, max_seq_len,
+                                   window or 0, sinks, workspace, num_decodes, decode_query_len, num_decode_tokens,
+                                   stable_metadata)
     if q.is_cuda:
         if out is None:
             out = torch.empty(q.shape[0], q.shape[1], kv_cache.shape[-1], dtype=q.dtype, device=q.device)

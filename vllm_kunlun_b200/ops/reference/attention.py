@@ -5,6 +5,8 @@ Cache layouts of this framework (chosen so a page of one KV head is one contiguo
 
 * GQA:  ``kv_cache[num_blocks, 2, num_kv_heads, block_size, head_dim]``
   (the reference keeps ``(2, blocks, kv_heads, block_size, head)``, ``ops/paged_attn.py:43-55``)
+* GQA in 8 bits: ``uint8[num_blocks, 2, num_kv_heads, block_size, head_dim + 4]`` holding, per block, K or V and head,
+  ``block_size`` rows of ``head_dim`` e4m3 codes and then ``block_size`` fp32 scales (:func:`kv8_rows`)
 * MLA:  ``kv_cache[num_blocks, block_size, 576]`` = ``[kv_c(512) | k_pe(64)]``
   (``v1/attention/backends/mla/common.py:296-304``)
 * fp8_ds_mla: ``uint8[num_blocks, block_size, 656]`` = 512 e4m3 | 4 fp32 scales | 64 bf16 rope
@@ -35,6 +37,56 @@ def reshape_and_cache(k, v, kv_cache, slot_mapping):
             continue
         kv_cache[s // bs, 0, :, s % bs] = k[t].to(kv_cache.dtype)
         kv_cache[s // bs, 1, :, s % bs] = v[t].to(kv_cache.dtype)
+
+
+def kv8_views(kv_cache):
+    """``(codes e4m3 [blocks, 2, heads, block_size, D], scales fp32 [blocks, 2, heads, block_size])`` views of an 8-bit cache."""
+    nb, two, h, bs, w = kv_cache.shape
+    if kv_cache.dtype != torch.uint8 or two != 2 or w <= 4:
+        raise ValueError("an 8-bit cache is uint8 [blocks, 2, kv_heads, block_size, head_dim + 4]")
+    D = w - 4
+    pages = kv_cache.view(nb, two, h, bs * w)
+    return (pages[..., :bs * D].unflatten(-1, (bs, D)).view(torch.float8_e4m3fn), pages[..., bs * D:].view(torch.float32))
+
+
+def kv8_rows(k, v):
+    """What the 8-bit cache holds for ``k, v [T, heads, D]``: codes ``[T, 2, heads, D]`` (e4m3) and scales ``[T, 2, heads]`` (fp32).
+    A row's scale is the smallest power of two ``2^e``, ``-15 <= e <= 7``, with ``max |x| <= 448 * 2^e`` (``2^7`` if there is none:
+    such values saturate), its codes are ``x / scale`` rounded to the nearest e4m3 number.  A head whose key or value has a NaN
+    gets NaN for both scales and codes of zero."""
+    x = torch.stack([k, v], 1).float()
+    nan = x.isnan().any(-1).any(1, keepdim=True).expand(x.shape[:-1])
+    amax = torch.nan_to_num(x.abs(), nan=0.0, posinf=math.inf).amax(-1)
+    m, e = torch.frexp(amax.clamp(2.0 ** -24, FP8_MAX * 128) / FP8_MAX)
+    scale = torch.ldexp(torch.ones_like(m), (e - (m == 0.5).int()).clamp(-15, 7))
+    codes = torch.nan_to_num(x, nan=0.0, posinf=math.inf, neginf=-math.inf) / scale[..., None]
+    codes = codes.clamp(-FP8_MAX, FP8_MAX).masked_fill(nan[..., None], 0.0).to(torch.float8_e4m3fn)
+    return codes, scale.masked_fill(nan, math.nan)
+
+
+def reshape_and_cache_kv8(k, v, kv_cache, slot_mapping):
+    """:func:`reshape_and_cache` onto an 8-bit cache; slots outside it are skipped."""
+    bs = kv_cache.shape[3]
+    codes, scales = kv8_views(kv_cache)
+    c, s = kv8_rows(k, v)
+    for t in range(k.shape[0]):
+        at = int(slot_mapping[t])
+        if 0 <= at < kv_cache.shape[0] * bs:
+            codes.view(torch.uint8)[at // bs, :, :, at % bs] = c[t].view(torch.uint8)
+            scales[at // bs, :, :, at % bs] = s[t]
+
+
+def gather_kv_cache(kv_cache, slots, dtype):
+    """Rows ``slots`` of a cache as ``k, v [M, heads, D]``; zeros for slots outside it."""
+    nb, bs = kv_cache.shape[0], kv_cache.shape[3]
+    if kv_cache.dtype == torch.uint8:
+        codes, scales = kv8_views(kv_cache)
+    inside = (slots >= 0) & (slots < nb * bs)
+    at = torch.where(inside, slots, 0)
+    b, o = at // bs, at % bs
+    rows = (codes[b, :, :, o].float() * scales[b, :, :, o][..., None] if kv_cache.dtype == torch.uint8 else kv_cache[b, :, :, o])
+    rows = torch.where(inside[:, None, None, None], rows, 0.0).to(dtype)
+    return rows[:, 0].contiguous(), rows[:, 1].contiguous()
 
 
 def concat_and_cache_mla(kv_c, k_pe, kv_cache, slot_mapping):
@@ -230,6 +282,31 @@ def paged_attention(q, kv_cache, block_tables, seq_lens, query_start_loc, scale,
         if gate is not None:
             o = o * torch.sigmoid(gate[qs:qe].float()).unsqueeze(-1)
         out[qs:qe] = o.to(q.dtype)
+    return out
+
+
+def paged_attention_kv8(q, kv_cache, block_tables, seq_lens, query_start_loc, scale, window: Optional[int] = None, sinks=None,
+                        dtype=torch.float32):
+    """:func:`paged_attention` over an 8-bit cache, in ``dtype``.  A key whose block is outside the pool is not there; a row that
+    sees no key gives zeros; what a row does not see does not reach it, whatever it holds."""
+    nb, bs, g = kv_cache.shape[0], kv_cache.shape[3], q.shape[1] // kv_cache.shape[2]
+    out = torch.zeros_like(q)
+    for r in range(block_tables.shape[0]):
+        qs, qe, L = int(query_start_loc[r]), int(query_start_loc[r + 1]), int(seq_lens[r])
+        for i in range(qs, qe):
+            pos = L - (qe - i)
+            first, end = max(0, pos - window + 1) if window else 0, min(pos + 1, block_tables.shape[1] * bs)
+            j = torch.arange(first, max(first, end))
+            blk = block_tables[r].long()[j // bs]
+            j, blk = j[(blk >= 0) & (blk < nb)], blk[(blk >= 0) & (blk < nb)]
+            if not len(j):
+                continue
+            k, v = (x.repeat_interleave(g, 1) for x in gather_kv_cache(kv_cache, blk * bs + j % bs, dtype))
+            s = torch.einsum("hd,jhd->hj", q[i].to(dtype), k) * scale
+            if sinks is not None:
+                s = torch.cat([s, sinks.to(dtype)[:, None]], 1)
+            p = torch.softmax(s, 1)[:, :len(j)]
+            out[i] = torch.einsum("hj,jhd->hd", p, v).to(q.dtype)
     return out
 
 
