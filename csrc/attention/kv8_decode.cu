@@ -1,0 +1,919 @@
+// Decode attention over the 8-bit paged cache (common/kv8.cuh) on tcgen05 + TMEM, fed by TMA straight from the pages: at most 16
+// query rows (heads of a group x query tokens) per key / value head, heads of 64, 128 or 256.
+//
+// What bounds it is reading the cache, D + 4 bytes a row, so nothing is converted on the way: codes go from memory to shared memory to
+// the tensor core as e4m3 operands, and the numbers that have more digits are taken apart instead.
+//   * Queries: q times a power of two that puts the row's largest element in (128, 256] is the sum of e4m3 pieces, each the rounded rest
+//     of those in front of it.  A piece has four significant bits and rests are signed, so two pieces hold the 8 bits of bf16 and three the
+//     11 of fp16 exactly, down to 2^-18 of the row's largest element.  All pieces add into one accumulator.
+//   * Weights: exp2(s - m) * 2^7 * v_scale / (largest v_scale so far) <= 2^8, in fp16 and then in the same pieces, each rest times 2^5 so that
+//     weights far below the largest keep their digits; every piece has accumulator columns of its own.  Two pieces are off by less
+//     than 2^-8 (the rounding of a bf16 weight), three carry the 11 bits of fp16.
+// Few query rows and many keys: keys are the UMMA M side, query rows the N side.
+//     S^T[128 rows, 16]        = K[128 rows, 128 B] . Q^T      per piece, K-major as cached
+//     O^T[128 dims, 16 pieces] += V^T[128 dims, 128 rows] . P   V MN-major as cached
+// Heads of 64: a row of 128 bytes holds two keys, so Q^T has 32 columns, (q, 0) and (0, q): scores of the even and the odd keys; P has the
+// even keys' weights in one half of its columns and the odd ones' in the other, and O is the sum of the two matching quadrants.
+// Heads of 256: two 128-byte blocks a key, two O^T accumulators.
+//
+// Work: all tiles of all (request, head) items in one line, cut into equal pieces, one a CTA (two CTAs an SM where shared memory lasts), so
+// that uneven requests cost what their sum costs.  Where a cut falls, from the lengths on the device: captured launches adapt.  An item
+// that lies in several CTAs is merged by the last of them to arrive, in the order of the cuts: the result does not depend on who that is.
+// 224 threads: warp 0 TMA producer (a lane per box of a tile, which looks its block up a tile ahead), warp 1 MMA issuer, warps 2-5 softmax
+// (thread = row of the tile; TMEM lane = output dim at the end), warp 6 queries.  Every wait is bounded; on time-out the status word is
+// set and the CTA unwinds.
+#include <cuda.h>
+#include <math.h>
+
+#include "../api.h"
+#include "../common/kv8.cuh"
+#include "../common/launch.cuh"
+#include "../common/ptx.cuh"
+#include "../gemm/gemm_common.cuh"
+
+namespace b200 {
+namespace kv8dec {
+
+constexpr int kThreads = 224;
+constexpr int kM = 128;          // rows of 128 bytes in a tile
+constexpr int kRows = 16;        // query rows, zero padded
+constexpr int kMaxB = 2048;      // requests a launch
+constexpr int kFactors = 4;      // ring of query factors: S runs at most two tiles ahead of the softmax
+constexpr float kSlack = 1.f;    // the running maximum moves when a score exceeds it by more (log2): weights stay below 2^(7 + 1)
+constexpr float kLift = 7.f;
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct Params {
+  const void* q;            // [T, Hq, D], token stride q_stride
+  void* out;                // [T, Hq, D]
+  const uint8_t* cache;
+  float* ws_o;              // [2 * grid][16][D]
+  float* ws_lse;            // [2 * grid][16]
+  int* tickets;             // [B * Hkv], zero between calls
+  const int* block_tables;
+  const int* seq_lens;
+  const int* qsl;
+  const float* sinks;
+  int* status;
+  int64_t num_blocks, bt_stride, q_stride;
+  int B, Hq, Hkv, block_size, max_blocks, window, slots, early_meta, min_tiles;
+  float scale_log2;
+};
+
+template <int D> struct Geo {
+  static constexpr int kPack = D == 64 ? 2 : 1;        // keys in a row of 128 bytes
+  static constexpr int kBlk = D == 256 ? 2 : 1;        // 128-byte blocks of a key
+  static constexpr int kKeys = kM * kPack;             // keys of a tile
+  static constexpr int kOp = kBlk * kM * 128;          // codes of K or V of a tile
+  static constexpr int kNS = kRows * kPack;            // columns of S^T
+};
+template <typename T> struct Pieces;
+template <> struct Pieces<__nv_bfloat16> { static constexpr int n = 2; };
+template <> struct Pieces<__half> { static constexpr int n = 3; };
+
+template <typename T, int D> struct Layout {
+  using G = Geo<D>;
+  static constexpr int P = Pieces<T>::n;
+  static constexpr int kNO = G::kNS * P;                       // columns of an O^T accumulator
+  static constexpr int kQ = P * G::kBlk * G::kNS * 128;        // one query buffer
+  static constexpr int kP = kNO * 128;                         // one weight buffer
+  static constexpr int kCols = 2 * G::kNS + G::kBlk * kNO;
+  static constexpr int kTmem = kCols <= 64 ? 64 : kCols <= 128 ? 128 : 256;
+  static constexpr int kScales = G::kKeys * 4;
+  // barriers, factors, flags, exchange buffers
+  static constexpr int kMisc = 4096 + (D == 64 ? kRows * 64 * 4 : 0);
+  static size_t smem(int slots, int B) {
+    return 1024 + (size_t)slots * (G::kOp + kScales) + 2 * kQ + 2 * kP + kMisc + (size_t)(B + 1) * 4;
+  }
+};
+
+__device__ __forceinline__ void named_bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
+__device__ __forceinline__ float warp_max_redux(float v) {
+  int i = __float_as_int(v);
+  i = i >= 0 ? i : i ^ 0x7fffffff;
+  i = __reduce_max_sync(0xffffffffu, i);
+  i = i >= 0 ? i : i ^ 0x7fffffff;
+  return __int_as_float(i);
+}
+// into the registers themselves: no copy may come before the wait
+__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld_x16(taddr, r); }
+__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld_x32(taddr, r); }
+__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ uint16_t f16x2_to_e4m3x2(__half2 v) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(*reinterpret_cast<const uint32_t*>(&v)));
+  return r;
+}
+__device__ __forceinline__ __half2 as_half2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
+
+// A CTA's share of the line of tiles, item by item.
+struct Walk {
+  const int* pre;          // [B + 1] tiles of the requests in front (of one head)
+  long long at, end;       // units left
+  int Hkv, B;
+  int req, head, tile, n;  // current item: its tiles, and the first of this CTA's among them
+  int count;               // this CTA's tiles of it
+  __device__ __forceinline__ void start(const int* pre_, int B_, int Hkv_, long long lo, long long hi) {
+    pre = pre_; B = B_; Hkv = Hkv_; at = lo; end = hi;
+    count = 0;
+    if (at >= end) return;
+    int a = 0, b = B;      // the last request whose tiles start at or before `at`: those without tiles lie in front of it
+    while (b - a > 1) {
+      const int mid = (a + b) >> 1;
+      if ((long long)pre[mid] * Hkv <= at) a = mid; else b = mid;
+    }
+    req = a;
+    n = pre[a + 1] - pre[a];
+    const long long in = at - (long long)pre[a] * Hkv;
+    head = (int)(in / n);
+    tile = (int)(in % n);
+    count = (int)min((long long)(n - tile), end - at);
+  }
+  __device__ __forceinline__ bool more() const { return count > 0; }
+  __device__ __forceinline__ void next() {
+    at += count;
+    count = 0;
+    if (at >= end) return;
+    tile = 0;
+    if (++head == Hkv) {
+      head = 0;
+      do { ++req; n = pre[req + 1] - pre[req]; } while (n == 0);
+    }
+    count = (int)min((long long)n, end - at);
+  }
+};
+
+struct Request {
+  int qs, q_len, seq_len, ctx, kv_begin;
+};
+template <int D>
+__device__ __forceinline__ Request request_of(const Params& p, int req) {
+  Request r;
+  r.qs = p.qsl[req];
+  r.q_len = p.qsl[req + 1] - r.qs;
+  r.seq_len = p.seq_lens[req];
+  r.ctx = r.seq_len - r.q_len;
+  r.kv_begin = p.window > 0 ? max(0, r.ctx - p.window + 1) / Geo<D>::kKeys * Geo<D>::kKeys : 0;
+  return r;
+}
+
+template <typename T, int D, int NR>
+__global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2)
+kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ Params p) {
+  using G = Geo<D>;
+  using L = Layout<T, D>;
+  constexpr int P = L::P, kPack = G::kPack, kBlk = G::kBlk, kKeys = G::kKeys, kNS = G::kNS, kNO = L::kNO;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int ns = p.slots;
+  uint8_t* sQ = smem + ns * G::kOp;                          // [2][P][kBlk][kNS][128 B]
+  uint8_t* sP = sQ + 2 * L::kQ;                              // [2][kNO][128 B]
+  float* sScale = reinterpret_cast<float*>(sP + 2 * L::kP);  // [ns][kKeys]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sScale + ns * kKeys);
+  uint64_t* kv_full = bars;              // [16]
+  uint64_t* kv_empty = bars + 16;        // [16] the product that reads the codes, and four warps that read the scales
+  uint64_t* s_full = bars + 32;          // [2]
+  uint64_t* s_empty = bars + 34;         // [2]
+  uint64_t* p_ready = bars + 36;         // [2]
+  uint64_t* p_free = bars + 38;          // [2]
+  uint64_t* q_full = bars + 40;          // [2]
+  uint64_t* q_empty = bars + 42;         // [2]
+  uint64_t* o_done = bars + 44;          // a phase per tile
+  uint64_t* o_final = bars + 45;         // a phase per item
+  uint64_t* f_full = bars + 46;          // [kFactors] factors, and q_full for those who may come two items late
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 46 + kFactors);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* ok_slot = abort_flag + 1;                    // [4]
+  int* s_last = const_cast<int*>(abort_flag) + 5;
+  uint32_t* sValid = tmem_slot + 8;                          // [16] boxes of a K slot that were read
+  uint32_t* sOdd = sValid + 16;                              // [16] heads of 64: 1 + the row of a K slot whose second key is behind the end
+  float* sFactor = reinterpret_cast<float*>(sOdd + 16);    // [kFactors][16]
+  float* sMax = sFactor + kFactors * kRows;                  // [4 warps][17]
+  float* sSum = sMax + 4 * 17;                               // [4][16]
+  float* sInv = sSum + 4 * kRows;                            // [16]
+  float* sW = sInv + kRows;                                  // [32][16]
+  int* sScan = reinterpret_cast<int*>(sW);                   // [8] (before the first item)
+  float* sHalf = sW + 32 * kRows;                            // [16][64] (heads of 64)
+  int* sPre = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(bars) + L::kMisc);   // [B + 1]
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  Abort ab{p.status, abort_flag};
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int s = 0; s < ns; ++s) { mbar_init(&kv_full[s], 1); mbar_init(&kv_empty[s], 5); }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&s_full[b], 1); mbar_init(&s_empty[b], 4);
+      mbar_init(&p_ready[b], 4); mbar_init(&p_free[b], 1);
+      mbar_init(&q_full[b], 1); mbar_init(&q_empty[b], 1);
+    }
+    for (int b = 0; b < kFactors; ++b) mbar_init(&f_full[b], 1);
+    mbar_init(o_done, 1);
+    mbar_init(o_final, 1);
+    mbar_fence_init();
+    prefetch_tmap(&tm);
+    griddep_launch();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, L::kTmem);
+    tmem_relinquish();
+  }
+  // columns of queries and weights that no row uses, and the halves of heads of 64, stay zero
+  for (int c = threadIdx.x; c < (2 * L::kQ + 2 * L::kP) / 16; c += kThreads) reinterpret_cast<uint4*>(sQ)[c] = make_uint4(0, 0, 0, 0);
+  fence_proxy_async_smem();
+
+  // With early_meta lengths and block tables were written long before this launch, and old tokens' rows as well: both are read before
+  // the wait for the kernels in front.
+  if (!p.early_meta) griddep_wait();
+  {
+    // tiles of every request, summed up over those in front: a thread has consecutive requests
+    const int per = (p.B + kThreads - 1) / kThreads, lo = min(p.B, (int)threadIdx.x * per), hi = min(p.B, lo + per);
+    int sum = 0;
+    for (int r = lo; r < hi; ++r) {
+      const Request q = request_of<D>(p, r);
+      const bool served = q.q_len > 0 && q.q_len * (p.Hq / p.Hkv) <= NR;
+      // a request whose rows see nothing has a tile all the same: it writes their zeros
+      const int n = served ? max(1, (q.seq_len - q.kv_begin + kKeys - 1) / kKeys) : 0;
+      sPre[r + 1] = n;
+      sum += n;
+    }
+    int incl = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    if (lane == 31) sScan[warp] = incl;
+    __syncthreads();
+    int base = incl - sum;
+    for (int w = 0; w < warp; ++w) base += sScan[w];
+    for (int r = lo; r < hi; ++r) { base += sPre[r + 1]; sPre[r + 1] = base; }
+    if (threadIdx.x == 0) sPre[0] = 0;
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+
+  const int g = p.Hq / p.Hkv;
+  const long long units = (long long)sPre[p.B] * p.Hkv;
+  const long long share = max((units + gridDim.x - 1) / gridDim.x, (long long)p.min_tiles);
+  const long long lo = min(units, share * blockIdx.x), hi = min(units, lo + share);
+  const int n_tiles = (int)(hi - lo);
+  Walk it;
+  it.start(sPre, p.B, p.Hkv, lo, hi);
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ TMA producer: lane b = box b of the tile
+    const int page_rows = p.block_size / kPack;
+    const int box = page_rows & -page_rows, R = min(kM, box), boxes = kM / R;      // power of two rows a box; the host's map agrees
+    const int64_t page_bytes = (int64_t)p.block_size * (D + 4);
+    int slot = 0, issued = 0;
+    uint32_t phase = 0;
+    bool ok = true, waited = !p.early_meta;
+    for (; ok && it.more(); it.next()) {
+      const Request r = request_of<D>(p, it.req);
+      const int* bt = p.block_tables + (int64_t)it.req * p.bt_stride;
+      auto lookup = [&](int i) -> int {      // block of this lane's box in tile i, -1: nothing to read
+        const int key = r.kv_begin + i * kKeys + lane * R * kPack;
+        if (lane >= boxes || key >= r.seq_len) return -1;
+        const int bi = key / p.block_size;
+        const int blk = bi < p.max_blocks ? bt[bi] : -1;
+        return blk >= 0 && blk < p.num_blocks ? blk : -1;
+      };
+      int blk = lookup(it.tile);
+      for (int i = it.tile; ok && i < it.tile + it.count; ++i) {
+        const int key0 = r.kv_begin + i * kKeys;
+        const int after = i + 1 < it.tile + it.count ? lookup(i + 1) : -1;
+        if (!waited && (issued >= ns || key0 + kKeys > r.ctx)) {   // rows of this step come from the kernels in front
+          griddep_wait();
+          waited = true;
+        }
+        const uint32_t valid = __ballot_sync(0xffffffffu, blk >= 0);
+        const int row = ((key0 + lane * R * kPack) % p.block_size) / kPack;
+        const int64_t page = ((int64_t)max(blk, 0) * 2) * p.Hkv + it.head;
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          if (issued >= ns) {
+            if (lane == 0) ok = wait_or_abort(&kv_empty[slot], phase ^ 1, ab, 901);
+            ok = __shfl_sync(0xffffffffu, ok, 0);
+            if (!ok) break;
+          }
+          if (lane == 0) {
+            if (w == 0) {
+              sValid[slot] = valid;
+              const int left = r.seq_len - key0;
+              if (kPack == 2) sOdd[slot] = left > 0 && left < kKeys && (left & 1) ? 1 + left / 2 : 0;
+            }
+            mbar_expect_tx(&kv_full[slot], __popc(valid) * (R * 128 * kBlk + R * kPack * 4));
+          }
+          __syncwarp();
+          if (blk >= 0) {
+            const int64_t pg = page + (int64_t)w * p.Hkv;
+#pragma unroll
+            for (int b = 0; b < kBlk; ++b)
+              tma_load_3d(smem + slot * G::kOp + b * (kM * 128) + lane * R * 128, &tm, &kv_full[slot], b * 128, row, (int)pg);
+            bulk_load_1d(sScale + slot * kKeys + lane * R * kPack,
+                         p.cache + pg * page_bytes + (int64_t)p.block_size * D + row * kPack * 4, R * kPack * 4, &kv_full[slot]);
+          }
+          ++issued;
+          if (++slot == ns) { slot = 0; phase ^= 1; }
+        }
+        blk = after;
+      }
+    }
+    if (!ok && lane == 0) {     // let the copies in flight land before the CTA's shared memory goes away (bounded)
+      const int pending = min(issued, ns);
+      for (int i = 0; i < pending; ++i) {
+        const int s = (slot - 1 - i + 2 * ns) % ns;
+        const uint32_t ph = s < slot ? phase : phase ^ 1;
+        for (uint32_t k = 0; k < (1u << 16); ++k)
+          if (mbar_try_wait(&kv_full[s], ph)) break;
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issuer
+    if (elect_one() && n_tiles > 0) {
+      constexpr uint32_t idesc_s = umma_idesc(kM, kNS, 0, 0, 0, 0);     // A = K (K-major), B = Q^T (K-major)
+      constexpr uint32_t idesc_o = umma_idesc(kM, kNO, 0, 0, 1, 0);     // A = V (MN-major), B = P (K-major)
+      const uint32_t tS = tmem_base, tO = tmem_base + 2 * kNS;
+      const uint32_t q_addr = smem_u32(sQ), p_addr = smem_u32(sP), kv_addr = smem_u32(smem);
+      // S of the next tile and P.V of the current one are independent: whichever is ready is issued
+      Walk ws = it, wp = it;
+      int s_in = 0, p_in = 0, s_item = 0;            // tiles of the current item issued; items begun
+      int ks = 0, vs = 1 % ns;                       // slots of the next K and V
+      uint32_t kph = 0, vph = 1 / ns;
+      int next_s = 0, next_pv = 0;
+      uint32_t spins = 0;
+      while (next_pv < n_tiles) {
+        bool progressed = false;
+        if (next_s < n_tiles && next_s <= next_pv + 1 && (s_in > 0 || mbar_try_wait(&q_full[s_item & 1], (s_item >> 1) & 1)) &&
+            mbar_try_wait(&kv_full[ks], kph) &&
+            (next_s < 2 || mbar_try_wait(&s_empty[next_s & 1], ((next_s >> 1) - 1) & 1))) {
+          tc_fence_after_sync();
+          if (kPack == 2 && sOdd[ks] != 0) {
+            // this key's codes were not written and meet zeros of Q^T in its neighbour's scores, which do not hide a NaN
+            const int row = (int)sOdd[ks] - 1;
+#pragma unroll
+            for (int c = 4; c < 8; ++c)
+              *reinterpret_cast<uint4*>(smem + ks * G::kOp + row * 128 + ((c ^ (row & 7)) << 4)) = make_uint4(0, 0, 0, 0);
+            fence_proxy_async_smem();
+          }
+          const uint32_t k_at = kv_addr + ks * G::kOp, q_at = q_addr + (s_item & 1) * L::kQ;
+#pragma unroll
+          for (int c = 0; c < P * kBlk * 4; ++c) {
+            const int piece = c / (kBlk * 4), b = (c / 4) % kBlk, k = c % 4;
+            umma_f8(tS + (next_s & 1) * kNS, umma_desc_k_sw128(k_at + b * (kM * 128) + k * 32),
+                    umma_desc_k_sw128(q_at + (piece * kBlk + b) * (kNS * 128) + k * 32), idesc_s, c > 0 ? 1u : 0u);
+          }
+          umma_commit(&s_full[next_s & 1]);
+          umma_commit(&kv_empty[ks]);
+          ks += 2;
+          if (ks >= ns) { ks -= ns; kph ^= 1; }
+          ++next_s;
+          if (++s_in == ws.count) {
+            umma_commit(&q_empty[s_item & 1]);
+            s_in = 0;
+            ++s_item;
+            ws.next();
+          }
+          progressed = true;
+        }
+        if (next_pv < next_s && mbar_try_wait(&p_ready[next_pv & 1], (next_pv >> 1) & 1) && mbar_try_wait(&kv_full[vs], vph)) {
+          tc_fence_after_sync();
+          const uint32_t v_at = kv_addr + vs * G::kOp, w_at = p_addr + (next_pv & 1) * L::kP;
+#pragma unroll
+          for (int b = 0; b < kBlk; ++b) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)       // 32 rows: four groups of eight, 1024 bytes apart
+              umma_f8(tO + b * kNO, umma_desc_mn_sw128(v_at + b * (kM * 128) + k * 4096, 1024, 1024),
+                      umma_desc_k_sw128(w_at + k * 32), idesc_o, (p_in > 0 || k > 0) ? 1u : 0u);
+          }
+          // o_done first: whoever has seen p_free of this tile may rely on o_done having advanced as well
+          umma_commit(o_done);
+          umma_commit(&kv_empty[vs]);
+          umma_commit(&p_free[next_pv & 1]);
+          vs += 2;
+          if (vs >= ns) { vs -= ns; vph ^= 1; }
+          ++next_pv;
+          if (++p_in == wp.count) {
+            umma_commit(o_final);
+            p_in = 0;
+            wp.next();
+          }
+          progressed = true;
+        }
+        if (progressed) { spins = 0; continue; }
+        if (++spins > (1u << 20)) { ab.raise(902); break; }
+        if ((spins & 255) == 255 && ab.aborted()) break;
+      }
+    }
+  } else if (warp == 6) {
+    // ------------------------------------------------------------------ queries in pieces
+    if (p.early_meta) griddep_wait();
+    constexpr int kLanes = D / 8, kPass = 32 / kLanes;      // lanes of a row, rows at a time
+    const int sub = lane / kLanes, l = lane % kLanes, d = l * 8;
+    bool ok = true;
+    for (int item = 0; ok && it.more(); it.next(), ++item) {
+      const Request r = request_of<D>(p, it.req);
+      const int rows = r.q_len * g;
+      if (item >= 2) {
+        if (lane == 0) ok = wait_or_abort(&q_empty[item & 1], ((item >> 1) - 1) & 1, ab, 903);
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (!ok) break;
+      }
+      uint8_t* dst = sQ + (item & 1) * L::kQ;
+#pragma unroll 4
+      for (int r0 = 0; r0 < NR; r0 += kPass) {
+        const int row = r0 + sub;
+        const bool in = row < rows;
+        float v[8];
+        float amax = 0.f;
+        bool bad = false;
+        if (in) {
+          const int tok = r.qs + row / g, hh = it.head * g + row % g;
+          const Vec16<T> a = ld_vec(reinterpret_cast<const T*>(p.q) + tok * p.q_stride + (int64_t)hh * D + d);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            v[j] = to_f(a.v[j]);
+            bad |= (__float_as_uint(v[j]) & 0x7f800000u) == 0x7f800000u;
+            amax = fmaxf(amax, fabsf(v[j]));
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = 0.f;
+        }
+#pragma unroll
+        for (int o = kLanes / 2; o > 0; o >>= 1) {
+          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+          bad |= __shfl_xor_sync(0xffffffffu, (int)bad, o) != 0;
+        }
+        const float top = bad ? 1.f : pow2_ceil(fmaxf(amax, 1e-30f));
+        const float up = bad ? 0.f : 256.f * pow2_inv(top);
+        if (l == 0) sFactor[(item % kFactors) * kRows + row] = bad ? __uint_as_float(0x7fffffffu) : top * (1.f / 256.f) * p.scale_log2;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = bad ? 0.f : v[j] * up;
+#pragma unroll
+        for (int c = 0; c < P; ++c) {
+          const uint2 w = kv8_pack8(v, 1.f);
+          if (c + 1 < P) {
+            const uint32_t x[2] = {w.x, w.y};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float2 f = e4m3x2_to_float2((uint16_t)(x[j / 2] >> (16 * (j & 1))));
+              v[2 * j] -= f.x;
+              v[2 * j + 1] -= f.y;
+            }
+          }
+#pragma unroll
+          for (int q2 = 0; q2 < kPack; ++q2) {
+            const int rr = q2 * kRows + row, byte = kPack == 2 ? q2 * 64 + d : d & 127;
+            uint8_t* at = dst + ((c * kBlk + (kBlk == 2 ? d >> 7 : 0)) * kNS + rr) * 128 + (((byte >> 4) ^ (rr & 7)) << 4) + (byte & 15);
+            *reinterpret_cast<uint2*>(at) = w;
+          }
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&q_full[item & 1]);
+        mbar_arrive(&f_full[item % kFactors]);
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ softmax + epilogue (warps 2..5)
+    if (p.early_meta) griddep_wait();
+    const int quarter = warp & 3, tid = (warp - 2) * 32 + lane;
+    const int row_id = quarter * 32 + lane;          // TMEM lane: row of the tile, output dim
+    const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
+    const uint32_t tS = tmem_base + lane_off, tO = tmem_base + 2 * kNS + lane_off;
+    const uint32_t inv_g = 65536u / g + 1;           // r / g = r * inv_g >> 16 for r < 16
+    const int page_rows = p.block_size / kPack, box_rows = min(kM, page_rows & -page_rows);
+    const uint32_t all_boxes = kM / box_rows == 32 ? 0xffffffffu : (1u << (kM / box_rows)) - 1;
+    const int my_box = row_id / box_rows;
+    const int p_off = row_id & 15, p_ch = row_id >> 4;
+    int t = 0;                                       // tiles so far
+    int slot = 0;
+    uint32_t phase = 0;
+    bool ok = true, fail = false;
+    for (int item = 0; it.more(); it.next(), ++item) {
+      const Request r = request_of<D>(p, it.req);
+      const int rows = r.q_len * g, pos_max = r.ctx + r.q_len - 1;
+      float m_used[NR], l_part[NR], vref = 0.f;
+#pragma unroll
+      for (int i = 0; i < NR; ++i) { m_used[i] = -INFINITY; l_part[i] = 0.f; }
+      if (ok && !wait_or_abort(&f_full[item % kFactors], (item / kFactors) & 1, ab, 909)) fail = true;
+      const float* factor = sFactor + (item % kFactors) * kRows;
+      for (int i = it.tile; ok && i < it.tile + it.count; ++i, ++t) {
+        const int buf = t & 1;
+        const int kslot = slot, vslot = slot + 1 == ns ? 0 : slot + 1;
+        const uint32_t vphase = slot + 1 == ns ? phase ^ 1 : phase;
+        if (!fail && !wait_or_abort(&s_full[buf], (t >> 1) & 1, ab, 905)) fail = true;
+        // weight buffer t & 1 is free (P.V of tile t - 2).  Waiting here, before a possible rescale, also keeps o_done at most one phase
+        // behind, so that the parity wait on it below cannot pass two phases early.
+        if (t >= 2 && !fail && !wait_or_abort(&p_free[buf], ((t >> 1) - 1) & 1, ab, 906)) fail = true;
+        if (!fail && !wait_or_abort(&kv_full[kslot], phase, ab, 904)) fail = true;
+        if (!fail && !wait_or_abort(&kv_full[vslot], vphase, ab, 904)) fail = true;
+        slot += 2;
+        if (slot >= ns) { slot -= ns; phase ^= 1; }
+        tc_fence_after_sync();
+        uint32_t sr[kNS];
+        tmem_ld_cols(tS + buf * kNS, sr);
+        float kscale[kPack], vscale[kPack];
+        if constexpr (kPack == 2) {
+          const float2 a = reinterpret_cast<const float2*>(sScale + kslot * kKeys)[row_id];
+          const float2 b = reinterpret_cast<const float2*>(sScale + vslot * kKeys)[row_id];
+          kscale[0] = a.x; kscale[kPack - 1] = a.y; vscale[0] = b.x; vscale[kPack - 1] = b.y;
+        } else {
+          kscale[0] = sScale[kslot * kKeys + row_id];
+          vscale[0] = sScale[vslot * kKeys + row_id];
+        }
+        const uint32_t valid = sValid[kslot];
+        tmem_ld_wait();
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&s_empty[buf]);
+          mbar_arrive(&kv_empty[kslot]);
+          mbar_arrive(&kv_empty[vslot]);
+        }
+        const int key0 = r.kv_begin + i * kKeys;
+        const bool whole = key0 + kKeys <= r.seq_len && (valid & all_boxes) == all_boxes;
+        const bool full = whole && key0 + kKeys - 1 <= r.ctx && (p.window <= 0 || key0 > pos_max - p.window);
+        float sc[kPack][NR];
+        bool need = fail;
+#pragma unroll
+        for (int q2 = 0; q2 < kPack; ++q2) {
+          const int key = key0 + row_id * kPack + q2;
+          const bool there = whole || (key < r.seq_len && (valid >> my_box & 1));
+          if (!there) {
+            vscale[q2] = 0.f;
+            // codes of rows that were not read, or not written, may be anything: zeros, since a weight of zero does not hide a NaN
+            uint8_t* v = smem + vslot * G::kOp + row_id * 128;
+#pragma unroll
+            for (int c = 0; c < 8 / kPack; ++c) {
+#pragma unroll
+              for (int b = 0; b < kBlk; ++b)
+                *reinterpret_cast<uint4*>(v + b * (kM * 128) + (((kPack == 2 ? q2 * 4 + c : c) ^ (row_id & 7)) << 4)) = make_uint4(0, 0, 0, 0);
+            }
+          }
+          need |= vscale[q2] > vref;
+#pragma unroll
+          for (int n = 0; n < NR; ++n) {
+            float v = __uint_as_float(sr[q2 * kRows + n]) * (kscale[q2] * factor[n]);
+            if (!full) {
+              const int pos = n < rows ? r.ctx + (int)((n * inv_g) >> 16) : -1;
+              v = there && key <= pos && (p.window <= 0 || key > pos - p.window) ? v : -INFINITY;
+            } else if (NR > 4 && n >= rows) {
+              v = -INFINITY;
+            }
+            sc[q2][n] = v;
+            need |= v > m_used[n] + kSlack;
+          }
+        }
+        if (bar_red_or(1, 128, need)) {
+          // ---- rare after the first tiles: move the reference maxima and the reference scale, rescale O^T
+#pragma unroll
+          for (int n = 0; n < NR; ++n) {
+            const float wm = warp_max_redux(kPack == 2 ? fmaxf(sc[0][n], sc[kPack - 1][n]) : sc[0][n]);
+            if (lane == n) sMax[quarter * 17 + n] = wm;
+          }
+          {
+            float vm = 0.f;
+#pragma unroll
+            for (int q2 = 0; q2 < kPack; ++q2) vm = fmaxf(vm, is_nan_bits(vscale[q2]) ? 0.f : vscale[q2]);
+            vm = warp_max_redux(vm);
+            if (lane == 16) sMax[quarter * 17 + 16] = vm;
+          }
+          const bool warp_failed = __any_sync(0xffffffffu, fail);
+          if (lane == 0) ok_slot[quarter] = warp_failed ? 0 : 1;
+          named_bar_sync(1, 128);
+          if ((ok_slot[0] & ok_slot[1] & ok_slot[2] & ok_slot[3]) == 0) { ok = false; break; }
+          auto over = [&](int n) { return fmaxf(fmaxf(sMax[n], sMax[17 + n]), fmaxf(sMax[34 + n], sMax[51 + n])); };
+          const float vm = over(16);
+          const float back = vm > vref ? (vref > 0.f ? vref * pow2_inv(vm) : 0.f) : 1.f;
+          vref = fmaxf(vref, vm);
+          float alpha[NR];
+          bool rescale = back != 1.f;
+#pragma unroll
+          for (int n = 0; n < NR; ++n) {
+            const float top = over(n);
+            alpha[n] = 1.f;
+            if (top > m_used[n] + kSlack) {            // also the first finite maximum (m_used = -inf)
+              alpha[n] = exp2f(m_used[n] - top);       // exp2(-inf) = 0: nothing accumulated yet
+              m_used[n] = top;
+              l_part[n] *= alpha[n];
+              rescale = true;
+            }
+            alpha[n] *= back;
+          }
+          if (rescale && i > it.tile) {    // the same decision in every thread: all of them read the same maxima
+            if (!wait_or_abort(o_done, (t - 1) & 1, ab, 908)) fail = true;
+            tc_fence_after_sync();
+#pragma unroll
+            for (int c = 0; c < kBlk * kNO; c += 16) {
+              uint32_t o[16];
+              tmem_ld_x16(tO + c, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int n = 0; n < NR; ++n) o[n] = __float_as_uint(__uint_as_float(o[n]) * alpha[n]);
+              tmem_st_x16(tO + c, o);
+            }
+            tmem_st_wait();
+          }
+          named_bar_sync(1, 128);          // sMax has been read
+        }
+        const float to_ref = vref > 0.f ? pow2_inv(vref) : 0.f;
+        if (!fail) {
+          uint8_t* wbuf = sP + buf * L::kP + p_off;
+#pragma unroll
+          for (int q2 = 0; q2 < kPack; ++q2) {
+            const float vs = vscale[q2] * to_ref;
+#pragma unroll
+            for (int n = 0; n < NR; n += 2) {
+              float w[2];
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const float m = m_used[n + e] == -INFINITY ? 0.f : m_used[n + e];
+                const float x = exp2f(sc[q2][n + e] - m + kLift);
+                l_part[n + e] += x;
+                w[e] = x > 0.f ? x * vs : x;         // a masked key's scale may be a NaN
+              }
+              __half2 rest = __floats2half2_rn(w[0], w[1]);
+#pragma unroll
+              for (int c = 0; c < P; ++c) {
+                const uint16_t code = f16x2_to_e4m3x2(rest);
+                const int rr = (c * kPack + q2) * kRows + n;
+                wbuf[rr * 128 + ((p_ch ^ (rr & 7)) << 4)] = (uint8_t)code;
+                wbuf[(rr + 1) * 128 + ((p_ch ^ ((rr + 1) & 7)) << 4)] = (uint8_t)(code >> 8);
+                if (c + 1 < P) rest = __hmul2(__hsub2(rest, as_half2(e4m3x2_to_f16x2(code))), __float2half2_rn(32.f));
+              }
+            }
+          }
+        }
+        fence_proxy_async_smem();
+        tc_fence_before_sync();
+        const bool warp_failed = __any_sync(0xffffffffu, fail);
+        __syncwarp();
+        if (lane == 0 && !warp_failed) mbar_arrive(&p_ready[buf]);
+      }
+      if (fail) ok = false;
+      // ---- epilogue: O^T lane = output dim, columns = query rows of every piece
+      if (ok && !wait_or_abort(o_final, item & 1, ab, 907)) ok = false;
+      tc_fence_after_sync();
+      ok = bar_red_or(1, 128, !ok) == 0;   // one thread's time-out ends the work of all
+      const long long first = (long long)sPre[it.req] * p.Hkv + (long long)it.head * it.n, last = first + it.n - 1;
+      const int c0 = (int)(first / share), c1 = (int)(last / share);     // the CTAs that have tiles of this item
+      const bool partial = c0 != c1;
+      const int64_t my_slot = 2 * (int64_t)blockIdx.x + ((long long)blockIdx.x * share >= first ? 0 : 1);
+#pragma unroll
+      for (int n = 0; n < NR; ++n) {
+        float v = l_part[n];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        if (lane == n) sSum[quarter * kRows + n] = v;
+      }
+      named_bar_sync(1, 128);
+      if (tid < NR) {
+        float m = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < NR; ++n) m = tid == n ? m_used[n] : m;
+        const float sum = sSum[tid] + sSum[kRows + tid] + sSum[2 * kRows + tid] + sSum[3 * kRows + tid];
+        const float ms = m == -INFINITY ? 0.f : m;
+        float den = sum;
+        if (!partial && p.sinks != nullptr && tid < rows)
+          den += exp2f(p.sinks[it.head * g + ((int)tid - (int)((tid * inv_g) >> 16) * g)] * kLog2e - ms + kLift);
+        // vref comes with the weights' scale; a row that saw nothing gives zeros, a NaN stays one
+        sInv[tid] = !ok || den == 0.f ? 0.f : vref / den;
+        if (partial) p.ws_lse[my_slot * kRows + tid] = !ok || sum == 0.f ? -INFINITY : ms + log2f(sum) - kLift;
+      }
+      named_bar_sync(1, 128);
+      // this thread's output dims of every row: pieces summed, both quadrants for heads of 64
+      float o_mine[kBlk][NR];
+      if (ok) {
+#pragma unroll
+        for (int b = 0; b < kBlk; ++b) {
+          float part[NR];
+#pragma unroll
+          for (int c = 0; c < P; ++c) {
+            uint32_t o[16];
+            tmem_ld_x16(tO + b * kNO + (c * kPack + (kPack == 2 ? row_id >> 6 : 0)) * kRows, o);
+            tmem_ld_wait();
+            const float unit = c == 0 ? 1.f : c == 1 ? 1.f / 32.f : 1.f / 1024.f;
+#pragma unroll
+            for (int n = 0; n < NR; ++n) part[n] = c == 0 ? __uint_as_float(o[n]) : part[n] + __uint_as_float(o[n]) * unit;
+          }
+#pragma unroll
+          for (int n = 0; n < NR; ++n) o_mine[b][n] = part[n];
+        }
+      } else {
+#pragma unroll
+        for (int b = 0; b < kBlk; ++b)
+#pragma unroll
+          for (int n = 0; n < NR; ++n) o_mine[b][n] = 0.f;
+      }
+      if constexpr (kPack == 2) {
+        if (row_id >= 64) {
+#pragma unroll
+          for (int n = 0; n < NR; ++n) sHalf[n * 64 + row_id - 64] = o_mine[0][n];
+        }
+        named_bar_sync(1, 128);
+        if (row_id < 64) {
+#pragma unroll
+          for (int n = 0; n < NR; ++n) o_mine[0][n] += sHalf[n * 64 + row_id];
+        }
+      }
+      auto out_row = [&](int n) {
+        const int tok = (int)((n * inv_g) >> 16);
+        return ((int64_t)(r.qs + tok) * p.Hq + it.head * g + (n - tok * g)) * D;
+      };
+      if (kPack == 1 || row_id < 64) {
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+          const float inv = sInv[n];
+#pragma unroll
+          for (int b = 0; b < kBlk; ++b) {
+            const float v = inv == 0.f ? 0.f : o_mine[b][n] * inv;
+            if (n < rows) {
+              if (partial) p.ws_o[(my_slot * kRows + n) * D + b * 128 + row_id] = v;
+              else reinterpret_cast<T*>(p.out)[out_row(n) + b * 128 + row_id] = from_f<T>(v);
+            }
+          }
+        }
+      }
+      if (partial) {
+        // ---- the last CTA of the item to arrive merges
+        __threadfence();
+        named_bar_sync(1, 128);
+        int* ticket = p.tickets + (int64_t)it.req * p.Hkv + it.head;
+        if (tid == 0) *s_last = atomicAdd(ticket, 1) == c1 - c0;
+        named_bar_sync(1, 128);
+        if (*s_last) {
+          __threadfence();
+          auto slot_of = [&](int c) { return 2 * (int64_t)c + ((long long)c * share >= first ? 0 : 1); };
+          const int n_parts = c1 - c0 + 1;
+          // row tid % 16: largest log-sum-exp and the sum, eight threads a row
+          {
+            const int n = tid & 15;
+            float M = -INFINITY, S = 0.f;
+            for (int c = tid >> 4; c < n_parts; c += 8) {
+              const float v = n < rows ? __ldcg(p.ws_lse + slot_of(c0 + c) * kRows + n) : -INFINITY;
+              if (v != -INFINITY) {
+                const float top = fmaxf(M, v);
+                S = S * exp2f(M - top) + exp2f(v - top);
+                M = top;
+              }
+            }
+            sW[tid] = M;
+            sW[128 + tid] = S;
+          }
+          named_bar_sync(1, 128);
+          if (tid < kRows) {
+            float M = -INFINITY, S = 0.f;
+            for (int c = 0; c < 8; ++c) M = fmaxf(M, sW[c * 16 + tid]);
+            const float Ms = M == -INFINITY ? 0.f : M;
+            for (int c = 0; c < 8; ++c) {
+              const float s = sW[128 + c * 16 + tid], mm = sW[c * 16 + tid];
+              S += is_nan_bits(s) ? s : s * exp2f(mm - Ms);
+            }
+            if (p.sinks != nullptr && tid < rows)
+              S += exp2f(p.sinks[it.head * g + ((int)tid - (int)((tid * inv_g) >> 16) * g)] * kLog2e - Ms);
+            sMax[tid] = Ms;
+            sInv[tid] = S == 0.f ? 0.f : 1.f / S;
+          }
+          named_bar_sync(1, 128);
+          float acc[kBlk][NR];
+#pragma unroll
+          for (int b = 0; b < kBlk; ++b)
+#pragma unroll
+            for (int n = 0; n < NR; ++n) acc[b][n] = 0.f;
+          for (int base = 0; base < n_parts; base += 32) {
+            const int cnt = min(32, n_parts - base);
+            for (int x = tid; x < cnt * kRows; x += 128) {
+              const int n = x & 15;
+              const float v = n < rows ? __ldcg(p.ws_lse + slot_of(c0 + base + (x >> 4)) * kRows + n) : -INFINITY;
+              sW[x] = v == -INFINITY ? 0.f : exp2f(v - sMax[n]) * sInv[n];
+            }
+            named_bar_sync(1, 128);
+            if (kPack == 1 || row_id < 64) {
+              for (int c = 0; c < cnt; ++c) {
+                const float* src = p.ws_o + slot_of(c0 + base + c) * kRows * D + row_id;
+#pragma unroll
+                for (int n = 0; n < NR; ++n) {
+                  if (n < rows) {
+                    const float w = sW[c * kRows + n];
+#pragma unroll
+                    for (int b = 0; b < kBlk; ++b) {
+                      const float v = __ldcg(src + n * D + b * 128);
+                      acc[b][n] += w == 0.f ? 0.f : v * w;
+                    }
+                  }
+                }
+              }
+            }
+            named_bar_sync(1, 128);
+          }
+          if (kPack == 1 || row_id < 64) {
+#pragma unroll
+            for (int n = 0; n < NR; ++n)
+              if (n < rows) {
+#pragma unroll
+                for (int b = 0; b < kBlk; ++b) reinterpret_cast<T*>(p.out)[out_row(n) + b * 128 + row_id] = from_f<T>(acc[b][n]);
+              }
+          }
+          if (tid == 0) *ticket = 0;
+        }
+      }
+      named_bar_sync(1, 128);              // the exchange buffers are free for the next item
+    }
+  }
+
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, L::kTmem);
+  }
+}
+
+template <typename T, int D, int NR>
+static int launch_nr(Params p, const CUtensorMap& tm, int grid, int slots, cudaStream_t st) {
+  auto kern = kv8_decode_kernel<T, D, NR>;
+  p.slots = slots;
+  const size_t smem = Layout<T, D>::smem(slots, p.B);
+  cudaError_t e = ensure_dynamic_smem((const void*)kern, (int)smem);
+  if (e != cudaSuccess) return (int)e;
+  return (int)launch_pdl(kern, dim3(grid), dim3(kThreads), smem, st, tm, p);
+}
+
+template <typename T, int D>
+static int launch(const Params& p0, const CUtensorMap& tm, int B, int max_rows, int num_sms, int64_t max_tiles, cudaStream_t st) {
+  Params p = p0;
+  for (int b0 = 0; b0 < B; b0 += kMaxB) {
+    p.B = B - b0 < kMaxB ? B - b0 : kMaxB;
+    p.block_tables = p0.block_tables + (int64_t)b0 * p.bt_stride;
+    p.seq_lens = p0.seq_lens + b0;
+    p.qsl = p0.qsl + b0;
+    p.tickets = p0.tickets + (int64_t)b0 * p.Hkv;
+    // two CTAs an SM where four operand slots each fit, otherwise one with as many as fit
+    int ctas = 2, slots = 6;
+    while (slots > 4 && Layout<T, D>::smem(slots, p.B) > 113 * 1024) --slots;
+    if (Layout<T, D>::smem(slots, p.B) > 113 * 1024) {
+      ctas = 1;
+      slots = 10;
+      while (slots > 4 && Layout<T, D>::smem(slots, p.B) > 226 * 1024) --slots;
+    }
+    const int64_t units = (int64_t)p.B * p.Hkv * (max_tiles < 1 ? 1 : max_tiles);
+    int grid = num_sms * ctas;
+    if (units < grid) grid = (int)units;
+    int rc;
+    if (max_rows <= 4) rc = launch_nr<T, D, 4>(p, tm, grid, slots, st);
+    else if (max_rows <= 8) rc = launch_nr<T, D, 8>(p, tm, grid, slots, st);
+    else rc = launch_nr<T, D, 16>(p, tm, grid, slots, st);
+    if (rc != 0) return rc;
+  }
+  return 0;
+}
+
+}  // namespace kv8dec
+}  // namespace b200
+
+// `tmap`: the codes as written by b200_encode_tmap_kv8.  ws_o: 2 * 2 * num_sms * 16 * D floats, ws_lse: 2 * 2 * num_sms * 16, tickets: B * Hkv zeros (zeros again on return).
+// Requests with more than max_query_len queries are left out.  Returns 3 for shapes it does not serve.
+extern "C" int b200_kv8_decode(void* out, const void* q, const void* cache, const void* tmap, const int* block_tables,
+                               const int* seq_lens, const int* qsl, const float* sinks, float* ws_o, float* ws_lse, int* tickets,
+                               int* status, int B, int Hq, int Hkv, int D, int block_size, int max_blocks, int64_t bt_stride,
+                               int64_t num_blocks, int max_query_len, int64_t max_seq_len, int window, float scale, int64_t q_stride,
+                               int early_meta, int dtype, int num_sms, cudaStream_t st) {
+  using namespace b200;
+  if (B == 0) return 0;
+  if (Hq % Hkv || max_query_len < 1 || (int64_t)max_query_len * (Hq / Hkv) > kv8dec::kRows || block_size % 16 ||
+      (D != 64 && D != 128 && D != 256) || (dtype != kBF16 && dtype != kF16) || num_blocks * 2 * Hkv > 0x7fffffff || q_stride % 8 ||
+      (reinterpret_cast<uintptr_t>(q) & 15) || window < 0 || num_sms < 1)
+    return 3;
+  kv8dec::Params p = {};
+  p.q = q; p.out = out; p.cache = static_cast<const uint8_t*>(cache); p.ws_o = ws_o; p.ws_lse = ws_lse; p.tickets = tickets;
+  p.block_tables = block_tables; p.seq_lens = seq_lens; p.qsl = qsl; p.sinks = sinks; p.status = status;
+  p.num_blocks = num_blocks; p.bt_stride = bt_stride; p.q_stride = q_stride; p.Hq = Hq; p.Hkv = Hkv; p.block_size = block_size;
+  p.max_blocks = max_blocks; p.window = window; p.early_meta = early_meta; p.min_tiles = 1;
+  p.scale_log2 = scale * kv8dec::kLog2e;
+  const CUtensorMap& tm = *reinterpret_cast<const CUtensorMap*>(tmap);
+  const int rows = max_query_len * (Hq / Hkv), keys = D == 64 ? 256 : 128;
+  const int64_t span = window > 0 && window + max_query_len < max_seq_len ? window + max_query_len + keys : max_seq_len;
+  const int64_t tiles = (span + keys - 1) / keys;
+#define B200_KV8_DEC(TT, DD) return kv8dec::launch<TT, DD>(p, tm, B, rows, num_sms, tiles, st)
+  if (dtype == kBF16) {
+    if (D == 64) B200_KV8_DEC(__nv_bfloat16, 64);
+    if (D == 128) B200_KV8_DEC(__nv_bfloat16, 128);
+    B200_KV8_DEC(__nv_bfloat16, 256);
+  }
+  if (D == 64) B200_KV8_DEC(__half, 64);
+  if (D == 128) B200_KV8_DEC(__half, 128);
+  B200_KV8_DEC(__half, 256);
+#undef B200_KV8_DEC
+}

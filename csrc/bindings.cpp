@@ -5,11 +5,13 @@
 // an alias of a CUDA tensor that does not own its storage, used to hold CUDA-graph outputs without
 // keeping the allocation alive.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/CUDAGraphsUtils.cuh>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
 #include <limits.h>
 
+#include <algorithm>
 #include <atomic>
 #include <mutex>
 #include <unordered_map>
@@ -1098,6 +1100,75 @@ void check_kv8_attention(const at::Tensor& out, const at::Tensor& q, const at::T
   if (sinks.has_value())
     TORCH_CHECK(sinks->scalar_type() == at::kFloat && sinks->is_contiguous() && sinks->numel() == q.size(1) && sinks->device() == q.device(),
                 "sinks: contiguous fp32 [heads]");
+}
+// Per device: status word (the GEMM module's where that lives on this device), tickets of the decode kernel per stream.
+struct Kv8State {
+  int num_sms = 0;
+  at::Tensor status;
+  std::unordered_map<cudaStream_t, at::Tensor> tickets;
+};
+Kv8State& kv8_state(GemmState& gs, const at::Tensor& like) {      // under gs.mu, with like's device current
+  static std::unordered_map<int, Kv8State> states;
+  Kv8State& s = states[like.device().index()];
+  if (s.num_sms == 0) {
+    s.num_sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+    if (gs.num_sms == 0) {
+      gs.num_sms = s.num_sms;
+      gs.ws = at::empty({16 << 20}, like.options().dtype(at::kFloat));
+      gs.counters = at::zeros({1 << 16}, like.options().dtype(at::kInt));
+      gs.status = at::zeros({1}, like.options().dtype(at::kInt));
+    }
+    s.status = gs.status.device() == like.device() ? gs.status : at::zeros({1}, like.options().dtype(at::kInt));
+  }
+  return s;
+}
+// n zeros that this stream's calls leave as zeros.  A captured call has its own, cleared in the graph: graphs may be replayed side by side.
+at::Tensor kv8_tickets(Kv8State& s, int64_t n, const at::Tensor& like) {
+  const auto options = like.options().dtype(at::kInt);
+  if (at::cuda::currentStreamCaptureStatus() != at::cuda::CaptureStatus::None) return at::zeros({n}, options);
+  at::Tensor& t = s.tickets[stream()];
+  if (!t.defined() || t.numel() < n) t = at::zeros({std::max<int64_t>(n, 4096)}, options);
+  return t;
+}
+Tmap get_tmap_kv8(GemmState& gs, const at::Tensor& cache) {
+  const int64_t pages = cache.size(0) * 2 * cache.size(2);
+  TmapKey key{cache.data_ptr(), pages, cache.size(3), cache.size(4), 0, -1};
+  auto it = gs.cache.find(key);
+  if (it != gs.cache.end()) return it->second;
+  if (gs.cache.size() > 4096) gs.cache.clear();
+  Tmap tm;
+  int rc = b200_encode_tmap_kv8(tm.b, cache.data_ptr(), pages, (int)cache.size(3), (int)cache.size(4) - 4);
+  TORCH_CHECK(rc == 0, "tensor map encode failed: ", rc);
+  return gs.cache.emplace(key, tm).first->second;
+}
+// At most 16 query rows per key / value head; `ws_o`, `ws_lse`, `tickets` (or none of them): scratch of the caller for one stream, the
+// tickets zero at first.
+void kv8_decode(at::Tensor out, const at::Tensor& q, const at::Tensor& cache, const at::Tensor& block_tables,
+                const at::Tensor& seq_lens, const at::Tensor& qsl, const c10::optional<at::Tensor>& sinks,
+                const c10::optional<at::Tensor>& ws_o, const c10::optional<at::Tensor>& ws_lse,
+                const c10::optional<at::Tensor>& tickets, int64_t max_query_len, int64_t max_seq_len, int64_t window, double scale,
+                bool early_meta) {
+  check_kv8_attention(out, q, cache, block_tables, seq_lens, qsl, sinks);
+  if (q.size(0) == 0 || seq_lens.size(0) == 0) return;
+  c10::cuda::CUDAGuard guard(q.device());
+  GemmState& gs = gemm_state();
+  std::lock_guard<std::mutex> lk(gs.mu);
+  Kv8State& s = kv8_state(gs, q);
+  const int64_t B = seq_lens.size(0), Hkv = cache.size(2), D = q.size(2), parts = 4LL * s.num_sms * 16;
+  auto scratch = [&](const c10::optional<at::Tensor>& t, int64_t n) {
+    if (t.has_value() && t->numel() >= n && t->device() == q.device() && t->scalar_type() == at::kFloat) return *t;
+    return at::empty({n}, q.options().dtype(at::kFloat));
+  };
+  const at::Tensor o = scratch(ws_o, parts * D), lse = scratch(ws_lse, parts);
+  const bool own = tickets.has_value() && tickets->numel() >= B * Hkv && tickets->device() == q.device() && tickets->scalar_type() == at::kInt;
+  const at::Tensor tk = own ? *tickets : kv8_tickets(s, B * Hkv, q);
+  const Tmap tm = get_tmap_kv8(gs, cache);
+  check(b200_kv8_decode(out.data_ptr(), q.data_ptr(), cache.data_ptr(), tm.b, block_tables.data_ptr<int>(), seq_lens.data_ptr<int>(),
+                        qsl.data_ptr<int>(), sinks.has_value() ? sinks->data_ptr<float>() : nullptr, o.data_ptr<float>(),
+                        lse.data_ptr<float>(), tk.data_ptr<int>(), s.status.data_ptr<int>(), (int)B, (int)q.size(1), (int)Hkv, (int)D,
+                        (int)cache.size(3), (int)block_tables.size(1), block_tables.stride(0), cache.size(0), (int)max_query_len,
+                        max_seq_len, (int)window, (float)scale, q.stride(0), early_meta ? 1 : 0, dtype_code(q), s.num_sms, stream()),
+        "kv8_decode");
 }
 void kv8_attention_generic(at::Tensor out, const at::Tensor& q, const at::Tensor& cache, const at::Tensor& block_tables,
                            const at::Tensor& seq_lens, const at::Tensor& qsl, const c10::optional<at::Tensor>& sinks, int64_t window,
@@ -2272,6 +2343,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("kv8_qkv", &kv8_qkv);
   m.def("kv_gather", &kv_gather);
   m.def("kv8_attention_generic", &kv8_attention_generic);
+  m.def("kv8_decode", &kv8_decode);
   m.def("concat_and_cache_mla", &concat_and_cache_mla);
   m.def("indexer_k_quant_and_cache", &indexer_k_quant_and_cache);
   m.def("convert_req_index_to_global_index", &convert_req_index_to_global_index);

@@ -31,13 +31,15 @@ def sm_count(device) -> int:
 
 
 class AttnWorkspace:
-    """Split-KV scratch: ``ws_o [splits, T, Hq, D]`` fp32 and ``ws_lse [splits, T, Hq]``."""
+    """Split-KV scratch: ``ws_o [splits, T, Hq, D]`` fp32 and ``ws_lse [splits, T, Hq]``; ``tickets [T, Hq]`` int32, zero between
+    calls, for the 8-bit cache's kernel.  One workspace serves one stream at a time."""
 
     def __init__(self, max_tokens: int, num_heads: int, head_dim: int, max_splits: int, device):
         self.max_splits = max_splits
         self.max_tokens = max_tokens
         self.o = torch.empty(max_splits * max_tokens * num_heads * head_dim, dtype=torch.float32, device=device)
         self.lse = torch.empty(max_splits * max_tokens * num_heads, dtype=torch.float32, device=device)
+        self.tickets = torch.zeros(max_tokens * num_heads, dtype=torch.int32, device=device)
 
 
 def plan_splits(num_reqs: int, num_kv_heads: int, q_tiles: int, max_seq_len: int, device, max_splits: int = 16,

@@ -5,9 +5,15 @@ kernel, the others to the prompt kernel; what neither takes (fp32 models, other 
 """
 from __future__ import annotations
 
+import os
+
 import torch
 
 from . import _ext
+
+# B200_KV8_UMMA=0 keeps every call on the generic kernel
+TENSOR_CORES = [os.environ.get("B200_KV8_UMMA", "1") != "0"]
+DECODE_ROWS = 16                # query rows (heads of a group x query tokens) that the decode kernel takes
 
 
 def paged_attention_kv8(out, q, kv_cache, block_tables, seq_lens, query_start_loc, scale: float, max_query_len: int,
@@ -15,5 +21,25 @@ def paged_attention_kv8(out, q, kv_cache, block_tables, seq_lens, query_start_lo
                         num_decode_tokens: int, stable_metadata: bool):
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    _ext.C().kv8_attention_generic(out, q, kv_cache, block_tables, seq_lens, query_start_loc, sinks, window, scale)
+    n = num_decodes
+    if 0 < n < seq_lens.shape[0]:       # start offsets are absolute: both parts work on the whole q and out
+        _attend(out, q, kv_cache, block_tables[:n], seq_lens[:n], query_start_loc[:n + 1], scale, decode_query_len, max_seq_len,
+                window, sinks, workspace, stable_metadata)
+        _attend(out, q, kv_cache, block_tables[n:], seq_lens[n:], query_start_loc[n:], scale, max_query_len, max_seq_len, window,
+                sinks, workspace, False)
+    else:
+        _attend(out, q, kv_cache, block_tables, seq_lens, query_start_loc, scale, max_query_len, max_seq_len, window, sinks,
+                workspace, stable_metadata)
     return out
+
+
+def _attend(out, q, kv_cache, block_tables, seq_lens, query_start_loc, scale, max_query_len, max_seq_len, window, sinks, workspace,
+            stable_metadata):
+    H, D = q.shape[1], q.shape[2]
+    if (TENSOR_CORES[0] and D in (64, 128, 256) and kv_cache.shape[3] % 16 == 0 and q.dtype != torch.float32
+            and max_query_len * (H // kv_cache.shape[2]) <= DECODE_ROWS and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0):
+        ws = (workspace.o, workspace.lse, workspace.tickets) if workspace is not None else (None, None, None)
+        _ext.C().kv8_decode(out, q, kv_cache, block_tables, seq_lens, query_start_loc, sinks, *ws, max_query_len, max_seq_len, window,
+                            scale, stable_metadata)
+        return
+    _ext.C().kv8_attention_generic(out, q, kv_cache, block_tables, seq_lens, query_start_loc, sinks, window, scale)
