@@ -1130,16 +1130,12 @@ at::Tensor kv8_tickets(Kv8State& s, int64_t n, const at::Tensor& like) {
   if (!t.defined() || t.numel() < n) t = at::zeros({std::max<int64_t>(n, 4096)}, options);
   return t;
 }
-Tmap get_tmap_kv8(GemmState& gs, const at::Tensor& cache) {
-  const int64_t pages = cache.size(0) * 2 * cache.size(2);
-  TmapKey key{cache.data_ptr(), pages, cache.size(3), cache.size(4), 0, -1};
-  auto it = gs.cache.find(key);
-  if (it != gs.cache.end()) return it->second;
-  if (gs.cache.size() > 4096) gs.cache.clear();
+Tmap kv8_tmap(const at::Tensor& cache, int max_rows) {
   Tmap tm;
-  int rc = b200_encode_tmap_kv8(tm.b, cache.data_ptr(), pages, (int)cache.size(3), (int)cache.size(4) - 4);
+  int rc = b200_encode_tmap_kv8(tm.b, cache.data_ptr(), cache.size(0) * 2 * cache.size(2), (int)cache.size(3), (int)cache.size(4) - 4,
+                                max_rows);
   TORCH_CHECK(rc == 0, "tensor map encode failed: ", rc);
-  return gs.cache.emplace(key, tm).first->second;
+  return tm;
 }
 // At most 16 query rows per key / value head; `ws_o`, `ws_lse`, `tickets` (or none of them): scratch of the caller for one stream, the
 // tickets zero at first.
@@ -1162,13 +1158,42 @@ void kv8_decode(at::Tensor out, const at::Tensor& q, const at::Tensor& cache, co
   const at::Tensor o = scratch(ws_o, parts * D), lse = scratch(ws_lse, parts);
   const bool own = tickets.has_value() && tickets->numel() >= B * Hkv && tickets->device() == q.device() && tickets->scalar_type() == at::kInt;
   const at::Tensor tk = own ? *tickets : kv8_tickets(s, B * Hkv, q);
-  const Tmap tm = get_tmap_kv8(gs, cache);
+  const Tmap tm = kv8_tmap(cache, 128);
   check(b200_kv8_decode(out.data_ptr(), q.data_ptr(), cache.data_ptr(), tm.b, block_tables.data_ptr<int>(), seq_lens.data_ptr<int>(),
                         qsl.data_ptr<int>(), sinks.has_value() ? sinks->data_ptr<float>() : nullptr, o.data_ptr<float>(),
                         lse.data_ptr<float>(), tk.data_ptr<int>(), s.status.data_ptr<int>(), (int)B, (int)q.size(1), (int)Hkv, (int)D,
                         (int)cache.size(3), (int)block_tables.size(1), block_tables.stride(0), cache.size(0), (int)max_query_len,
                         max_seq_len, (int)window, (float)scale, q.stride(0), early_meta ? 1 : 0, dtype_code(q), s.num_sms, stream()),
         "kv8_decode");
+}
+// More rows than that: prompts and chunks.
+void kv8_prompt(at::Tensor out, const at::Tensor& q, const at::Tensor& cache, const at::Tensor& block_tables,
+                const at::Tensor& seq_lens, const at::Tensor& qsl, const c10::optional<at::Tensor>& sinks, int64_t max_query_len,
+                int64_t max_seq_len, int64_t window, double scale) {
+  check_kv8_attention(out, q, cache, block_tables, seq_lens, qsl, sinks);
+  if (q.size(0) == 0 || seq_lens.size(0) == 0) return;
+  c10::cuda::CUDAGuard guard(q.device());
+  GemmState& gs = gemm_state();
+  std::lock_guard<std::mutex> lk(gs.mu);
+  Kv8State& s = kv8_state(gs, q);
+  const int64_t B = seq_lens.size(0), T = q.size(0), Hq = q.size(1), Hkv = cache.size(2), D = q.size(2), g = Hq / Hkv;
+  TORCH_CHECK(g <= 128, "kv8_prompt: ", g, " heads a group");
+  const int splits = b200_kv8_prompt_splits((int)B, (int)Hq, (int)Hkv, (int)max_query_len, max_seq_len, (int)window, s.num_sms);
+  at::Tensor o, lse;
+  if (splits > 1) {
+    o = at::empty({splits, T, Hq, D}, q.options().dtype(at::kFloat));
+    lse = at::empty({splits, T, Hq}, q.options().dtype(at::kFloat));
+  }
+  Tmap tq;
+  int rc = b200_encode_tmap_heads(tq.b, q.data_ptr(), T, (int)Hq, (int)D, q.stride(0) * 2, (int)g, (int)(128 / g));
+  TORCH_CHECK(rc == 0, "tensor map encode failed: ", rc);
+  const Tmap tk = kv8_tmap(cache, (int)(64 * D / 128));
+  check(b200_kv8_prompt(out.data_ptr(), cache.data_ptr(), tq.b, tk.b, block_tables.data_ptr<int>(), seq_lens.data_ptr<int>(),
+                        qsl.data_ptr<int>(), sinks.has_value() ? sinks->data_ptr<float>() : nullptr,
+                        splits > 1 ? o.data_ptr<float>() : nullptr, splits > 1 ? lse.data_ptr<float>() : nullptr, splits,
+                        s.status.data_ptr<int>(), T, (int)B, (int)Hq, (int)Hkv, (int)D, (int)cache.size(3), (int)block_tables.size(1),
+                        block_tables.stride(0), cache.size(0), (int)max_query_len, (int)window, (float)scale, dtype_code(q), s.num_sms,
+                        stream()), "kv8_prompt", splits > 1 ? 2 : 1);
 }
 void kv8_attention_generic(at::Tensor out, const at::Tensor& q, const at::Tensor& cache, const at::Tensor& block_tables,
                            const at::Tensor& seq_lens, const at::Tensor& qsl, const c10::optional<at::Tensor>& sinks, int64_t window,
@@ -2344,6 +2369,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("kv_gather", &kv_gather);
   m.def("kv8_attention_generic", &kv8_attention_generic);
   m.def("kv8_decode", &kv8_decode);
+  m.def("kv8_prompt", &kv8_prompt);
   m.def("concat_and_cache_mla", &concat_and_cache_mla);
   m.def("indexer_k_quant_and_cache", &indexer_k_quant_and_cache);
   m.def("convert_req_index_to_global_index", &convert_req_index_to_global_index);

@@ -35,11 +35,15 @@ def paged_attention_kv8(out, q, kv_cache, block_tables, seq_lens, query_start_lo
 
 def _attend(out, q, kv_cache, block_tables, seq_lens, query_start_loc, scale, max_query_len, max_seq_len, window, sinks, workspace,
             stable_metadata):
-    H, D = q.shape[1], q.shape[2]
-    if (TENSOR_CORES[0] and D in (64, 128, 256) and kv_cache.shape[3] % 16 == 0 and q.dtype != torch.float32
-            and max_query_len * (H // kv_cache.shape[2]) <= DECODE_ROWS and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0):
-        ws = (workspace.o, workspace.lse, workspace.tickets) if workspace is not None else (None, None, None)
-        _ext.C().kv8_decode(out, q, kv_cache, block_tables, seq_lens, query_start_loc, sinks, *ws, max_query_len, max_seq_len, window,
-                            scale, stable_metadata)
-        return
+    D, group = q.shape[2], q.shape[1] // kv_cache.shape[2]
+    if TENSOR_CORES[0] and kv_cache.shape[3] % 16 == 0 and q.dtype != torch.float32 and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0:
+        if max_query_len * group <= DECODE_ROWS and D in (64, 128, 256):
+            ws = (workspace.o, workspace.lse, workspace.tickets) if workspace is not None else (None, None, None)
+            _ext.C().kv8_decode(out, q, kv_cache, block_tables, seq_lens, query_start_loc, sinks, *ws, max_query_len, max_seq_len,
+                                window, scale, stable_metadata)
+            return
+        if D in (64, 128) and group <= 128 and scale > 0:
+            _ext.C().kv8_prompt(out, q, kv_cache, block_tables, seq_lens, query_start_loc, sinks, max_query_len, max_seq_len, window,
+                                scale)
+            return
     _ext.C().kv8_attention_generic(out, q, kv_cache, block_tables, seq_lens, query_start_loc, sinks, window, scale)
