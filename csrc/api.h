@@ -157,7 +157,7 @@ int b200_kv8_qkv(void* q_out, const void* qkv, const int64_t* positions, const f
 // rows of either cache (eight = 0: one in the type of `dtype`, [num_blocks][2][Hkv][block_size][D]) to k, v [M, Hkv, D]
 int b200_kv_gather(void* k, void* v, const void* cache, const int64_t* slots, int64_t M, int Hkv, int D, int block_size,
                    int64_t num_blocks, int eight, int dtype, cudaStream_t st);
-int b200_encode_tmap_kv8(void* out, const void* base, uint64_t pages, int block_size, int D, int max_rows);
+int b200_encode_tmap_kv8(void* out, const void* base, uint64_t pages, int block_size, int D, int width, int max_rows);
 int b200_encode_tmap_heads(void* out, const void* base, uint64_t T, int H, int D, uint64_t token_stride_bytes, int heads, int tokens);
 int b200_kv8_prompt_splits(int B, int Hq, int Hkv, int max_query_len, int64_t max_seq_len, int window, int num_sms);
 int b200_kv8_prompt(void* out, const void* cache, const void* tmQ, const void* tmKV, const int* block_tables, const int* seq_lens,

@@ -441,7 +441,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             v[j] = to_f(a.v[j]);
-            bad |= (__float_as_uint(v[j]) & 0x7f800000u) == 0x7f800000u;
+            bad |= !(fabsf(v[j]) <= 8.5e37f);      // infinities, NaN, and what is too large for its scale to be a number: NaN
             amax = fmaxf(amax, fabsf(v[j]));
           }
         } else {

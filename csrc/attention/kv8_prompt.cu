@@ -1,22 +1,23 @@
 // Prompt and chunk attention over the 8-bit paged cache (common/kv8.cuh) on tcgen05 + TMEM, fed by TMA from the pages: heads of 64 and
 // 128, any number of query tokens.
 //
-// The products are 16-bit: per 128-key tile and 128-row query tile
-//     S[128 rows, 128 keys]  = Q . K_tile^T          in the queries' type (bf16 or fp16)
-//     O[128 rows, D dims]   += P[128 rows, 128 keys] . V    in fp16, P in TMEM over the columns of S
-// Four warps turn codes into operands between the TMA's buffer and the tensor core's: every stored value is an exact bf16 and fp16 number
-// (common/kv8.cuh), so nothing is lost, scales are gone before the products, and V and P in fp16 round weights to 11 bits.  Products in e4m3
-// would not be faster: queries and weights need two pieces each, twice the work at twice the rate.
-// What bounds it: per tile the tensor core needs 1024 cycles (2 x 128^3 products), the special-function units as many (128 x 128
-// exponentials at 16 a cycle); conversion is 2 x 128 x 128 values per two tiles.
+// Per 128-key tile and 128-row query tile
+//     S[128 rows, 128 keys]  = Q . K_tile^T                 e4m3: codes as cached, queries in pieces
+//     O[128 rows, D dims]   += P[128 rows, 128 keys] . V    fp16, P in TMEM over the columns of S
+// Queries are sums of e4m3 pieces as in kv8_decode.cu (two hold bf16 exactly, three fp16), so K is an operand as it comes from memory; its
+// scales are multiplied onto the scores.  Two pieces at twice the rate of a 16-bit product cost what that would.  V and P go the other
+// way: pieces of P would have to be made by the softmax warps, which have no time left, so four warps widen V to fp16 between the TMA's
+// buffer and the tensor core's.  Every stored value is an exact fp16 number (common/kv8.cuh): its scale is gone then, and P rounds to 11 bits.
+// What bounds it: per tile the tensor core needs 1024 cycles, the special-function units as many (128 x 128 exponentials at 16 a cycle),
+// shared memory a little more for two tiles than both (1216 a tile: operands, TMA, widening, scales).
 //
 // A row is (token, head of a group): a tile holds 128 / g tokens of all g heads of one key / value head, so that a few new tokens fill it,
 // and K and V are read and converted once for the group.  A persistent CTA works on two tiles ("streams") of consecutive tokens that read
 // the same K / V tiles; the tensor core works on one while the other is in its softmax.  A stream's products are issued in the order
 // P.V(i), S(i + 1), so the arrival of S(i + 1) also says that O holds P.V(i).  With few tiles behind a long context the keys of an item are
 // split over CTAs, whose normalised partial results a second kernel joins.
-// 512 threads: warp 0 TMA producer (a lane per 16 keys), warp 1 MMA issuer, warps 4-7 / 8-11 softmax and epilogue of stream 0 / 1 (thread =
-// row), warps 12-15 conversion.  The grid has a CTA per item, in descending order of row blocks; a CTA that is done takes the next
+// 512 threads: warp 0 TMA producer (a lane per 16 keys), warp 1 MMA issuer, warps 4-7 / 8-11 queries, softmax and epilogue of stream 0 / 1
+// (thread = row), warps 12-15 widening.  The grid has a CTA per item, in descending order of row blocks; a CTA that is done takes the next
 // pending one's item (cluster launch control).  Every wait is bounded; on time-out the status word is set and the CTA unwinds.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -37,17 +38,27 @@ constexpr int kThreads = 4 * 128;
 // 65536, and the split takes 128 x (64 + 192 + 192 + 64) = 65536.
 constexpr int kRegsFew = 64, kRegsSoft = 192;
 constexpr int kTile = 128, kPage = 64;
-constexpr int kKStages = 2, kVStages = 4, kRaw = 4;      // K tiles, V pages, pages of codes
+constexpr int kVStages = 4;                              // V pages as operands
+constexpr int kRing = 4;                                 // K scales and valid masks: one more than the K stages
 constexpr int kTmemCols = 512;
 constexpr float kMaxSlack = 8.f;
 constexpr float kLog2e = 1.4426950408889634f;
 
-template <int D> struct Cfg {
-  static constexpr int kB = D / 64;                    // 64-dim blocks
-  static constexpr int kBlock = kTile * 128;           // one block of a 128-row operand tile
-  static constexpr int kQ = kB * kBlock, kK = kB * kBlock, kV = kB * kPage * 128;
-  static constexpr int kCodes = kPage * D;
-  static constexpr size_t kSmem = 1024 + 2 * kQ + kKStages * kK + kVStages * kV + kRaw * (kCodes + kPage * 4) + 512;
+template <typename T> struct Pieces;
+template <> struct Pieces<__nv_bfloat16> { static constexpr int n = 2; };
+template <> struct Pieces<__half> { static constexpr int n = 3; };
+
+template <typename T, int D> struct Cfg {
+  static constexpr int P = Pieces<T>::n;
+  static constexpr int kPiece = kTile * D;             // 128 rows of D e4m3 bytes
+  static constexpr int kQ = P * kPiece;                // a stream's queries; in 16 bits (2 * kPiece) until they are taken apart
+  static constexpr int kKStages = 3 - (P == 3 && D == 128), kK = kTile * D;
+  static constexpr int kB = D / 64;                    // 64-dim blocks of a 16-bit row
+  static constexpr int kV = kB * kPage * 128;
+  static constexpr int kRaw = P == 3 && D == 128 ? 3 : 4, kCodes = kPage * D;      // V pages as codes
+  static constexpr size_t kSmem =
+      1024 + 2 * kQ + kKStages * kK + kVStages * kV + kRaw * (kCodes + kPage * 4) + kRing * kTile * 4 + 512;
+  static_assert(kSmem <= 227 * 1024 && kKStages < kRing);
 };
 
 struct Params {
@@ -122,10 +133,20 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
   return d;
 }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t d;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
+}
+__device__ __forceinline__ uint16_t f16x2_to_e4m3x2(__half2 v) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(*reinterpret_cast<const uint32_t*>(&v)));
+  return r;
 }
 // 2^x on the special-function unit (-inf -> 0)
 __device__ __forceinline__ float ex2_approx(float x) {
@@ -133,9 +154,6 @@ __device__ __forceinline__ float ex2_approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-template <typename T> struct FmtOf;
-template <> struct FmtOf<__nv_bfloat16> { static constexpr uint32_t v = 1; };
-template <> struct FmtOf<__half> { static constexpr uint32_t v = 0; };
 template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
   uint32_t d;
@@ -148,34 +166,24 @@ template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi
   return d;
 }
 
-// Codes -> 16-bit values times a power of two, exact.
-template <typename T> struct Widen;
-template <> struct Widen<__half> {
-  static __device__ __forceinline__ uint32_t factor(float s) { return pack2<__half>(s, s); }
-  static __device__ __forceinline__ void four(uint32_t w, uint32_t f, uint32_t& lo, uint32_t& hi) {
-    const uint32_t a = e4m3x2_to_f16x2((uint16_t)w), b = e4m3x2_to_f16x2((uint16_t)(w >> 16));
-    const __half2 s = *reinterpret_cast<const __half2*>(&f);
-    const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&a), s), y = __hmul2(*reinterpret_cast<const __half2*>(&b), s);
-    lo = *reinterpret_cast<const uint32_t*>(&x);
-    hi = *reinterpret_cast<const uint32_t*>(&y);
-  }
-};
-// Exponent and mantissa of an e4m3 number four places lower in a bf16 number are its value times 2^-120, below the normal range too.
-template <> struct Widen<__nv_bfloat16> {
-  static __device__ __forceinline__ uint32_t factor(float s) {
-    const uint32_t b = __float_as_uint(s * 1.329227995784916e36f);      // 2^120
-    return __byte_perm(b, b, 0x3232);
-  }
-  static __device__ __forceinline__ uint32_t two(uint32_t u, uint32_t f) {
-    const uint32_t x = ((u >> 4) & 0x07f007f0u) | (u & 0x80008000u);
-    const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&f));
-    return *reinterpret_cast<const uint32_t*>(&y);
-  }
-  static __device__ __forceinline__ void four(uint32_t w, uint32_t f, uint32_t& lo, uint32_t& hi) {
-    lo = two(__byte_perm(w, 0, 0x1404), f);
-    hi = two(__byte_perm(w, 0, 0x3424), f);
-  }
-};
+// four codes -> four fp16 values times a power of two, exact
+__device__ __forceinline__ void widen4(uint32_t w, __half2 f, uint32_t& lo, uint32_t& hi) {
+  const uint32_t a = e4m3x2_to_f16x2((uint16_t)w), b = e4m3x2_to_f16x2((uint16_t)(w >> 16));
+  const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&a), f), y = __hmul2(*reinterpret_cast<const __half2*>(&b), f);
+  lo = *reinterpret_cast<const uint32_t*>(&x);
+  hi = *reinterpret_cast<const uint32_t*>(&y);
+}
+
+// K-major operand whose rows are D e4m3 bytes, swizzled over 128 or 64 bytes; and where 16-byte chunk c of row r lies
+template <int D>
+__device__ __forceinline__ uint64_t desc_rows(uint32_t addr) {
+  if constexpr (D == 128) return umma_desc_k_sw128(addr);
+  return (uint64_t)((addr & 0x3FFFF) >> 4) | (uint64_t)1 << 16 | (uint64_t)(512 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)4 << 61;
+}
+template <int D>
+__device__ __forceinline__ int chunk_at(int r, int c) {
+  return D == 128 ? r * 128 + ((c ^ (r & 7)) << 4) : r * 64 + ((c ^ (r >> 1 & 3)) << 4);
+}
 
 // One work item: what the two streams of a CTA share and their own rows.
 struct Item {
@@ -233,42 +241,45 @@ __device__ __forceinline__ int taken_cta(uint32_t src) {
   return ok ? (int)x : -1;
 }
 
-// What a page of codes is, for the conversion warps: bits 0-3 which 16 keys were read, 4-10 keys in front of the request's end, 11 V, 12 the
-// end of all work; 16-18 the tile's place in the ring of valid masks (K).
-constexpr uint32_t kMetaV = 1u << 11, kMetaEnd = 1u << 12;
+// What a page of V is, for the widening warps: bits 0-3 which 16 keys were read, 4-10 keys in front of the request's end, 12 the end of
+// all work.
+constexpr uint32_t kMetaEnd = 1u << 12;
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
 kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmKV, const __grid_constant__ Params p) {
-  using C = Cfg<D>;
-  constexpr int kB = C::kB;
+  using C = Cfg<T, D>;
+  constexpr int kB = C::kB, kKStages = C::kKStages, kRaw = C::kRaw;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sQ = smem;                                  // [2 streams][kB dim blocks][128 rows][128 B]
-  uint8_t* sK = sQ + 2 * C::kQ;                        // [kKStages][kB dim blocks][128 keys][128 B]
+  uint8_t* sQ = smem;                                  // [2 streams][pieces][128 rows][D B]
+  uint8_t* sK = sQ + 2 * C::kQ;                        // [kKStages][128 keys][D B]
   uint8_t* sV = sK + kKStages * C::kK;                 // [kVStages][kB dim blocks][64 keys][128 B]
   uint8_t* sRaw = sV + kVStages * C::kV;               // [kRaw][64 keys][D B]
-  float* sScale = reinterpret_cast<float*>(sRaw + kRaw * C::kCodes);   // [kRaw][64]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sScale + kRaw * kPage);
+  float* sScaleV = reinterpret_cast<float*>(sRaw + kRaw * C::kCodes);   // [kRaw][64]
+  float* sScaleK = sScaleV + kRaw * kPage;             // [kRing][128]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sScaleK + kRing * kTile);
   uint64_t* q_full = bars;              // one phase per item
   uint64_t* q_empty = bars + 1;         // the item's last S has been computed
-  uint64_t* k_full = bars + 2;          // [2] four warps, two pages
-  uint64_t* k_empty = bars + 4;         // [2] both streams' S of the tile have been computed
-  uint64_t* v_full = bars + 6;          // [4] four warps
-  uint64_t* v_empty = bars + 10;        // [4]
-  uint64_t* raw_full = bars + 14;       // [4]
-  uint64_t* raw_empty = bars + 18;      // [4] four warps
-  uint64_t* s_full = bars + 22;         // [2 streams]
-  uint64_t* p_ready = bars + 24;        // [2 streams][2 halves] one arrival per softmax warp
-  uint64_t* o_final = bars + 28;        // [2 streams] one phase per item with work for the stream
+  uint64_t* q_ready = bars + 2;         // [2 streams] in pieces: four warps, a phase per item with work for the stream
+  uint64_t* k_full = bars + 4;          // [3]
+  uint64_t* k_empty = bars + 7;         // [3] both streams' S of the tile have been computed
+  uint64_t* ks_full = bars + 10;        // [kRing] scales and valid mask
+  uint64_t* v_full = bars + 14;         // [4] four warps
+  uint64_t* v_empty = bars + 18;        // [4]
+  uint64_t* raw_full = bars + 22;       // [4]
+  uint64_t* raw_empty = bars + 26;      // [4] four warps
+  uint64_t* s_full = bars + 30;         // [2 streams]
+  uint64_t* p_ready = bars + 32;        // [2 streams][2 halves] one arrival per softmax warp
+  uint64_t* o_final = bars + 36;        // [2 streams] one phase per item with work for the stream
   // answers about the next item: question k uses slot k & 1
-  uint64_t* next_full = bars + 30;      // [2]
-  uint64_t* next_empty = bars + 32;     // [2] read by the MMA thread and the eight softmax warps
-  const uint32_t next_at = smem_u32(bars + 34);   // [2] x 16 bytes
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 38);
+  uint64_t* next_full = bars + 38;      // [2]
+  uint64_t* next_empty = bars + 40;     // [2] read by the MMA thread and the eight softmax warps
+  const uint32_t next_at = smem_u32(bars + 42);   // [2] x 16 bytes
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 46);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  uint32_t* sMeta = tmem_slot + 2;      // [kRaw]
-  volatile uint32_t* sValid = sMeta + kRaw;   // [8] which 16 keys of a tile are there
+  uint32_t* sMeta = tmem_slot + 2;      // [4]
+  uint32_t* sValid = sMeta + 4;         // [kRing] which 16 keys of a tile are there
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   Abort ab{p.status, abort_flag};
@@ -276,10 +287,12 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     *abort_flag = 0;
     mbar_init(q_full, 1);
     mbar_init(q_empty, 1);
-    for (int b = 0; b < kKStages; ++b) { mbar_init(&k_full[b], 8); mbar_init(&k_empty[b], 1); }
+    for (int b = 0; b < kKStages; ++b) { mbar_init(&k_full[b], 1); mbar_init(&k_empty[b], 1); }
+    for (int b = 0; b < kRing; ++b) mbar_init(&ks_full[b], 1);
     for (int b = 0; b < kVStages; ++b) { mbar_init(&v_full[b], 4); mbar_init(&v_empty[b], 1); }
     for (int b = 0; b < kRaw; ++b) { mbar_init(&raw_full[b], 1); mbar_init(&raw_empty[b], 4); }
     for (int s = 0; s < 2; ++s) {
+      mbar_init(&q_ready[s], 4);
       mbar_init(&s_full[s], 1);
       mbar_init(&o_final[s], 1);
       for (int h = 0; h < 2; ++h) mbar_init(&p_ready[s * 2 + h], 4);
@@ -317,11 +330,9 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   if (warp < 4 || warp >= 12) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsFew));
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer: lane u = keys 16 u .. of a tile
-    const int page_rows = p.block_size * D / 128;                        // rows of 128 bytes of a cache page
-    const int R = min(kPage * D / 128, page_rows & -page_rows);          // ... of a box; the host's map agrees
-    const int box_keys = R * 128 / D, units = box_keys / 16;
+    const int R = min(kPage, p.block_size & -p.block_size), units = R / 16;      // keys of a box; the host's map agrees
     const int64_t page_bytes = (int64_t)p.block_size * (D + 4);
-    int rc = 0, qc = 0, asked = 0, tiles = 0;      // pages and items issued, questions asked, K tiles so far
+    int kc = 0, rc = 0, qc = 0, asked = 0;      // K tiles, V pages and items issued, questions asked so far
     bool ok = true;
     auto wait_all = [&](uint64_t* bar, uint32_t parity, int code) { return __all_sync(0xffffffffu, wait_or_abort(bar, parity, ab, code)) != 0; };
     // asked when the item's last loads are due: late enough that a CTA does not hold an item it cannot start, early enough that the
@@ -342,13 +353,13 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       if (n_max > 0) {
         if (qc > 0 && !wait_all(q_empty, (qc - 1) & 1, 920)) { ok = false; break; }
         if (lane == 0) {
-          mbar_expect_tx(q_full, p.toks * p.g * 128 * kB * ((it.n[0] > 0) + (it.n[1] > 0)));
+          mbar_expect_tx(q_full, p.toks * p.g * 2 * D * ((it.n[0] > 0) + (it.n[1] > 0)));
 #pragma unroll
           for (int s = 0; s < 2; ++s)
             if (it.n[s] > 0) {
 #pragma unroll
               for (int h = 0; h < kB; ++h)
-                tma_load_3d(sQ + s * C::kQ + h * C::kBlock, &tmQ, q_full, h * 64, it.head * p.g, it.qs + it.tok0[s]);
+                tma_load_3d(sQ + s * C::kQ + h * (kTile * 128), &tmQ, q_full, h * 64, it.head * p.g, it.qs + it.tok0[s]);
             }
         }
         ++qc;
@@ -361,8 +372,31 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           const int blk = bi < p.max_blocks ? bt[bi] : -1;
           return blk >= 0 && blk < p.num_blocks ? blk : -1;
         };
-        // pages of tile j: lanes at the start of a box issue it
-        auto load = [&](int j, int blk, bool is_v, int place) {
+        // lanes at the start of a box issue it
+        auto copy = [&](int key, int blk, int which, uint8_t* codes, float* scales, uint64_t* full_codes, uint64_t* full_scales) {
+          const int in = key % p.block_size;
+          const int64_t page = ((int64_t)blk * 2 + which) * p.Hkv + it.head;
+          tma_load_3d(codes, &tmKV, full_codes, 0, in, (int)page);
+          bulk_load_1d(scales, p.cache + page * page_bytes + (int64_t)p.block_size * D + in * 4, R * 4, full_scales);
+        };
+        auto load_k = [&](int j, int blk) {
+          const uint32_t valid = __ballot_sync(0xffffffffu, blk >= 0);
+          const bool issuer = blk >= 0 && lane % units == 0;
+          const int boxes = __popc(__ballot_sync(0xffffffffu, issuer)), st = kc % kKStages, at = kc % kRing;
+          if (kc >= kKStages && !wait_all(&k_empty[st], (kc / kKStages - 1) & 1, 921)) return false;
+          if (lane == 0) {
+            sValid[at] = valid;
+            mbar_expect_tx(&k_full[st], boxes * R * D);
+            mbar_expect_tx(&ks_full[at], boxes * R * 4);
+          }
+          __syncwarp();
+          if (issuer)
+            copy(it.key0 + j * kTile + lane * 16, blk, 0, sK + st * C::kK + lane * 16 * D, sScaleK + at * kTile + lane * 16, &k_full[st],
+                 &ks_full[at]);
+          ++kc;
+          return true;
+        };
+        auto load_v = [&](int j, int blk) {
           const uint32_t valid = __ballot_sync(0xffffffffu, blk >= 0);
           const int key0 = it.key0 + j * kTile;
           const bool issuer = blk >= 0 && lane % units == 0;
@@ -370,20 +404,16 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 #pragma unroll 1
           for (int pg = 0; pg < 2; ++pg) {
             const int st = rc % kRaw;
-            if (rc >= kRaw && !wait_all(&raw_empty[st], (rc / kRaw - 1) & 1, 921)) return false;
+            if (rc >= kRaw && !wait_all(&raw_empty[st], (rc / kRaw - 1) & 1, 922)) return false;
             if (lane == 0) {
               const int left = max(0, min(kPage, it.seq_len - key0 - pg * kPage));
-              sMeta[st] = (valid >> (4 * pg) & 15u) | (uint32_t)left << 4 | (is_v ? kMetaV : 0u) | (uint32_t)place << 16;
-              mbar_expect_tx(&raw_full[st], __popc(starts >> (4 * pg) & 15u) * (R * 128 + box_keys * 4));
+              sMeta[st] = (valid >> (4 * pg) & 15u) | (uint32_t)left << 4;
+              mbar_expect_tx(&raw_full[st], __popc(starts >> (4 * pg) & 15u) * R * (D + 4));
             }
             __syncwarp();
-            if (issuer && lane >> 2 == pg) {
-              const int in = (key0 + lane * 16) % p.block_size, at = (lane & 3) * 16;      // key within its block, within the page
-              const int64_t page = ((int64_t)blk * 2 + is_v) * p.Hkv + it.head;
-              tma_load_3d(sRaw + st * C::kCodes + at * D, &tmKV, &raw_full[st], 0, in * D / 128, (int)page);
-              bulk_load_1d(sScale + st * kPage + at, p.cache + page * page_bytes + (int64_t)p.block_size * D + in * 4, box_keys * 4,
-                           &raw_full[st]);
-            }
+            if (issuer && lane >> 2 == pg)
+              copy(key0 + lane * 16, blk, 1, sRaw + st * C::kCodes + (lane & 3) * 16 * D, sScaleV + st * kPage + (lane & 3) * 16,
+                   &raw_full[st], &raw_full[st]);
             ++rc;
           }
           return true;
@@ -392,12 +422,11 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         for (int j = 0; ok && j <= n_max; ++j) {      // K(0), K(1), V(0), K(2), V(1), ...
           if (j == n_max - 1 && p.take && !ask()) { ok = false; break; }
           const int after = lookup(j + 1);
-          if (j < n_max) ok = load(j, blk, false, (tiles + j) & 7);
-          if (ok && j >= 1) ok = load(j - 1, blk_v, true, 0);
+          if (j < n_max) ok = load_k(j, blk);
+          if (ok && j >= 1) ok = load_v(j - 1, blk_v);
           blk_v = blk;
           blk = after;
         }
-        tiles += n_max;
       } else if (p.take) {
         ok = ask();
       }
@@ -407,9 +436,9 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       fence_proxy_async_smem();
       __syncwarp();
     }
-    if (ok) {          // the conversion warps' end
+    if (ok) {          // the widening warps' end
       const int st = rc % kRaw;
-      if (rc >= kRaw) ok = wait_all(&raw_empty[st], (rc / kRaw - 1) & 1, 921);
+      if (rc >= kRaw) ok = wait_all(&raw_empty[st], (rc / kRaw - 1) & 1, 922);
       if (ok && lane == 0) {
         sMeta[st] = kMetaEnd;
         mbar_arrive(&raw_full[st]);
@@ -421,15 +450,17 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           if (mbar_try_wait(bar, parity)) break;
       };
       if (qc > 0) drain(q_full, (qc - 1) & 1);
+      for (int i = max(0, kc - kKStages); i < kc; ++i) drain(&k_full[i % kKStages], (i / kKStages) & 1);
+      for (int i = max(0, kc - kRing); i < kc; ++i) drain(&ks_full[i % kRing], (i / kRing) & 1);
       for (int i = max(0, rc - kRaw); i < rc; ++i) drain(&raw_full[i % kRaw], (i / kRaw) & 1);
       if (asked > 0) drain(&next_full[(asked - 1) & 1], ((asked - 1) >> 1) & 1);
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
     if (elect_one()) {
-      constexpr uint32_t idesc_s = umma_idesc(kTile, kTile, FmtOf<T>::v, FmtOf<T>::v, 0, 0);   // A = Q, B = K tile, both K-major
+      constexpr uint32_t idesc_s = umma_idesc(kTile, kTile, 0, 0, 0, 0);   // A = Q, B = K tile, both e4m3 and K-major
       constexpr uint32_t idesc_o = umma_idesc(kTile, D, 0, 0, 0, 1);       // A = P (TMEM), B = V tile (MN-major), fp16
-      int kc = 0, vc = 0, qc = 0, tc[2] = {0, 0};   // consumed so far; tc: tiles of each stream whose P has been awaited
+      int kc = 0, vc = 0, qc[2] = {0, 0}, tc[2] = {0, 0};   // consumed so far; tc: tiles of each stream whose P has been awaited
       bool ok = true;
       for (int idx = blockIdx.x, round = 0; idx >= 0; idx = ok ? next_item(round++, false, ok) : -1) {
         get_item(p, idx, it);
@@ -439,9 +470,9 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         auto issue_s = [&](int s, int j) {
           const uint32_t q_addr = smem_u32(sQ + s * C::kQ), k_addr = smem_u32(sK + ((kc + j) % kKStages) * C::kK);
 #pragma unroll
-          for (int k = 0; k < kB * 4; ++k)
-            umma_f16(tmem_base + s * kTile, umma_desc_k_sw128(q_addr + (k / 4) * C::kBlock + (k % 4) * 32),
-                     umma_desc_k_sw128(k_addr + (k / 4) * C::kBlock + (k % 4) * 32), idesc_s, k > 0 ? 1u : 0u);
+          for (int c = 0; c < C::P * (D / 32); ++c)
+            umma_f8(tmem_base + s * kTile, desc_rows<D>(q_addr + c / (D / 32) * C::kPiece + c % (D / 32) * 32),
+                    desc_rows<D>(k_addr + c % (D / 32) * 32), idesc_s, c > 0 ? 1u : 0u);
           umma_commit(&s_full[s]);
           const bool last = s == 1 || j >= it.n[1];
           if (last) {
@@ -449,12 +480,17 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             if (j == n_max - 1) umma_commit(q_empty);
           }
         };
-        ok = wait_or_abort(q_full, qc & 1, ab, 923) && wait_or_abort(&k_full[kc % kKStages], (kc / kKStages) & 1, ab, 924);
+        ok = wait_or_abort(&k_full[kc % kKStages], (kc / kKStages) & 1, ab, 924);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          if (!ok || it.n[s] == 0) continue;
+          ok = wait_or_abort(&q_ready[s], qc[s] & 1, ab, 923);
+          if (!ok) break;
+          ++qc[s];
+          tc_fence_after_sync();
+          issue_s(s, 0);
+        }
         if (!ok) break;
-        ++qc;
-        tc_fence_after_sync();
-        if (it.n[0] > 0) issue_s(0, 0);
-        if (it.n[1] > 0) issue_s(1, 0);
         for (int i = 0; ok && i < n_max; ++i) {
 #pragma unroll
           for (int s = 0; s < 2; ++s) {
@@ -493,87 +529,61 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       }
     }
   } else if (warp >= 12) {
-    // ------------------------------------------------------------------ conversion: 16 codes a thread and step
+    // ------------------------------------------------------------------ V in fp16: 16 codes a thread and step
     const int w = warp - 12;
-    int kp = 0, vp = 0;       // pages of K and V so far
     for (int n = 0;; ++n) {
-      const int st = n % kRaw;
+      const int st = n % kRaw, to = n % kVStages;
       if (__any_sync(0xffffffffu, !wait_or_abort(&raw_full[st], (n / kRaw) & 1, ab, 931))) break;
       const uint32_t meta = sMeta[st];
       if (meta & kMetaEnd) break;
-      const bool is_v = (meta & kMetaV) != 0;
-      const uint8_t* src = sRaw + st * C::kCodes;
-      const float* scale = sScale + st * kPage;
-      uint8_t* dst;
-      int block_bytes;
-      uint64_t* full;
-      if (is_v) {
-        const int s = vp % kVStages;
-        if (vp >= kVStages && __any_sync(0xffffffffu, !wait_or_abort(&v_empty[s], (vp / kVStages - 1) & 1, ab, 932))) break;
-        dst = sV + s * C::kV;
-        block_bytes = kPage * 128;
-        full = &v_full[s];
-        ++vp;
-      } else {
-        const int tile = kp >> 1, s = tile % kKStages;
-        if (tile >= kKStages && __any_sync(0xffffffffu, !wait_or_abort(&k_empty[s], (tile / kKStages - 1) & 1, ab, 933))) break;
-        dst = sK + s * C::kK + (kp & 1) * (kPage * 128);
-        block_bytes = C::kBlock;
-        full = &k_full[s];
-        if (w == 0 && lane == 0) {       // this half's bits; the first half clears the other's
-          const int at = meta >> 16 & 7;
-          sValid[at] = (kp & 1) ? sValid[at] | (meta & 15u) << 4 : meta & 15u;
-        }
-        ++kp;
-      }
       const int left = meta >> 4 & 127;
+      const uint8_t* src = sRaw + st * C::kCodes;
+      const float* scale = sScaleV + st * kPage;
+      uint8_t* dst = sV + to * C::kV;
       // A warp takes 16 keys.  Eight lanes together must meet eight different 16-byte places of a 128-byte line, when they read (place =
-      // chunk ^ row % 8) and when they write (two chunks of eight values, places of one parity for a row): the lower four take the lower
-      // half of a row's codes, the upper four the upper half of the next row's, and the other halves a step later.  Heads of 64: a row of
-      // codes is two keys, and its halves are keys of different parity anyway.
-#pragma unroll
-      for (int i = 0; i < 16 * D / 512; ++i) {
-        int key, src_row, chunk, dim;     // chunk: 16 codes of the source row; dim: first dim
+      // chunk ^ row % 8) and when they write (two chunks of eight values, places of one parity for a row).  Heads of 128: the lower four
+      // take the lower half of a row's codes, the upper four the upper half of the next row's, and the other halves a step later.  Heads
+      // of 64: two rows of 64 bytes.
+      constexpr int kSteps = 16 * D / 512;
+      auto where = [&](int i, int& key, int& chunk) {    // chunk: 16 codes of a row
         if constexpr (D == 128) {
-          const int sub = (lane >> 2 & 1) ^ (i & 1);
           key = w * 16 + (i >> 1) * 8 + (lane >> 2);
-          src_row = key;
-          chunk = (lane & 3) + 4 * sub;
-          dim = chunk * 16;
+          chunk = (lane & 3) + 4 * ((lane >> 2 & 1) ^ (i & 1));
         } else {
-          src_row = w * 8 + i * 4 + (lane >> 3);
-          chunk = lane & 7;
-          key = 2 * src_row + (chunk >> 2);
-          dim = (chunk & 3) * 16;
+          key = w * 16 + i * 8 + (lane >> 2);
+          chunk = lane & 3;
         }
-        const uint4 c = *reinterpret_cast<const uint4*>(src + src_row * 128 + ((chunk ^ (src_row & 7)) << 4));
-        const float s = scale[key];
-        const uint32_t x[4] = {c.x, c.y, c.z, c.w};
+      };
+      uint4 c[kSteps];          // all loads in front of the first store: the compiler cannot tell the buffers apart
+      float sc[kSteps];
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        int key, chunk;
+        where(i, key, chunk);
+        c[i] = *reinterpret_cast<const uint4*>(src + chunk_at<D>(key, chunk));
+        sc[i] = scale[key];
+      }
+      if (n >= kVStages && __any_sync(0xffffffffu, !wait_or_abort(&v_empty[to], (n / kVStages - 1) & 1, ab, 932))) break;
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        int key, chunk;
+        where(i, key, chunk);
+        // rows that were not read, lie behind the end or hold a NaN (whose key says so): zeros, since a weight of zero does not hide one
+        const bool there = key < left && (meta >> (key >> 4) & 1u) && !is_nan_bits(sc[i]);
+        const __half2 f = __float2half2_rn(there ? sc[i] : 0.f);
+        const uint32_t x[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
         uint32_t y[8];
-        if (is_v) {
-          // rows that were not read, lie behind the end or hold a NaN (whose key says so): zeros, since a weight of zero does not hide one
-          const bool there = key < left && (meta >> (key >> 4) & 1u) && !is_nan_bits(s);
-          const uint32_t f = Widen<__half>::factor(s);
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            Widen<__half>::four(x[q], f, y[2 * q], y[2 * q + 1]);
-            y[2 * q] = there ? y[2 * q] : 0u;
-            y[2 * q + 1] = there ? y[2 * q + 1] : 0u;
-          }
-        } else {
-          const uint32_t f = Widen<T>::factor(s);
-#pragma unroll
-          for (int q = 0; q < 4; ++q) Widen<T>::four(x[q], f, y[2 * q], y[2 * q + 1]);
-        }
-        uint8_t* row = dst + (dim >> 6) * block_bytes + key * 128;
-        const int at = (dim & 63) >> 3;
+        for (int q = 0; q < 4; ++q) widen4(there ? x[q] : 0u, f, y[2 * q], y[2 * q + 1]);
+        const int at = 2 * (chunk & 3);
+        uint8_t* row = dst + (chunk >> 2) * (kPage * 128) + key * 128;
         *reinterpret_cast<uint4*>(row + ((at ^ (key & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
         *reinterpret_cast<uint4*>(row + (((at + 1) ^ (key & 7)) << 4)) = make_uint4(y[4], y[5], y[6], y[7]);
       }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
-        mbar_arrive(full);
+        mbar_arrive(&v_full[to]);
         mbar_arrive(&raw_empty[st]);
       }
     }
@@ -585,8 +595,7 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const int r_tok = r / p.g, r_head = r % p.g;
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
     const uint32_t tS = tmem_base + s * kTile + lane_off, tO = tmem_base + (2 + s) * kTile + lane_off;
-    const float sc = p.scale_log2;
-    int tc = 0, oc = 0, tiles = 0;    // tiles and items of this stream so far, K tiles of all items
+    int tc = 0, oc = 0, tiles = 0, qc = 0;    // tiles and items of this stream so far, K tiles and items of both
     bool fail = false;
     bool ok = true;
     for (int idx = blockIdx.x, round = 0; idx >= 0; idx = next_item(round++, true, ok)) {
@@ -594,13 +603,61 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       const int n = s ? it.n[1] : it.n[0], tok0 = s ? it.tok0[1] : it.tok0[0], toks = s ? it.toks[1] : it.toks[0];
       const bool row_ok = r_tok < toks;                // toks <= 128 / g
       const int64_t orow = (int64_t)(it.qs + tok0 + r_tok) * p.Hq + it.head * p.g + r_head;
+      if (it.n_max > 0) ++qc;
       if (n == 0) {
         if (p.splits > 1 && row_ok) p.ws_lse[(int64_t)it.split * p.T * p.Hq + orow] = -INFINITY;
         tiles += it.n_max;
         continue;
       }
       const int pos_first = it.ctx + tok0, pos_last = pos_first + toks - 1, pos = pos_first + r_tok;
-      float m_used = -INFINITY, l_sum = 0.f;
+      float m_used = -INFINITY, l_sum = 0.f, sc;
+      // ---- this row's queries in pieces, over the 16-bit ones; sc: what a score is still to be multiplied with
+      {
+        const bool late = !wait_or_abort(q_full, (qc - 1) & 1, ab, 920);
+        uint8_t* q = sQ + s * C::kQ;
+        uint4 x[D / 8];
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) x[c] = *reinterpret_cast<const uint4*>(q + (c >> 3) * (kTile * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+        // magnitudes compare as integers.  Infinities and NaN, and what is too large for its scale to be a number: NaN
+        uint32_t top = 0;
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c)
+          top = __vmaxu2(__vmaxu2(__vmaxu2(top, x[c].x & 0x7fff7fffu), x[c].y & 0x7fff7fffu), __vmaxu2(x[c].z & 0x7fff7fffu, x[c].w & 0x7fff7fffu));
+        const uint32_t t16 = max(top & 0xffffu, top >> 16);
+        const float amax = to_f(__builtin_bit_cast(T, (uint16_t)t16));
+        const bool bad = !row_ok || !(amax <= 8.5e37f);
+        const float up2 = pow2_ceil(bad ? 1.f : fmaxf(amax, 1e-30f)), up = 256.f * pow2_inv(up2);
+        sc = bad ? __uint_as_float(0x7fffffffu) : up2 * (1.f / 256.f) * p.scale_log2;
+        if (bar_red_or(1 + s, 128, late)) { fail = true; break; }     // also: rows of pieces and of queries overlap
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) {
+          __half2 rest[8];                   // 16 elements, scaled: at most 256, fp16 holds them
+          const uint32_t in[8] = {x[2 * c].x, x[2 * c].y, x[2 * c].z, x[2 * c].w, x[2 * c + 1].x, x[2 * c + 1].y, x[2 * c + 1].z, x[2 * c + 1].w};
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float lo = to_f(__builtin_bit_cast(T, (uint16_t)in[j])), hi = to_f(__builtin_bit_cast(T, (uint16_t)(in[j] >> 16)));
+            rest[j] = bad ? __float2half2_rn(0.f) : __floats2half2_rn(lo * up, hi * up);
+          }
+#pragma unroll
+          for (int k = 0; k < C::P; ++k) {
+            uint32_t y[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const uint16_t a = f16x2_to_e4m3x2(rest[2 * j]), b = f16x2_to_e4m3x2(rest[2 * j + 1]);
+              y[j] = a | (uint32_t)b << 16;
+              if (k + 1 < C::P) {
+                const uint32_t ua = e4m3x2_to_f16x2(a), ub = e4m3x2_to_f16x2(b);
+                rest[2 * j] = __hsub2(rest[2 * j], *reinterpret_cast<const __half2*>(&ua));
+                rest[2 * j + 1] = __hsub2(rest[2 * j + 1], *reinterpret_cast<const __half2*>(&ub));
+              }
+            }
+            *reinterpret_cast<uint4*>(q + k * C::kPiece + chunk_at<D>(r, c)) = make_uint4(y[0], y[1], y[2], y[3]);
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_ready[s]);
+      }
       for (int i = 0; i < n; ++i, ++tc) {
         if (__any_sync(0xffffffffu, !wait_or_abort(&s_full[s], tc & 1, ab, 927))) { fail = true; break; }
         tc_fence_after_sync();
@@ -608,8 +665,22 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         uint32_t v[kTile];
 #pragma unroll
         for (int c = 0; c < kTile; c += 32) tmem_ld_x32_p(tS + c, v + c);
-        const uint32_t valid = sValid[(tiles + i) & 7];
+        const int ring = (tiles + i) % kRing;
+        if (__any_sync(0xffffffffu, !wait_or_abort(&ks_full[ring], ((tiles + i) / kRing) & 1, ab, 934))) { fail = true; break; }
+        const uint32_t valid = sValid[ring];
+        const float4* kscale = reinterpret_cast<const float4*>(sScaleK + ring * kTile);
         tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < kTile; e += 4) {
+          const float4 f = kscale[e / 4];
+          float a, b;
+          unf2(mul2(f2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), f2(f.x, f.y)), a, b);
+          v[e] = __float_as_uint(a);
+          v[e + 1] = __float_as_uint(b);
+          unf2(mul2(f2(__uint_as_float(v[e + 2]), __uint_as_float(v[e + 3])), f2(f.z, f.w)), a, b);
+          v[e + 2] = __float_as_uint(a);
+          v[e + 3] = __float_as_uint(b);
+        }
         // a tile that every row of this stream sees in full needs no mask
         const bool full_tile = key0 + kTile - 1 <= pos_first && key0 + kTile <= it.seq_len && valid == 0xffu &&
                                (p.window <= 0 || key0 > pos_last - p.window);
@@ -759,9 +830,9 @@ kv8_join_kernel(T* __restrict__ out, const float* __restrict__ ws_o, const float
 template <typename T, int D>
 static int launch(const Params& p, const CUtensorMap& tmQ, const CUtensorMap& tmKV, int64_t items, cudaStream_t st) {
   auto kern = kv8_prompt_kernel<T, D>;
-  cudaError_t e = ensure_dynamic_smem((const void*)kern, (int)Cfg<D>::kSmem);
+  cudaError_t e = ensure_dynamic_smem((const void*)kern, (int)Cfg<T, D>::kSmem);
   if (e != cudaSuccess) return (int)e;
-  e = launch_pdl(kern, dim3((unsigned)items), dim3(kThreads), Cfg<D>::kSmem, st, tmQ, tmKV, p);
+  e = launch_pdl(kern, dim3((unsigned)items), dim3(kThreads), Cfg<T, D>::kSmem, st, tmQ, tmKV, p);
   if (e != cudaSuccess || p.splits == 1) return (int)e;
   const int64_t rows = p.T * p.Hq;
   return (int)launch_pdl(kv8_join_kernel<T, D>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, (T*)p.out, (const float*)p.ws_o,

@@ -1130,10 +1130,10 @@ at::Tensor kv8_tickets(Kv8State& s, int64_t n, const at::Tensor& like) {
   if (!t.defined() || t.numel() < n) t = at::zeros({std::max<int64_t>(n, 4096)}, options);
   return t;
 }
-Tmap kv8_tmap(const at::Tensor& cache, int max_rows) {
+Tmap kv8_tmap(const at::Tensor& cache, int width, int max_rows) {
   Tmap tm;
   int rc = b200_encode_tmap_kv8(tm.b, cache.data_ptr(), cache.size(0) * 2 * cache.size(2), (int)cache.size(3), (int)cache.size(4) - 4,
-                                max_rows);
+                                width, max_rows);
   TORCH_CHECK(rc == 0, "tensor map encode failed: ", rc);
   return tm;
 }
@@ -1158,7 +1158,7 @@ void kv8_decode(at::Tensor out, const at::Tensor& q, const at::Tensor& cache, co
   const at::Tensor o = scratch(ws_o, parts * D), lse = scratch(ws_lse, parts);
   const bool own = tickets.has_value() && tickets->numel() >= B * Hkv && tickets->device() == q.device() && tickets->scalar_type() == at::kInt;
   const at::Tensor tk = own ? *tickets : kv8_tickets(s, B * Hkv, q);
-  const Tmap tm = kv8_tmap(cache, 128);
+  const Tmap tm = kv8_tmap(cache, std::max<int>(128, (int)D), 128);
   check(b200_kv8_decode(out.data_ptr(), q.data_ptr(), cache.data_ptr(), tm.b, block_tables.data_ptr<int>(), seq_lens.data_ptr<int>(),
                         qsl.data_ptr<int>(), sinks.has_value() ? sinks->data_ptr<float>() : nullptr, o.data_ptr<float>(),
                         lse.data_ptr<float>(), tk.data_ptr<int>(), s.status.data_ptr<int>(), (int)B, (int)q.size(1), (int)Hkv, (int)D,
@@ -1187,7 +1187,7 @@ void kv8_prompt(at::Tensor out, const at::Tensor& q, const at::Tensor& cache, co
   Tmap tq;
   int rc = b200_encode_tmap_heads(tq.b, q.data_ptr(), T, (int)Hq, (int)D, q.stride(0) * 2, (int)g, (int)(128 / g));
   TORCH_CHECK(rc == 0, "tensor map encode failed: ", rc);
-  const Tmap tk = kv8_tmap(cache, (int)(64 * D / 128));
+  const Tmap tk = kv8_tmap(cache, (int)D, 64);
   check(b200_kv8_prompt(out.data_ptr(), cache.data_ptr(), tq.b, tk.b, block_tables.data_ptr<int>(), seq_lens.data_ptr<int>(),
                         qsl.data_ptr<int>(), sinks.has_value() ? sinks->data_ptr<float>() : nullptr,
                         splits > 1 ? o.data_ptr<float>() : nullptr, splits > 1 ? lse.data_ptr<float>() : nullptr, splits,

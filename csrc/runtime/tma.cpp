@@ -44,24 +44,26 @@ extern "C" int b200_encode_tmap_2d(void* out, const void* base, uint64_t rows, u
   return 0;
 }
 
-// The codes of an 8-bit cache: bytes [pages][rows][max(D, 128)], boxes 128 bytes wide of as many rows as the largest power of two that
-// divides a page's, max_rows (a power of two) at most; 128-byte swizzle.
-extern "C" int b200_encode_tmap_kv8(void* out, const void* base, uint64_t pages, int block_size, int D, int max_rows) {
+// The codes of an 8-bit cache: bytes [pages][block_size * D / width][width], boxes of at most 128 bytes and of as many rows as the largest
+// power of two that divides a page's, max_rows (a power of two) at most; swizzled over the box's width (64 or 128 bytes).
+extern "C" int b200_encode_tmap_kv8(void* out, const void* base, uint64_t pages, int block_size, int D, int width, int max_rows) {
   EncodeTiledFn enc = get_encode();
   if (enc == nullptr) return 1001;
-  const uint64_t width = D < 128 ? 128 : D, rows = (uint64_t)block_size * D / width, page = (uint64_t)block_size * (D + 4);
+  const uint64_t page = (uint64_t)block_size * (D + 4);
   if ((reinterpret_cast<uintptr_t>(base) & 15) || (page & 15)) return 1002;
-  if (width % 128 || ((uint64_t)block_size * D) % width || rows == 0) return 1003;
+  if ((width % 128 && width != 64) || ((uint64_t)block_size * D) % width) return 1003;
+  const uint64_t rows = (uint64_t)block_size * D / width;
   uint64_t box_rows = rows & (~rows + 1);
+  if (box_rows == 0) return 1003;
   if (box_rows > (uint64_t)max_rows) box_rows = max_rows;
   CUtensorMap tm;
-  cuuint64_t dims[3] = {width, rows, pages};
-  cuuint64_t strides[2] = {width, page};
-  cuuint32_t box[3] = {128, (cuuint32_t)box_rows, 1};
+  cuuint64_t dims[3] = {(cuuint64_t)width, rows, pages};
+  cuuint64_t strides[2] = {(cuuint64_t)width, page};
+  cuuint32_t box[3] = {(cuuint32_t)(width < 128 ? width : 128), (cuuint32_t)box_rows, 1};
   cuuint32_t estr[3] = {1, 1, 1};
   CUresult r = enc(&tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
-                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, width == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return 2000 + (int)r;
   memcpy(out, &tm, sizeof(tm));
   return 0;
