@@ -19,16 +19,8 @@
 // 512 threads: warp 0 TMA producer (a lane per 16 keys), warp 1 MMA issuer, warps 4-7 / 8-11 queries, softmax and epilogue of stream 0 / 1
 // (thread = row), warps 12-15 widening.  The grid has a CTA per item, in descending order of row blocks; a CTA that is done takes the next
 // pending one's item (cluster launch control).  Every wait is bounded; on time-out the status word is set and the CTA unwinds.
-#include <cuda.h>
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-#include <math.h>
-
 #include "../api.h"
-#include "../common/kv8.cuh"
-#include "../common/launch.cuh"
-#include "../common/ptx.cuh"
-#include "../gemm/gemm_common.cuh"
+#include "kv8_prompt.cuh"
 
 namespace b200 {
 namespace kv8prompt {
@@ -37,12 +29,8 @@ constexpr int kThreads = 4 * 128;
 // Registers a thread of the first and the last warpgroup keeps and one of the softmax warpgroups gets: the launch brings 512 x 128 =
 // 65536, and the split takes 128 x (64 + 192 + 192 + 64) = 65536.
 constexpr int kRegsFew = 64, kRegsSoft = 192;
-constexpr int kTile = 128, kPage = 64;
 constexpr int kVStages = 4;                              // V pages as operands
 constexpr int kRing = 4;                                 // K scales and valid masks: one more than the K stages
-constexpr int kTmemCols = 512;
-constexpr float kMaxSlack = 8.f;
-constexpr float kLog2e = 1.4426950408889634f;
 
 template <typename T> struct Pieces;
 template <> struct Pieces<__nv_bfloat16> { static constexpr int n = 2; };
@@ -61,111 +49,6 @@ template <typename T, int D> struct Cfg {
   static_assert(kSmem <= 227 * 1024 && kKStages < kRing);
 };
 
-struct Params {
-  void* out;                // [T, Hq, D]
-  float* ws_o;              // [splits][T][Hq][D]
-  float* ws_lse;            // [splits][T][Hq], log2
-  const uint8_t* cache;
-  const int* block_tables;
-  const int* seq_lens;
-  const int* qsl;
-  const float* sinks;
-  int* status;
-  int64_t num_blocks, bt_stride, T;
-  int B, Hq, Hkv, g, block_size, max_blocks, window;
-  int toks;                 // tokens of a tile
-  int single;               // one stream a CTA
-  int row_blocks, splits;
-  int take;                 // CTAs may be pending: whoever is done takes their items
-  float scale_log2;
-};
-
-__device__ __forceinline__ void tmem_ld_x32_p(uint32_t taddr, uint32_t* r) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr)
-      : "memory");
-}
-__device__ __forceinline__ void tmem_st_x32_p(uint32_t taddr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-      : "memory");
-}
-__device__ __forceinline__ void tmem_st_x16_p(uint32_t taddr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
-}
-// D[tmem] (+)= A[tmem] * B[smem]; issued by ONE thread.  A: lane = row, two 16-bit elements of K per column.
-__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
-                                            uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-      ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-// two fp32 values in one 64-bit register: a fused multiply-add or an add of both is one instruction
-__device__ __forceinline__ uint64_t f2(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void unf2(uint64_t r, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r)); }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ uint16_t f16x2_to_e4m3x2(__half2 v) {
-  uint16_t r;
-  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(*reinterpret_cast<const uint32_t*>(&v)));
-  return r;
-}
-// 2^x on the special-function unit (-inf -> 0)
-__device__ __forceinline__ float ex2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
-template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
-  uint32_t d;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
-  return d;
-}
-template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
-  uint32_t d;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
-  return d;
-}
-
 // four codes -> four fp16 values times a power of two, exact
 __device__ __forceinline__ void widen4(uint32_t w, __half2 f, uint32_t& lo, uint32_t& hi) {
   const uint32_t a = e4m3x2_to_f16x2((uint16_t)w), b = e4m3x2_to_f16x2((uint16_t)(w >> 16));
@@ -183,62 +66,6 @@ __device__ __forceinline__ uint64_t desc_rows(uint32_t addr) {
 template <int D>
 __device__ __forceinline__ int chunk_at(int r, int c) {
   return D == 128 ? r * 128 + ((c ^ (r & 7)) << 4) : r * 64 + ((c ^ (r >> 1 & 3)) << 4);
-}
-
-// One work item: what the two streams of a CTA share and their own rows.
-struct Item {
-  int req, qs, q_len, ctx, seq_len, key0, head, split;     // key0: first key of the first tile
-  int tok0[2], toks[2], n[2];                              // per stream: first token within the request, tokens, key tiles
-  int n_max;
-};
-// Items are ordered by descending row block, so by descending number of key tiles for prompts of one length.
-__device__ __forceinline__ void get_item(const Params& p, int idx, Item& it) {
-  const int heads = p.Hkv * p.splits, per = p.B * heads, rb = p.row_blocks - 1 - idx / per, rem = idx % per;
-  it.req = rem / heads;
-  it.head = rem % heads / p.splits;
-  it.split = rem % p.splits;
-  it.qs = p.qsl[it.req];
-  it.q_len = p.qsl[it.req + 1] - it.qs;
-  it.seq_len = p.seq_lens[it.req];
-  it.ctx = it.seq_len - it.q_len;
-  const int step = p.single ? p.toks : 2 * p.toks;
-  int all[2];
-  int kv_begin = 0;
-#pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    it.tok0[s] = rb * step + s * p.toks;
-    it.toks[s] = (s == 1 && p.single) ? 0 : max(0, min(p.toks, it.q_len - it.tok0[s]));
-    // a window hides everything in front of the first token's first visible key (whole tiles of it)
-    if (s == 0) kv_begin = p.window > 0 ? max(0, it.ctx + it.tok0[0] - p.window + 1) / kTile * kTile : 0;
-    // keys visible to the tile end with the position of its last token; rows that see nothing have a tile all the same
-    const int kv_end = min(it.seq_len, it.ctx + it.tok0[s] + it.toks[s]);
-    all[s] = it.toks[s] > 0 ? max(1, (kv_end - kv_begin + kTile - 1) / kTile) : 0;
-  }
-  const int each = (max(all[0], all[1]) + p.splits - 1) / p.splits, first = it.split * each;
-#pragma unroll
-  for (int s = 0; s < 2; ++s) it.n[s] = max(0, min(all[s] - first, each));
-  it.key0 = kv_begin + first * kTile;
-  it.n_max = max(it.n[0], it.n[1]);
-}
-
-// Asks for the index of a CTA of this grid that has not been started, which then never will be: 16 bytes at `dst`, complete_tx on `bar`.
-__device__ __forceinline__ void ask_for_cta(uint32_t dst, uint64_t* bar) {
-  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(dst),
-               "r"(smem_u32(bar)) : "memory");
-}
-// The answer: a CTA's index, or -1 when all have been started or taken (then no further question may be asked).
-__device__ __forceinline__ int taken_cta(uint32_t src) {
-  uint32_t ok, x = 0;
-  asm volatile(
-      "{\n\t.reg .b128 r;\n\t.reg .b64 lo, hi;\n\t.reg .pred p;\n\t"
-      "ld.shared.v2.b64 {lo, hi}, [%2];\n\t"
-      "mov.b128 r, {lo, hi};\n\t"
-      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t"
-      "mov.u32 %1, 0;\n\t"
-      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t}"
-      : "=r"(ok), "=r"(x) : "r"(src) : "memory");
-  return ok ? (int)x : -1;
 }
 
 // What a page of V is, for the widening warps: bits 0-3 which 16 keys were read, 4-10 keys in front of the request's end, 12 the end of
@@ -348,7 +175,7 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       return true;
     };
     for (int idx = blockIdx.x; ok && idx >= 0;) {
-      get_item(p, idx, it);
+      get_item<kTile>(p, idx, it);
       const int n_max = it.n_max;
       if (n_max > 0) {
         if (qc > 0 && !wait_all(q_empty, (qc - 1) & 1, 920)) { ok = false; break; }
@@ -463,7 +290,7 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       int kc = 0, vc = 0, qc[2] = {0, 0}, tc[2] = {0, 0};   // consumed so far; tc: tiles of each stream whose P has been awaited
       bool ok = true;
       for (int idx = blockIdx.x, round = 0; idx >= 0; idx = ok ? next_item(round++, false, ok) : -1) {
-        get_item(p, idx, it);
+        get_item<kTile>(p, idx, it);
         if (it.n_max == 0) continue;
         const int n_max = it.n_max;
         // S of tile j of the item; the last reader of a K stage (of Q) gives it back
@@ -599,7 +426,7 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     bool fail = false;
     bool ok = true;
     for (int idx = blockIdx.x, round = 0; idx >= 0; idx = next_item(round++, true, ok)) {
-      get_item(p, idx, it);
+      get_item<kTile>(p, idx, it);
       const int n = s ? it.n[1] : it.n[0], tok0 = s ? it.tok0[1] : it.tok0[0], toks = s ? it.toks[1] : it.toks[0];
       const bool row_ok = r_tok < toks;                // toks <= 128 / g
       const int64_t orow = (int64_t)(it.qs + tok0 + r_tok) * p.Hq + it.head * p.g + r_head;
@@ -791,42 +618,6 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   }
 }
 
-// Joins the splits of a row: out = sum_s w_s O_s / (sum_s w_s [+ sink]), w_s = 2^(lse_s - max).  A warp per (token, head).
-template <typename T, int D>
-__global__ void __launch_bounds__(256)
-kv8_join_kernel(T* __restrict__ out, const float* __restrict__ ws_o, const float* __restrict__ ws_lse, const float* __restrict__ sinks,
-                int64_t rows, int Hq, int splits, const int* __restrict__ qsl, int B) {
-  griddep_launch();
-  griddep_wait();
-  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (row >= rows || row / Hq < qsl[0] || row / Hq >= qsl[B]) return;
-  constexpr int N = D / 32;
-  const float mine = lane < splits ? ws_lse[lane * rows + row] : -INFINITY;      // at most 32 splits
-  const float M = warp_max(mine), Ms = M == -INFINITY ? 0.f : M;
-  float w = mine == -INFINITY ? 0.f : exp2f(mine - Ms);
-  float den = warp_sum(w);
-  if (sinks != nullptr) den += exp2f(sinks[row % Hq] * kLog2e - Ms);
-  w = den == 0.f ? 0.f : w / den;
-  float acc[N];
-#pragma unroll
-  for (int j = 0; j < N; ++j) acc[j] = 0.f;
-  for (int s = 0; s < splits; ++s) {
-    const float ws = __shfl_sync(0xffffffffu, w, s);
-    if (ws == 0.f) continue;             // an empty split's row may hold anything
-    const float* src = ws_o + (s * rows + row) * D + lane * N;
-#pragma unroll
-    for (int j = 0; j < N; j += 2) {
-      const float2 v = *reinterpret_cast<const float2*>(src + j);
-      acc[j] += ws * v.x;
-      acc[j + 1] += ws * v.y;
-    }
-  }
-  uint32_t* dst = reinterpret_cast<uint32_t*>(out + row * D + lane * N);
-#pragma unroll
-  for (int j = 0; j < N; j += 2) dst[j / 2] = pack2<T>(acc[j], acc[j + 1]);
-}
-
 template <typename T, int D>
 static int launch(const Params& p, const CUtensorMap& tmQ, const CUtensorMap& tmKV, int64_t items, cudaStream_t st) {
   auto kern = kv8_prompt_kernel<T, D>;
@@ -872,6 +663,7 @@ extern "C" int b200_kv8_prompt(void* out, const void* cache, const void* tmQ, co
   p.out = out; p.ws_o = ws_o; p.ws_lse = ws_lse; p.cache = static_cast<const uint8_t*>(cache); p.block_tables = block_tables;
   p.seq_lens = seq_lens; p.qsl = qsl; p.sinks = sinks; p.status = status; p.num_blocks = num_blocks; p.bt_stride = bt_stride;
   p.T = T_; p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.g = Hq / Hkv; p.block_size = block_size; p.max_blocks = max_blocks; p.window = window;
+  p.max_keys = 0x7fffff80;
   p.toks = kv8prompt::kTile / p.g; p.splits = splits; p.scale_log2 = scale * kv8prompt::kLog2e;
   const int64_t tiles = (int64_t)B * Hkv * ((max_query_len + p.toks - 1) / p.toks);
   p.single = tiles * splits <= num_sms;

@@ -1166,10 +1166,12 @@ void kv8_decode(at::Tensor out, const at::Tensor& q, const at::Tensor& cache, co
                         max_seq_len, (int)window, (float)scale, q.stride(0), early_meta ? 1 : 0, dtype_code(q), s.num_sms, stream()),
         "kv8_decode");
 }
-// More rows than that: prompts and chunks.
+// More rows than that: prompts and chunks.  `wide`: keys and values of all requests in 16 bits first (scratch), otherwise widened by the
+// attention kernel.  The scratch is bounded: a batch that needs more is worked on request by request group.
+constexpr int64_t kKv8Scratch = 1LL << 30;
 void kv8_prompt(at::Tensor out, const at::Tensor& q, const at::Tensor& cache, const at::Tensor& block_tables,
                 const at::Tensor& seq_lens, const at::Tensor& qsl, const c10::optional<at::Tensor>& sinks, int64_t max_query_len,
-                int64_t max_seq_len, int64_t window, double scale) {
+                int64_t max_seq_len, int64_t window, double scale, bool wide) {
   check_kv8_attention(out, q, cache, block_tables, seq_lens, qsl, sinks);
   if (q.size(0) == 0 || seq_lens.size(0) == 0) return;
   c10::cuda::CUDAGuard guard(q.device());
@@ -1178,22 +1180,49 @@ void kv8_prompt(at::Tensor out, const at::Tensor& q, const at::Tensor& cache, co
   Kv8State& s = kv8_state(gs, q);
   const int64_t B = seq_lens.size(0), T = q.size(0), Hq = q.size(1), Hkv = cache.size(2), D = q.size(2), g = Hq / Hkv;
   TORCH_CHECK(g <= 128, "kv8_prompt: ", g, " heads a group");
-  const int splits = b200_kv8_prompt_splits((int)B, (int)Hq, (int)Hkv, (int)max_query_len, max_seq_len, (int)window, s.num_sms);
-  at::Tensor o, lse;
-  if (splits > 1) {
-    o = at::empty({splits, T, Hq, D}, q.options().dtype(at::kFloat));
-    lse = at::empty({splits, T, Hq}, q.options().dtype(at::kFloat));
-  }
-  Tmap tq;
+  Tmap tq, tk, tv;
   int rc = b200_encode_tmap_heads(tq.b, q.data_ptr(), T, (int)Hq, (int)D, q.stride(0) * 2, (int)g, (int)(128 / g));
   TORCH_CHECK(rc == 0, "tensor map encode failed: ", rc);
-  const Tmap tk = kv8_tmap(cache, (int)D, 64);
-  check(b200_kv8_prompt(out.data_ptr(), cache.data_ptr(), tq.b, tk.b, block_tables.data_ptr<int>(), seq_lens.data_ptr<int>(),
-                        qsl.data_ptr<int>(), sinks.has_value() ? sinks->data_ptr<float>() : nullptr,
-                        splits > 1 ? o.data_ptr<float>() : nullptr, splits > 1 ? lse.data_ptr<float>() : nullptr, splits,
-                        s.status.data_ptr<int>(), T, (int)B, (int)Hq, (int)Hkv, (int)D, (int)cache.size(3), (int)block_tables.size(1),
-                        block_tables.stride(0), cache.size(0), (int)max_query_len, (int)window, (float)scale, dtype_code(q), s.num_sms,
-                        stream()), "kv8_prompt", splits > 1 ? 2 : 1);
+  const float* sk = sinks.has_value() ? sinks->data_ptr<float>() : nullptr;
+  // rows per request and head: no more than the block tables can name
+  const int64_t longest = std::max<int64_t>(1, std::min(max_seq_len, block_tables.size(1) * cache.size(3)));
+  const int64_t rows = wide ? (longest + 127) / 128 * 128 : 0;
+  const int64_t per = Hkv * rows * D * 2;
+  const int64_t group = wide ? std::min(B, std::max<int64_t>(1, kKv8Scratch / (2 * per))) : B;
+  at::Tensor o, lse, wk, wv, ok;
+  if (wide) {
+    wk = at::empty({group, Hkv, rows, D}, q.options());
+    wv = at::empty({group, Hkv, rows, D}, q.options().dtype(at::kHalf));
+    ok = at::empty({group, rows / 128}, q.options().dtype(at::kByte));
+    rc = b200_encode_tmap_2d(tk.b, wk.data_ptr(), group * Hkv * rows, D, D * 2, D == 256 ? 64 : 128, 64, 2);
+    if (rc == 0) rc = b200_encode_tmap_2d(tv.b, wv.data_ptr(), group * Hkv * rows, D, D * 2, 64, 64, 2);
+    TORCH_CHECK(rc == 0, "tensor map encode failed: ", rc);
+  } else {
+    tk = kv8_tmap(cache, (int)D, 64);
+  }
+  for (int64_t b0 = 0; b0 < B; b0 += group) {
+    const int n = (int)std::min(group, B - b0);
+    const int splits = b200_kv8_prompt_splits(n, (int)Hq, (int)Hkv, (int)max_query_len, max_seq_len, (int)window, s.num_sms);
+    if (splits > 1 && (!o.defined() || o.size(0) < splits)) {
+      o = at::empty({splits, T, Hq, D}, q.options().dtype(at::kFloat));
+      lse = at::empty({splits, T, Hq}, q.options().dtype(at::kFloat));
+    }
+    float* po = splits > 1 ? o.data_ptr<float>() : nullptr;
+    float* pl = splits > 1 ? lse.data_ptr<float>() : nullptr;
+    const int* bt = block_tables.data_ptr<int>() + b0 * block_tables.stride(0);
+    const int* sl = seq_lens.data_ptr<int>() + b0;
+    const int* ql = qsl.data_ptr<int>() + b0;
+    if (wide)
+      rc = b200_kv8_wide(out.data_ptr(), cache.data_ptr(), tq.b, tk.b, tv.b, wk.data_ptr(), wv.data_ptr(), ok.data_ptr(), (int)rows, bt, sl,
+                         ql, sk, po, pl, splits, s.status.data_ptr<int>(), T, n, (int)Hq, (int)Hkv, (int)D, (int)cache.size(3),
+                         (int)block_tables.size(1), block_tables.stride(0), cache.size(0), (int)max_query_len, (int)window, (float)scale,
+                         dtype_code(q), s.num_sms, stream());
+    else
+      rc = b200_kv8_prompt(out.data_ptr(), cache.data_ptr(), tq.b, tk.b, bt, sl, ql, sk, po, pl, splits, s.status.data_ptr<int>(), T, n,
+                           (int)Hq, (int)Hkv, (int)D, (int)cache.size(3), (int)block_tables.size(1), block_tables.stride(0),
+                           cache.size(0), (int)max_query_len, (int)window, (float)scale, dtype_code(q), s.num_sms, stream());
+    check(rc, "kv8_prompt", 1 + (wide ? 1 : 0) + (splits > 1 ? 1 : 0));
+  }
 }
 void kv8_attention_generic(at::Tensor out, const at::Tensor& q, const at::Tensor& cache, const at::Tensor& block_tables,
                            const at::Tensor& seq_lens, const at::Tensor& qsl, const c10::optional<at::Tensor>& sinks, int64_t window,

@@ -1,7 +1,7 @@
 """CUDA attention over the 8-bit paged cache (``csrc/attention/kv8_*.cu``).
 
 A batch is decode-first, as in :func:`ops.paged_attention`: requests with few query rows per key / value head go to the decode
-kernel, the others to the prompt kernel; what neither takes (fp32 models, other head or block sizes) to the generic one.
+kernel, the others to the prompt kernels; what neither takes (fp32 models, other head or block sizes) to the generic one.
 """
 from __future__ import annotations
 
@@ -42,8 +42,10 @@ def _attend(out, q, kv_cache, block_tables, seq_lens, query_start_loc, scale, ma
             _ext.C().kv8_decode(out, q, kv_cache, block_tables, seq_lens, query_start_loc, sinks, *ws, max_query_len, max_seq_len,
                                 window, scale, stable_metadata)
             return
-        if D in (64, 128) and group <= 128 and scale > 0:
+        if D in (64, 128, 256) and group <= 128 and scale > 0:
+            # widened once for all query tiles where more than one pair of them (128 // group tokens each) reads the same keys
+            wide = D == 256 or max_query_len > 2 * (128 // group)
             _ext.C().kv8_prompt(out, q, kv_cache, block_tables, seq_lens, query_start_loc, sinks, max_query_len, max_seq_len, window,
-                                scale)
+                                scale, wide)
             return
     _ext.C().kv8_attention_generic(out, q, kv_cache, block_tables, seq_lens, query_start_loc, sinks, window, scale)
