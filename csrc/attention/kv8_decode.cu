@@ -19,8 +19,10 @@
 // Work: all tiles of all (request, head) items in one line, cut into equal pieces, one a CTA (two CTAs an SM where shared memory lasts), so
 // that uneven requests cost what their sum costs.  Where a cut falls, from the lengths on the device: captured launches adapt.  An item
 // that lies in several CTAs is merged by the last of them to arrive, in the order of the cuts: the result does not depend on who that is.
-// 224 threads: warp 0 TMA producer (a lane per box of a tile, which looks its block up a tile ahead), warp 1 MMA issuer, warps 2-5 softmax
-// (thread = row of the tile; TMEM lane = output dim at the end), warp 6 queries.  Every wait is bounded; on time-out the status word is
+// 192 or 320 threads: warp 0 TMA producer (a lane per box of a tile, which looks its block up a tile ahead), warp 1 MMA issuer, the others
+// softmax (thread = row of the tile; TMEM lane = output dim at the end) and queries: four warps, or, where a row of the tile brings 16 scores
+// or more, eight, which share them by query rows (heads of 64: by keys of a row).  What is done once an item is kept short in code as well as in
+// time: half of a call's time went into it before, most of that into fetching instructions.  Every wait is bounded; on time-out the status word is
 // set and the CTA unwinds.
 #include <cuda.h>
 #include <math.h>
@@ -34,11 +36,9 @@
 namespace b200 {
 namespace kv8dec {
 
-constexpr int kThreads = 224;
 constexpr int kM = 128;          // rows of 128 bytes in a tile
 constexpr int kRows = 16;        // query rows, zero padded
 constexpr int kMaxB = 2048;      // requests a launch
-constexpr int kFactors = 4;      // ring of query factors: S runs at most two tiles ahead of the softmax
 constexpr float kSlack = 1.f;    // the running maximum moves when a score exceeds it by more (log2): weights stay below 2^(7 + 1)
 constexpr float kLift = 7.f;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -56,7 +56,7 @@ struct Params {
   const float* sinks;
   int* status;
   int64_t num_blocks, bt_stride, q_stride;
-  int B, Hq, Hkv, block_size, max_blocks, window, slots, early_meta, min_tiles;
+  int B, Hq, Hkv, block_size, max_blocks, max_keys, window, slots, early_meta, min_tiles;
   float scale_log2;
 };
 
@@ -71,11 +71,16 @@ template <typename T> struct Pieces;
 template <> struct Pieces<__nv_bfloat16> { static constexpr int n = 2; };
 template <> struct Pieces<__half> { static constexpr int n = 3; };
 
-template <typename T, int D> struct Layout {
+template <typename T, int D, int NR> struct Layout {
   using G = Geo<D>;
   static constexpr int P = Pieces<T>::n;
+  static constexpr int kGroups = NR * G::kPack >= 16 ? 2 : 1;  // groups of four softmax warps
+  static constexpr int kSoft = 128 * kGroups, kThreads = 64 + kSoft;
+  static constexpr int kCtas = D == 256 || (D == 64 && kGroups == 2) ? 1 : 2;   // an SM at most: shared memory, registers
+  static constexpr int kKeysOf = G::kPack / (G::kPack == 2 ? kGroups : 1);       // keys and query rows of a thread
+  static constexpr int kRowsOf = NR / (G::kPack == 1 ? kGroups : 1);
   static constexpr int kNO = G::kNS * P;                       // columns of an O^T accumulator
-  static constexpr int kQ = P * G::kBlk * G::kNS * 128;        // one query buffer
+  static constexpr int kQ = P * G::kBlk * G::kNS * 128;        // queries
   static constexpr int kP = kNO * 128;                         // one weight buffer
   static constexpr int kCols = 2 * G::kNS + G::kBlk * kNO;
   static constexpr int kTmem = kCols <= 64 ? 64 : kCols <= 128 ? 128 : 256;
@@ -83,7 +88,7 @@ template <typename T, int D> struct Layout {
   // barriers, factors, flags, exchange buffers
   static constexpr int kMisc = 4096 + (D == 64 ? kRows * 64 * 4 : 0);
   static size_t smem(int slots, int B) {
-    return 1024 + (size_t)slots * (G::kOp + kScales) + 2 * kQ + 2 * kP + kMisc + (size_t)(B + 1) * 4;
+    return 1024 + (size_t)slots * (G::kOp + kScales) + kQ + 2 * kP + kMisc + (size_t)(B + 1) * 4;
   }
 };
 
@@ -96,8 +101,13 @@ __device__ __forceinline__ float warp_max_redux(float v) {
   return __int_as_float(i);
 }
 // into the registers themselves: no copy may come before the wait
+__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&r)[8]) { tmem_ld_x8(taddr, r); }
 __device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld_x16(taddr, r); }
-__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld_x32(taddr, r); }
+__device__ __forceinline__ void tmem_st_x8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
 __device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
@@ -115,25 +125,26 @@ __device__ __forceinline__ __half2 as_half2(uint32_t v) { return *reinterpret_ca
 // A CTA's share of the line of tiles, item by item.
 struct Walk {
   const int* pre;          // [B + 1] tiles of the requests in front (of one head)
-  long long at, end;       // units left
+  int at, end;             // units left
   int Hkv, B;
   int req, head, tile, n;  // current item: its tiles, and the first of this CTA's among them
   int count;               // this CTA's tiles of it
-  __device__ __forceinline__ void start(const int* pre_, int B_, int Hkv_, long long lo, long long hi) {
+  __device__ __forceinline__ void start(const int* pre_, int B_, int Hkv_, int lo, int hi) {
     pre = pre_; B = B_; Hkv = Hkv_; at = lo; end = hi;
     count = 0;
     if (at >= end) return;
     int a = 0, b = B;      // the last request whose tiles start at or before `at`: those without tiles lie in front of it
+#pragma unroll 1
     while (b - a > 1) {
       const int mid = (a + b) >> 1;
-      if ((long long)pre[mid] * Hkv <= at) a = mid; else b = mid;
+      if (pre[mid] * Hkv <= at) a = mid; else b = mid;
     }
     req = a;
     n = pre[a + 1] - pre[a];
-    const long long in = at - (long long)pre[a] * Hkv;
-    head = (int)(in / n);
-    tile = (int)(in % n);
-    count = (int)min((long long)(n - tile), end - at);
+    const unsigned in = at - pre[a] * Hkv;
+    head = in / (unsigned)n;
+    tile = in - head * n;
+    count = min(n - tile, end - at);
   }
   __device__ __forceinline__ bool more() const { return count > 0; }
   __device__ __forceinline__ void next() {
@@ -143,9 +154,10 @@ struct Walk {
     tile = 0;
     if (++head == Hkv) {
       head = 0;
+#pragma unroll 1
       do { ++req; n = pre[req + 1] - pre[req]; } while (n == 0);
     }
-    count = (int)min((long long)n, end - at);
+    count = min(n, end - at);
   }
 };
 
@@ -164,41 +176,40 @@ __device__ __forceinline__ Request request_of(const Params& p, int req) {
 }
 
 template <typename T, int D, int NR>
-__global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2)
+__global__ void __launch_bounds__((Layout<T, D, NR>::kThreads), (Layout<T, D, NR>::kCtas))
 kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ Params p) {
   using G = Geo<D>;
-  using L = Layout<T, D>;
-  constexpr int P = L::P, kPack = G::kPack, kBlk = G::kBlk, kKeys = G::kKeys, kNS = G::kNS, kNO = L::kNO;
+  using L = Layout<T, D, NR>;
+  constexpr int P = L::P, kPack = G::kPack, kBlk = G::kBlk, kKeys = G::kKeys, kNS = G::kNS, kNO = L::kNO, kSoft = L::kSoft, kWarps = kSoft / 32;
+  constexpr int kKeysOf = L::kKeysOf, kRowsOf = L::kRowsOf, kThreads = L::kThreads;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int ns = p.slots;
-  uint8_t* sQ = smem + ns * G::kOp;                          // [2][P][kBlk][kNS][128 B]
-  uint8_t* sP = sQ + 2 * L::kQ;                              // [2][kNO][128 B]
+  uint8_t* sQ = smem + ns * G::kOp;                          // [P][kBlk][kNS][128 B]
+  uint8_t* sP = sQ + L::kQ;                                  // [2][kNO][128 B]
   float* sScale = reinterpret_cast<float*>(sP + 2 * L::kP);  // [ns][kKeys]
   uint64_t* bars = reinterpret_cast<uint64_t*>(sScale + ns * kKeys);
   uint64_t* kv_full = bars;              // [16]
-  uint64_t* kv_empty = bars + 16;        // [16] the product that reads the codes, and four warps that read the scales
+  uint64_t* kv_empty = bars + 16;        // [16] the product that reads the codes, and the warps that read the scales
   uint64_t* s_full = bars + 32;          // [2]
   uint64_t* s_empty = bars + 34;         // [2]
   uint64_t* p_ready = bars + 36;         // [2]
   uint64_t* p_free = bars + 38;          // [2]
-  uint64_t* q_full = bars + 40;          // [2]
-  uint64_t* q_empty = bars + 42;         // [2]
-  uint64_t* o_done = bars + 44;          // a phase per tile
-  uint64_t* o_final = bars + 45;         // a phase per item
-  uint64_t* f_full = bars + 46;          // [kFactors] factors, and q_full for those who may come two items late
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 46 + kFactors);
+  uint64_t* q_ready = bars + 40;         // a phase per item
+  uint64_t* o_done = bars + 41;          // a phase per tile
+  uint64_t* o_final = bars + 42;         // a phase per item
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 44);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  volatile int* ok_slot = abort_flag + 1;                    // [4]
-  int* s_last = const_cast<int*>(abort_flag) + 5;
-  uint32_t* sValid = tmem_slot + 8;                          // [16] boxes of a K slot that were read
+  volatile int* ok_slot = abort_flag + 1;                    // [8]
+  int* s_last = const_cast<int*>(abort_flag) + 9;
+  uint32_t* sValid = tmem_slot + 12;                         // [16] boxes of a K slot that were read
   uint32_t* sOdd = sValid + 16;                              // [16] heads of 64: 1 + the row of a K slot whose second key is behind the end
-  float* sFactor = reinterpret_cast<float*>(sOdd + 16);    // [kFactors][16]
-  float* sMax = sFactor + kFactors * kRows;                  // [4 warps][17]
-  float* sSum = sMax + 4 * 17;                               // [4][16]
-  float* sInv = sSum + 4 * kRows;                            // [16]
+  float* sFactor = reinterpret_cast<float*>(sOdd + 16);      // [2 items][16]
+  float* sMax = sFactor + 2 * kRows;                         // [8 warps][17]
+  float* sSum = sMax + 8 * 17;                               // [8][16]
+  float* sInv = sSum + 8 * kRows;                            // [16]
   float* sW = sInv + kRows;                                  // [32][16]
-  int* sScan = reinterpret_cast<int*>(sW);                   // [8] (before the first item)
+  int* sScan = reinterpret_cast<int*>(sW);                   // [10] (before the first item)
   float* sHalf = sW + 32 * kRows;                            // [16][64] (heads of 64)
   int* sPre = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(bars) + L::kMisc);   // [B + 1]
 
@@ -206,13 +217,12 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
   Abort ab{p.status, abort_flag};
   if (threadIdx.x == 0) {
     *abort_flag = 0;
-    for (int s = 0; s < ns; ++s) { mbar_init(&kv_full[s], 1); mbar_init(&kv_empty[s], 5); }
+    for (int s = 0; s < ns; ++s) { mbar_init(&kv_full[s], 1); mbar_init(&kv_empty[s], 1 + kWarps); }
     for (int b = 0; b < 2; ++b) {
-      mbar_init(&s_full[b], 1); mbar_init(&s_empty[b], 4);
-      mbar_init(&p_ready[b], 4); mbar_init(&p_free[b], 1);
-      mbar_init(&q_full[b], 1); mbar_init(&q_empty[b], 1);
+      mbar_init(&s_full[b], 1); mbar_init(&s_empty[b], kWarps);
+      mbar_init(&p_ready[b], kWarps); mbar_init(&p_free[b], 1);
     }
-    for (int b = 0; b < kFactors; ++b) mbar_init(&f_full[b], 1);
+    mbar_init(q_ready, kWarps);
     mbar_init(o_done, 1);
     mbar_init(o_final, 1);
     mbar_fence_init();
@@ -224,21 +234,23 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
     tmem_relinquish();
   }
   // columns of queries and weights that no row uses, and the halves of heads of 64, stay zero
-  for (int c = threadIdx.x; c < (2 * L::kQ + 2 * L::kP) / 16; c += kThreads) reinterpret_cast<uint4*>(sQ)[c] = make_uint4(0, 0, 0, 0);
+  for (int c = threadIdx.x; c < (L::kQ + 2 * L::kP) / 16; c += kThreads) reinterpret_cast<uint4*>(sQ)[c] = make_uint4(0, 0, 0, 0);
   fence_proxy_async_smem();
 
   // With early_meta lengths and block tables were written long before this launch, and old tokens' rows as well: both are read before
   // the wait for the kernels in front.
   if (!p.early_meta) griddep_wait();
+  const int g = p.Hq / p.Hkv;
   {
     // tiles of every request, summed up over those in front: a thread has consecutive requests
     const int per = (p.B + kThreads - 1) / kThreads, lo = min(p.B, (int)threadIdx.x * per), hi = min(p.B, lo + per);
     int sum = 0;
     for (int r = lo; r < hi; ++r) {
       const Request q = request_of<D>(p, r);
-      const bool served = q.q_len > 0 && q.q_len * (p.Hq / p.Hkv) <= NR;
+      const bool served = q.q_len > 0 && q.q_len * g <= NR;
       // a request whose rows see nothing has a tile all the same: it writes their zeros
-      const int n = served ? max(1, (q.seq_len - q.kv_begin + kKeys - 1) / kKeys) : 0;
+      const int end = min(q.seq_len, p.max_keys);      // the block table has no more
+      const int n = served ? max(1, (end - q.kv_begin + kKeys - 1) / kKeys) : 0;
       sPre[r + 1] = n;
       sum += n;
     }
@@ -260,11 +272,10 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
 
-  const int g = p.Hq / p.Hkv;
-  const long long units = (long long)sPre[p.B] * p.Hkv;
-  const long long share = max((units + gridDim.x - 1) / gridDim.x, (long long)p.min_tiles);
-  const long long lo = min(units, share * blockIdx.x), hi = min(units, lo + share);
-  const int n_tiles = (int)(hi - lo);
+  const int units = sPre[p.B] * p.Hkv;
+  const int share = max((units + (int)gridDim.x - 1) / (int)gridDim.x, p.min_tiles);
+  const int lo = min((long long)units, (long long)share * blockIdx.x), hi = min(units - lo, share) + lo;
+  const int n_tiles = hi - lo;
   Walk it;
   it.start(sPre, p.B, p.Hkv, lo, hi);
 
@@ -352,7 +363,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
       uint32_t spins = 0;
       while (next_pv < n_tiles) {
         bool progressed = false;
-        if (next_s < n_tiles && next_s <= next_pv + 1 && (s_in > 0 || mbar_try_wait(&q_full[s_item & 1], (s_item >> 1) & 1)) &&
+        if (next_s < n_tiles && next_s <= next_pv + 1 && (s_in > 0 || mbar_try_wait(q_ready, s_item & 1)) &&
             mbar_try_wait(&kv_full[ks], kph) &&
             (next_s < 2 || mbar_try_wait(&s_empty[next_s & 1], ((next_s >> 1) - 1) & 1))) {
           tc_fence_after_sync();
@@ -364,7 +375,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
               *reinterpret_cast<uint4*>(smem + ks * G::kOp + row * 128 + ((c ^ (row & 7)) << 4)) = make_uint4(0, 0, 0, 0);
             fence_proxy_async_smem();
           }
-          const uint32_t k_at = kv_addr + ks * G::kOp, q_at = q_addr + (s_item & 1) * L::kQ;
+          const uint32_t k_at = kv_addr + ks * G::kOp, q_at = q_addr;
 #pragma unroll
           for (int c = 0; c < P * kBlk * 4; ++c) {
             const int piece = c / (kBlk * 4), b = (c / 4) % kBlk, k = c % 4;
@@ -377,7 +388,6 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
           if (ks >= ns) { ks -= ns; kph ^= 1; }
           ++next_s;
           if (++s_in == ws.count) {
-            umma_commit(&q_empty[s_item & 1]);
             s_in = 0;
             ++s_item;
             ws.next();
@@ -413,103 +423,100 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
         if ((spins & 255) == 255 && ab.aborted()) break;
       }
     }
-  } else if (warp == 6) {
-    // ------------------------------------------------------------------ queries in pieces
+  } else {
+    // ------------------------------------------------------------------ softmax, queries, epilogue
     if (p.early_meta) griddep_wait();
-    constexpr int kLanes = D / 8, kPass = 32 / kLanes;      // lanes of a row, rows at a time
-    const int sub = lane / kLanes, l = lane % kLanes, d = l * 8;
-    bool ok = true;
-    for (int item = 0; ok && it.more(); it.next(), ++item) {
-      const Request r = request_of<D>(p, it.req);
-      const int rows = r.q_len * g;
-      if (item >= 2) {
-        if (lane == 0) ok = wait_or_abort(&q_empty[item & 1], ((item >> 1) - 1) & 1, ab, 903);
-        ok = __shfl_sync(0xffffffffu, ok, 0);
-        if (!ok) break;
+    const int wi = warp - 2, tid = wi * 32 + lane, group = wi >> 2, quarter = warp & 3;
+    const int row_id = quarter * 32 + lane;          // TMEM lane: row of the tile, output dim
+    const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
+    const int key_of = kPack == 2 && L::kGroups == 2 ? group : 0;        // first key (of a row of the tile) and query row of this thread
+    const int row_of = kPack == 1 && L::kGroups == 2 ? group * kRowsOf : 0;
+    const uint32_t tS = tmem_base + lane_off + key_of * kRows + row_of, tO = tmem_base + 2 * kNS + lane_off + key_of * kRows + row_of;
+    const uint32_t inv_g = 65536u / g + 1;           // r / g = r * inv_g >> 16 for r < 16
+    const int page_rows = p.block_size / kPack, box_rows = min(kM, page_rows & -page_rows);
+    const uint32_t all_boxes = (1u << (kM / box_rows)) - 1;              // 16 boxes at most
+    const int my_box = row_id / box_rows;
+    const int p_off = row_id & 15, p_ch = row_id >> 4;
+
+    // ---- queries in pieces: 8 elements a thread and step, lanes of a row next to one another
+    constexpr int kLanes = D / 8, kQSteps = (NR * kLanes + kSoft - 1) / kSoft;
+    uint4 raw[kQSteps];
+    auto q_load = [&](const Walk& w, const Request& r) {
+#pragma unroll
+      for (int i = 0; i < kQSteps; ++i) {
+        const int x = i * kSoft + tid, row = x / kLanes;
+        raw[i] = make_uint4(0, 0, 0, 0);
+        if (row < r.q_len * g) {
+          const int tok = (row * inv_g) >> 16;
+          raw[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q) + (r.qs + tok) * p.q_stride +
+                                                   (int64_t)(w.head * g + row - tok * g) * D + x % kLanes * 8);
+        }
       }
-      uint8_t* dst = sQ + (item & 1) * L::kQ;
-#pragma unroll 4
-      for (int r0 = 0; r0 < NR; r0 += kPass) {
-        const int row = r0 + sub;
-        const bool in = row < rows;
-        float v[8];
-        float amax = 0.f;
-        bool bad = false;
-        if (in) {
-          const int tok = r.qs + row / g, hh = it.head * g + row % g;
-          const Vec16<T> a = ld_vec(reinterpret_cast<const T*>(p.q) + tok * p.q_stride + (int64_t)hh * D + d);
+    };
+    auto q_store = [&](int item) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            v[j] = to_f(a.v[j]);
-            bad |= !(fabsf(v[j]) <= 8.5e37f);      // infinities, NaN, and what is too large for its scale to be a number: NaN
-            amax = fmaxf(amax, fabsf(v[j]));
-          }
-        } else {
+      for (int i = 0; i < kQSteps; ++i) {
+        const int x = i * kSoft + tid, row = x / kLanes, d = x % kLanes * 8;
+        const Vec16<T> a = *reinterpret_cast<const Vec16<T>*>(&raw[i]);
+        float v[8], amax = 0.f;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = 0.f;
+        for (int j = 0; j < 8; ++j) {
+          v[j] = to_f(a.v[j]);
+          amax = fabsf(v[j]) <= 8.5e37f ? fmaxf(amax, fabsf(v[j])) : INFINITY;
         }
 #pragma unroll
-        for (int o = kLanes / 2; o > 0; o >>= 1) {
-          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-          bad |= __shfl_xor_sync(0xffffffffu, (int)bad, o) != 0;
-        }
-        const float top = bad ? 1.f : pow2_ceil(fmaxf(amax, 1e-30f));
-        const float up = bad ? 0.f : 256.f * pow2_inv(top);
-        if (l == 0) sFactor[(item % kFactors) * kRows + row] = bad ? __uint_as_float(0x7fffffffu) : top * (1.f / 256.f) * p.scale_log2;
+        for (int o = kLanes / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        // infinities, NaN, and what is too large for its scale to be a number: NaN
+        const bool bad = amax == INFINITY;
+        const float top = bad ? 1.f : pow2_ceil(fmaxf(amax, 1e-30f)), up = 256.f * pow2_inv(top);
+        if (row >= NR) continue;       // whole warps, or the same lanes of every exchange above
+        if (d == 0) sFactor[(item & 1) * kRows + row] = bad ? __uint_as_float(0x7fffffffu) : top * (1.f / 256.f) * p.scale_log2;
+        __half2 rest[4];               // at most 256: fp16 holds it
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = bad ? 0.f : v[j] * up;
+        for (int j = 0; j < 4; ++j) rest[j] = bad ? __float2half2_rn(0.f) : __floats2half2_rn(v[2 * j] * up, v[2 * j + 1] * up);
 #pragma unroll
         for (int c = 0; c < P; ++c) {
-          const uint2 w = kv8_pack8(v, 1.f);
-          if (c + 1 < P) {
-            const uint32_t x[2] = {w.x, w.y};
+          uint16_t e[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float2 f = e4m3x2_to_float2((uint16_t)(x[j / 2] >> (16 * (j & 1))));
-              v[2 * j] -= f.x;
-              v[2 * j + 1] -= f.y;
-            }
+          for (int j = 0; j < 4; ++j) {
+            e[j] = f16x2_to_e4m3x2(rest[j]);
+            if (c + 1 < P) rest[j] = __hsub2(rest[j], as_half2(e4m3x2_to_f16x2(e[j])));
           }
+          const uint2 w = make_uint2(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16);
 #pragma unroll
           for (int q2 = 0; q2 < kPack; ++q2) {
             const int rr = q2 * kRows + row, byte = kPack == 2 ? q2 * 64 + d : d & 127;
-            uint8_t* at = dst + ((c * kBlk + (kBlk == 2 ? d >> 7 : 0)) * kNS + rr) * 128 + (((byte >> 4) ^ (rr & 7)) << 4) + (byte & 15);
-            *reinterpret_cast<uint2*>(at) = w;
+            *reinterpret_cast<uint2*>(sQ + ((c * kBlk + (kBlk == 2 ? d >> 7 : 0)) * kNS + rr) * 128 + (((byte >> 4) ^ (rr & 7)) << 4) +
+                                      (byte & 15)) = w;
           }
         }
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&q_full[item & 1]);
-        mbar_arrive(&f_full[item % kFactors]);
-      }
-    }
-  } else {
-    // ------------------------------------------------------------------ softmax + epilogue (warps 2..5)
-    if (p.early_meta) griddep_wait();
-    const int quarter = warp & 3, tid = (warp - 2) * 32 + lane;
-    const int row_id = quarter * 32 + lane;          // TMEM lane: row of the tile, output dim
-    const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
-    const uint32_t tS = tmem_base + lane_off, tO = tmem_base + 2 * kNS + lane_off;
-    const uint32_t inv_g = 65536u / g + 1;           // r / g = r * inv_g >> 16 for r < 16
-    const int page_rows = p.block_size / kPack, box_rows = min(kM, page_rows & -page_rows);
-    const uint32_t all_boxes = kM / box_rows == 32 ? 0xffffffffu : (1u << (kM / box_rows)) - 1;
-    const int my_box = row_id / box_rows;
-    const int p_off = row_id & 15, p_ch = row_id >> 4;
+      if (lane == 0) mbar_arrive(q_ready);
+    };
+
     int t = 0;                                       // tiles so far
     int slot = 0;
     uint32_t phase = 0;
     bool ok = true, fail = false;
-    for (int item = 0; it.more(); it.next(), ++item) {
-      const Request r = request_of<D>(p, it.req);
+    Request r = {};
+    if (it.more()) {
+      r = request_of<D>(p, it.req);
+      q_load(it, r);
+      q_store(0);
+    }
+    named_bar_sync(1, kSoft);                        // factors
+#pragma unroll 1
+    for (int item = 0; it.more(); ++item) {
       const int rows = r.q_len * g, pos_max = r.ctx + r.q_len - 1;
-      float m_used[NR], l_part[NR], vref = 0.f;
+      float m_used[kRowsOf], l_part[kRowsOf], vref = 0.f;
 #pragma unroll
-      for (int i = 0; i < NR; ++i) { m_used[i] = -INFINITY; l_part[i] = 0.f; }
-      if (ok && !wait_or_abort(&f_full[item % kFactors], (item / kFactors) & 1, ab, 909)) fail = true;
-      const float* factor = sFactor + (item % kFactors) * kRows;
-      for (int i = it.tile; ok && i < it.tile + it.count; ++i, ++t) {
+      for (int i = 0; i < kRowsOf; ++i) { m_used[i] = -INFINITY; l_part[i] = 0.f; }
+      const float* factor = sFactor + (item & 1) * kRows + row_of;
+      const int tile_end = it.tile + it.count;
+#pragma unroll 1
+      for (int i = it.tile; ok && i < tile_end; ++i, ++t) {
         const int buf = t & 1;
         const int kslot = slot, vslot = slot + 1 == ns ? 0 : slot + 1;
         const uint32_t vphase = slot + 1 == ns ? phase ^ 1 : phase;
@@ -522,16 +529,14 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
         slot += 2;
         if (slot >= ns) { slot -= ns; phase ^= 1; }
         tc_fence_after_sync();
-        uint32_t sr[kNS];
-        tmem_ld_cols(tS + buf * kNS, sr);
-        float kscale[kPack], vscale[kPack];
-        if constexpr (kPack == 2) {
-          const float2 a = reinterpret_cast<const float2*>(sScale + kslot * kKeys)[row_id];
-          const float2 b = reinterpret_cast<const float2*>(sScale + vslot * kKeys)[row_id];
-          kscale[0] = a.x; kscale[kPack - 1] = a.y; vscale[0] = b.x; vscale[kPack - 1] = b.y;
-        } else {
-          kscale[0] = sScale[kslot * kKeys + row_id];
-          vscale[0] = sScale[vslot * kKeys + row_id];
+        uint32_t sr[kKeysOf][kRowsOf <= 8 ? 8 : 16];
+#pragma unroll
+        for (int q2 = 0; q2 < kKeysOf; ++q2) tmem_ld_cols(tS + buf * kNS + q2 * kRows, sr[q2]);
+        float kscale[kKeysOf], vscale[kKeysOf];
+#pragma unroll
+        for (int q2 = 0; q2 < kKeysOf; ++q2) {
+          kscale[q2] = sScale[kslot * kKeys + row_id * kPack + key_of + q2];
+          vscale[q2] = sScale[vslot * kKeys + row_id * kPack + key_of + q2];
         }
         const uint32_t valid = sValid[kslot];
         tmem_ld_wait();
@@ -545,11 +550,11 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
         const int key0 = r.kv_begin + i * kKeys;
         const bool whole = key0 + kKeys <= r.seq_len && (valid & all_boxes) == all_boxes;
         const bool full = whole && key0 + kKeys - 1 <= r.ctx && (p.window <= 0 || key0 > pos_max - p.window);
-        float sc[kPack][NR];
+        float sc[kKeysOf][kRowsOf];
         bool need = fail;
 #pragma unroll
-        for (int q2 = 0; q2 < kPack; ++q2) {
-          const int key = key0 + row_id * kPack + q2;
+        for (int q2 = 0; q2 < kKeysOf; ++q2) {
+          const int key = key0 + row_id * kPack + key_of + q2;
           const bool there = whole || (key < r.seq_len && (valid >> my_box & 1));
           if (!there) {
             vscale[q2] = 0.f;
@@ -559,50 +564,57 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
             for (int c = 0; c < 8 / kPack; ++c) {
 #pragma unroll
               for (int b = 0; b < kBlk; ++b)
-                *reinterpret_cast<uint4*>(v + b * (kM * 128) + (((kPack == 2 ? q2 * 4 + c : c) ^ (row_id & 7)) << 4)) = make_uint4(0, 0, 0, 0);
+                *reinterpret_cast<uint4*>(v + b * (kM * 128) + (((kPack == 2 ? (key_of + q2) * 4 + c : c) ^ (row_id & 7)) << 4)) =
+                    make_uint4(0, 0, 0, 0);
             }
           }
           need |= vscale[q2] > vref;
 #pragma unroll
-          for (int n = 0; n < NR; ++n) {
-            float v = __uint_as_float(sr[q2 * kRows + n]) * (kscale[q2] * factor[n]);
+          for (int n = 0; n < kRowsOf; ++n) {
+            const int row = row_of + n;
+            float v = __uint_as_float(sr[q2][n]) * (kscale[q2] * factor[n]);
             if (!full) {
-              const int pos = n < rows ? r.ctx + (int)((n * inv_g) >> 16) : -1;
+              const int pos = row < rows ? r.ctx + (int)((row * inv_g) >> 16) : -1;
               v = there && key <= pos && (p.window <= 0 || key > pos - p.window) ? v : -INFINITY;
-            } else if (NR > 4 && n >= rows) {
+            } else if (NR > 4 && row >= rows) {
               v = -INFINITY;
             }
             sc[q2][n] = v;
             need |= v > m_used[n] + kSlack;
           }
         }
-        if (bar_red_or(1, 128, need)) {
+        if (bar_red_or(1, kSoft, need)) {
           // ---- rare after the first tiles: move the reference maxima and the reference scale, rescale O^T
 #pragma unroll
-          for (int n = 0; n < NR; ++n) {
-            const float wm = warp_max_redux(kPack == 2 ? fmaxf(sc[0][n], sc[kPack - 1][n]) : sc[0][n]);
-            if (lane == n) sMax[quarter * 17 + n] = wm;
+          for (int n = 0; n < kRowsOf; ++n) {
+            const float wm = warp_max_redux(kKeysOf == 2 ? fmaxf(sc[0][n], sc[kKeysOf - 1][n]) : sc[0][n]);
+            if (lane == n) sMax[wi * 17 + n] = wm;
           }
           {
             float vm = 0.f;
 #pragma unroll
-            for (int q2 = 0; q2 < kPack; ++q2) vm = fmaxf(vm, is_nan_bits(vscale[q2]) ? 0.f : vscale[q2]);
+            for (int q2 = 0; q2 < kKeysOf; ++q2) vm = fmaxf(vm, is_nan_bits(vscale[q2]) ? 0.f : vscale[q2]);
             vm = warp_max_redux(vm);
-            if (lane == 16) sMax[quarter * 17 + 16] = vm;
+            if (lane == 16) sMax[wi * 17 + 16] = vm;
           }
           const bool warp_failed = __any_sync(0xffffffffu, fail);
-          if (lane == 0) ok_slot[quarter] = warp_failed ? 0 : 1;
-          named_bar_sync(1, 128);
-          if ((ok_slot[0] & ok_slot[1] & ok_slot[2] & ok_slot[3]) == 0) { ok = false; break; }
-          auto over = [&](int n) { return fmaxf(fmaxf(sMax[n], sMax[17 + n]), fmaxf(sMax[34 + n], sMax[51 + n])); };
-          const float vm = over(16);
+          if (lane == 0) ok_slot[wi] = warp_failed ? 0 : 1;
+          named_bar_sync(1, kSoft);
+          bool all_ok = true;
+          float vm = 0.f;
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) { all_ok &= ok_slot[w] != 0; vm = fmaxf(vm, sMax[w * 17 + 16]); }
+          if (!all_ok) { ok = false; break; }
           const float back = vm > vref ? (vref > 0.f ? vref * pow2_inv(vm) : 0.f) : 1.f;
           vref = fmaxf(vref, vm);
-          float alpha[NR];
+          float alpha[kRowsOf];
           bool rescale = back != 1.f;
 #pragma unroll
-          for (int n = 0; n < NR; ++n) {
-            const float top = over(n);
+          for (int n = 0; n < kRowsOf; ++n) {
+            // keys of a row may be with both groups; rows are with one
+            const float* mx = sMax + (kPack == 1 ? group * 4 * 17 : 0) + n;
+            float top = fmaxf(fmaxf(mx[0], mx[17]), fmaxf(mx[34], mx[51]));
+            if (kPack == 2 && L::kGroups == 2) top = fmaxf(top, fmaxf(fmaxf(mx[68], mx[85]), fmaxf(mx[102], mx[119])));
             alpha[n] = 1.f;
             if (top > m_used[n] + kSlack) {            // also the first finite maximum (m_used = -inf)
               alpha[n] = exp2f(m_used[n] - top);       // exp2(-inf) = 0: nothing accumulated yet
@@ -612,30 +624,43 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
             }
             alpha[n] *= back;
           }
-          if (rescale && i > it.tile) {    // the same decision in every thread: all of them read the same maxima
+          // every group has its own columns; the waits of its threads agree because they read the same maxima
+          if (rescale && i > it.tile) {
             if (!wait_or_abort(o_done, (t - 1) & 1, ab, 908)) fail = true;
+            __syncwarp();
             tc_fence_after_sync();
+            constexpr int kParts = kBlk * P * kKeysOf;
 #pragma unroll
-            for (int c = 0; c < kBlk * kNO; c += 16) {
-              uint32_t o[16];
-              tmem_ld_x16(tO + c, o);
-              tmem_ld_wait();
+            for (int c = 0; c < kParts; ++c) {
+              const uint32_t at = tO + c / (P * kKeysOf) * kNO + (c / kKeysOf % P * kPack + c % kKeysOf) * kRows;
+              if constexpr (kRowsOf <= 8) {
+                uint32_t o[8];
+                tmem_ld_x8(at, o);
+                tmem_ld_wait();
 #pragma unroll
-              for (int n = 0; n < NR; ++n) o[n] = __float_as_uint(__uint_as_float(o[n]) * alpha[n]);
-              tmem_st_x16(tO + c, o);
+                for (int n = 0; n < kRowsOf; ++n) o[n] = __float_as_uint(__uint_as_float(o[n]) * alpha[n]);
+                tmem_st_x8(at, o);
+              } else {
+                uint32_t o[16];
+                tmem_ld_x16(at, o);
+                tmem_ld_wait();
+#pragma unroll
+                for (int n = 0; n < kRowsOf; ++n) o[n] = __float_as_uint(__uint_as_float(o[n]) * alpha[n]);
+                tmem_st_x16(at, o);
+              }
             }
             tmem_st_wait();
           }
-          named_bar_sync(1, 128);          // sMax has been read
+          named_bar_sync(1, kSoft);          // sMax has been read
         }
         const float to_ref = vref > 0.f ? pow2_inv(vref) : 0.f;
         if (!fail) {
           uint8_t* wbuf = sP + buf * L::kP + p_off;
 #pragma unroll
-          for (int q2 = 0; q2 < kPack; ++q2) {
+          for (int q2 = 0; q2 < kKeysOf; ++q2) {
             const float vs = vscale[q2] * to_ref;
 #pragma unroll
-            for (int n = 0; n < NR; n += 2) {
+            for (int n = 0; n < kRowsOf; n += 2) {
               float w[2];
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
@@ -648,7 +673,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
 #pragma unroll
               for (int c = 0; c < P; ++c) {
                 const uint16_t code = f16x2_to_e4m3x2(rest);
-                const int rr = (c * kPack + q2) * kRows + n;
+                const int rr = (c * kPack + key_of + q2) * kRows + row_of + n;
                 wbuf[rr * 128 + ((p_ch ^ (rr & 7)) << 4)] = (uint8_t)code;
                 wbuf[(rr + 1) * 128 + ((p_ch ^ ((rr + 1) & 7)) << 4)] = (uint8_t)(code >> 8);
                 if (c + 1 < P) rest = __hmul2(__hsub2(rest, as_half2(e4m3x2_to_f16x2(code))), __float2half2_rn(32.f));
@@ -663,173 +688,183 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
         if (lane == 0 && !warp_failed) mbar_arrive(&p_ready[buf]);
       }
       if (fail) ok = false;
-      // ---- epilogue: O^T lane = output dim, columns = query rows of every piece
-      if (ok && !wait_or_abort(o_final, item & 1, ab, 907)) ok = false;
-      tc_fence_after_sync();
-      ok = bar_red_or(1, 128, !ok) == 0;   // one thread's time-out ends the work of all
-      const long long first = (long long)sPre[it.req] * p.Hkv + (long long)it.head * it.n, last = first + it.n - 1;
-      const int c0 = (int)(first / share), c1 = (int)(last / share);     // the CTAs that have tiles of this item
-      const bool partial = c0 != c1;
-      const int64_t my_slot = 2 * (int64_t)blockIdx.x + ((long long)blockIdx.x * share >= first ? 0 : 1);
+      // ---- the next item's queries, so that its first product runs while this one ends: every S of this item has been read
+      const Walk cur = it;
+      const Request rc = r;
+      it.next();
+      if (it.more()) {
+        r = request_of<D>(p, it.req);
+        q_load(it, r);
+      }
+      // ---- row sums
 #pragma unroll
-      for (int n = 0; n < NR; ++n) {
+      for (int n = 0; n < kRowsOf; ++n) {
         float v = l_part[n];
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        if (lane == n) sSum[quarter * kRows + n] = v;
+        if (lane == n) {
+          sSum[wi * kRows + n] = v;
+          sMax[wi * 17 + n] = m_used[n];
+        }
       }
-      named_bar_sync(1, 128);
+      if (it.more()) q_store(item + 1);
+      const int first = sPre[cur.req] * p.Hkv + cur.head * cur.n;
+      const int c0 = first / share, c1 = (first + cur.n - 1) / share;      // the CTAs that have tiles of this item
+      const bool partial = c0 != c1;
+      const int64_t my_slot = 2 * (int64_t)blockIdx.x + ((long long)blockIdx.x * share >= first ? 0 : 1);
+      if (ok && !wait_or_abort(o_final, item & 1, ab, 907)) ok = false;
+      ok = bar_red_or(1, kSoft, !ok) == 0;   // one thread's time-out ends the work of all
+      tc_fence_after_sync();
       if (tid < NR) {
-        float m = -INFINITY;
-#pragma unroll
-        for (int n = 0; n < NR; ++n) m = tid == n ? m_used[n] : m;
-        const float sum = sSum[tid] + sSum[kRows + tid] + sSum[2 * kRows + tid] + sSum[3 * kRows + tid];
-        const float ms = m == -INFINITY ? 0.f : m;
+        const int w0 = kPack == 1 ? tid / kRowsOf * 4 : 0, n = tid % kRowsOf;
+        float sum = 0.f;
+#pragma unroll 1
+        for (int w = w0; w < w0 + (kPack == 1 ? 4 : kWarps); ++w) sum += sSum[w * kRows + n];
+        const float m = sMax[w0 * 17 + n], ms = m == -INFINITY ? 0.f : m;
         float den = sum;
         if (!partial && p.sinks != nullptr && tid < rows)
-          den += exp2f(p.sinks[it.head * g + ((int)tid - (int)((tid * inv_g) >> 16) * g)] * kLog2e - ms + kLift);
+          den += exp2f(p.sinks[cur.head * g + ((int)tid - (int)((tid * inv_g) >> 16) * g)] * kLog2e - ms + kLift);
         // vref comes with the weights' scale; a row that saw nothing gives zeros, a NaN stays one
         sInv[tid] = !ok || den == 0.f ? 0.f : vref / den;
         if (partial) p.ws_lse[my_slot * kRows + tid] = !ok || sum == 0.f ? -INFINITY : ms + log2f(sum) - kLift;
       }
-      named_bar_sync(1, 128);
-      // this thread's output dims of every row: pieces summed, both quadrants for heads of 64
-      float o_mine[kBlk][NR];
-      if (ok) {
+      named_bar_sync(1, kSoft);
+      // this thread's output dims of its rows: pieces summed; heads of 64: even keys' in lanes 0 .. 63, odd ones' behind
+      constexpr bool kBoth = kPack == 2 && L::kGroups == 1;
+      const bool reads = kPack == 1 || L::kGroups == 1 || (row_id >> 6) == group;
+      float o_mine[kBlk][kRowsOf];
 #pragma unroll
-        for (int b = 0; b < kBlk; ++b) {
-          float part[NR];
+      for (int b = 0; b < kBlk; ++b) {
 #pragma unroll
-          for (int c = 0; c < P; ++c) {
-            uint32_t o[16];
-            tmem_ld_x16(tO + b * kNO + (c * kPack + (kPack == 2 ? row_id >> 6 : 0)) * kRows, o);
-            tmem_ld_wait();
-            const float unit = c == 0 ? 1.f : c == 1 ? 1.f / 32.f : 1.f / 1024.f;
+        for (int n = 0; n < kRowsOf; ++n) o_mine[b][n] = 0.f;
+        if (!ok) continue;
 #pragma unroll
-            for (int n = 0; n < NR; ++n) part[n] = c == 0 ? __uint_as_float(o[n]) : part[n] + __uint_as_float(o[n]) * unit;
-          }
+        for (int c = 0; c < P; ++c) {
+          const uint32_t at = tO + b * kNO + (c * kPack + (kBoth ? row_id >> 6 : 0)) * kRows;
+          uint32_t o[kRowsOf <= 8 ? 8 : 16];
+          if constexpr (kRowsOf <= 8) tmem_ld_x8(at, o); else tmem_ld_x16(at, o);
+          tmem_ld_wait();
+          const float unit = c == 0 ? 1.f : c == 1 ? 1.f / 32.f : 1.f / 1024.f;
 #pragma unroll
-          for (int n = 0; n < NR; ++n) o_mine[b][n] = part[n];
+          for (int n = 0; n < kRowsOf; ++n) o_mine[b][n] += __uint_as_float(o[n]) * unit;
         }
-      } else {
+      }
+      if constexpr (kPack == 2) {
+        if (row_id >= 64 && reads) {
+#pragma unroll
+          for (int n = 0; n < kRowsOf; ++n) sHalf[n * 64 + row_id - 64] = o_mine[0][n];
+        }
+        named_bar_sync(1, kSoft);
+        if (row_id < 64 && reads) {
+#pragma unroll
+          for (int n = 0; n < kRowsOf; ++n) o_mine[0][n] += sHalf[n * 64 + row_id];
+        }
+      }
+      auto out_row = [&](int row) {
+        const int tok = (int)((row * inv_g) >> 16);
+        return ((int64_t)(rc.qs + tok) * p.Hq + cur.head * g + (row - tok * g)) * D + row_id;
+      };
+      const bool writes = (kPack == 1 || row_id < 64) && reads;
+      if (writes) {
+#pragma unroll
+        for (int n = 0; n < kRowsOf; ++n) {
+          const int row = row_of + n;
+          const float inv = sInv[row];
+          if (row < rows) {
+#pragma unroll
+            for (int b = 0; b < kBlk; ++b) {
+              const float v = inv == 0.f ? 0.f : o_mine[b][n] * inv;
+              if (partial) p.ws_o[(my_slot * kRows + row) * D + b * 128 + row_id] = v;
+              else reinterpret_cast<T*>(p.out)[out_row(row) + b * 128] = from_f<T>(v);
+            }
+          }
+        }
+      }
+      named_bar_sync(1, kSoft);
+      if (!partial) continue;
+      // ---- the last CTA of the item to arrive merges.  The barrier has ordered everyone's stores in front of this thread's release.
+      int* ticket = p.tickets + (int64_t)cur.req * p.Hkv + cur.head;
+      if (tid == 0) {
+        int seen;
+        asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(seen) : "l"(ticket) : "memory");
+        *s_last = seen == c1 - c0;
+      }
+      named_bar_sync(1, kSoft);
+      if (*s_last) {
+        const int n_parts = c1 - c0 + 1;
+        float acc[kBlk][kRowsOf];
 #pragma unroll
         for (int b = 0; b < kBlk; ++b)
 #pragma unroll
-          for (int n = 0; n < NR; ++n) o_mine[b][n] = 0.f;
-      }
-      if constexpr (kPack == 2) {
-        if (row_id >= 64) {
-#pragma unroll
-          for (int n = 0; n < NR; ++n) sHalf[n * 64 + row_id - 64] = o_mine[0][n];
-        }
-        named_bar_sync(1, 128);
-        if (row_id < 64) {
-#pragma unroll
-          for (int n = 0; n < NR; ++n) o_mine[0][n] += sHalf[n * 64 + row_id];
-        }
-      }
-      auto out_row = [&](int n) {
-        const int tok = (int)((n * inv_g) >> 16);
-        return ((int64_t)(r.qs + tok) * p.Hq + it.head * g + (n - tok * g)) * D;
-      };
-      if (kPack == 1 || row_id < 64) {
-#pragma unroll
-        for (int n = 0; n < NR; ++n) {
-          const float inv = sInv[n];
-#pragma unroll
-          for (int b = 0; b < kBlk; ++b) {
-            const float v = inv == 0.f ? 0.f : o_mine[b][n] * inv;
-            if (n < rows) {
-              if (partial) p.ws_o[(my_slot * kRows + n) * D + b * 128 + row_id] = v;
-              else reinterpret_cast<T*>(p.out)[out_row(n) + b * 128 + row_id] = from_f<T>(v);
-            }
-          }
-        }
-      }
-      if (partial) {
-        // ---- the last CTA of the item to arrive merges
-        __threadfence();
-        named_bar_sync(1, 128);
-        int* ticket = p.tickets + (int64_t)it.req * p.Hkv + it.head;
-        if (tid == 0) *s_last = atomicAdd(ticket, 1) == c1 - c0;
-        named_bar_sync(1, 128);
-        if (*s_last) {
-          __threadfence();
-          auto slot_of = [&](int c) { return 2 * (int64_t)c + ((long long)c * share >= first ? 0 : 1); };
-          const int n_parts = c1 - c0 + 1;
-          // row tid % 16: largest log-sum-exp and the sum, eight threads a row
-          {
-            const int n = tid & 15;
-            float M = -INFINITY, S = 0.f;
-            for (int c = tid >> 4; c < n_parts; c += 8) {
-              const float v = n < rows ? __ldcg(p.ws_lse + slot_of(c0 + c) * kRows + n) : -INFINITY;
-              if (v != -INFINITY) {
-                const float top = fmaxf(M, v);
-                S = S * exp2f(M - top) + exp2f(v - top);
-                M = top;
-              }
-            }
-            sW[tid] = M;
-            sW[128 + tid] = S;
-          }
-          named_bar_sync(1, 128);
+          for (int n = 0; n < kRowsOf; ++n) acc[b][n] = 0.f;
+        float M = -INFINITY, S = 0.f;            // of row tid, for tid < 16; acc is relative to M
+#pragma unroll 1
+        for (int base = 0; base < n_parts; base += 32) {
+          const int cnt = min(32, n_parts - base);
+          auto slot_of = [&](int c) { return 2 * (int64_t)(c0 + base + c) + ((long long)(c0 + base + c) * share >= first ? 0 : 1); };
+          for (int x = tid; x < cnt * kRows; x += kSoft)
+            sW[x] = (x & 15) < rows ? __ldcg(p.ws_lse + slot_of(x >> 4) * kRows + (x & 15)) : -INFINITY;
+          named_bar_sync(1, kSoft);
           if (tid < kRows) {
-            float M = -INFINITY, S = 0.f;
-            for (int c = 0; c < 8; ++c) M = fmaxf(M, sW[c * 16 + tid]);
-            const float Ms = M == -INFINITY ? 0.f : M;
-            for (int c = 0; c < 8; ++c) {
-              const float s = sW[128 + c * 16 + tid], mm = sW[c * 16 + tid];
-              S += is_nan_bits(s) ? s : s * exp2f(mm - Ms);
+            float top = M;
+#pragma unroll 1
+            for (int c = 0; c < cnt; ++c) top = fmaxf(top, sW[c * kRows + tid]);
+            const float ts = top == -INFINITY ? 0.f : top;
+            const float old = M == -INFINITY ? 0.f : exp2f(M - ts);
+            S *= old;
+#pragma unroll 1
+            for (int c = 0; c < cnt; ++c) {
+              const float v = sW[c * kRows + tid], e = v == -INFINITY ? 0.f : exp2f(v - ts);      // a NaN stays one
+              S += e;
+              sW[c * kRows + tid] = e;
             }
-            if (p.sinks != nullptr && tid < rows)
-              S += exp2f(p.sinks[it.head * g + ((int)tid - (int)((tid * inv_g) >> 16) * g)] * kLog2e - Ms);
-            sMax[tid] = Ms;
-            sInv[tid] = S == 0.f ? 0.f : 1.f / S;
+            M = top;
+            sInv[tid] = old;
           }
-          named_bar_sync(1, 128);
-          float acc[kBlk][NR];
+          named_bar_sync(1, kSoft);
+          if (writes) {
+            if (base > 0) {
 #pragma unroll
-          for (int b = 0; b < kBlk; ++b)
+              for (int n = 0; n < kRowsOf; ++n)
 #pragma unroll
-            for (int n = 0; n < NR; ++n) acc[b][n] = 0.f;
-          for (int base = 0; base < n_parts; base += 32) {
-            const int cnt = min(32, n_parts - base);
-            for (int x = tid; x < cnt * kRows; x += 128) {
-              const int n = x & 15;
-              const float v = n < rows ? __ldcg(p.ws_lse + slot_of(c0 + base + (x >> 4)) * kRows + n) : -INFINITY;
-              sW[x] = v == -INFINITY ? 0.f : exp2f(v - sMax[n]) * sInv[n];
+                for (int b = 0; b < kBlk; ++b) acc[b][n] *= sInv[row_of + n];
             }
-            named_bar_sync(1, 128);
-            if (kPack == 1 || row_id < 64) {
-              for (int c = 0; c < cnt; ++c) {
-                const float* src = p.ws_o + slot_of(c0 + base + c) * kRows * D + row_id;
+#pragma unroll 1
+            for (int c = 0; c < cnt; ++c) {
+              const float* src = p.ws_o + (slot_of(c) * kRows + row_of) * D + row_id;
 #pragma unroll
-                for (int n = 0; n < NR; ++n) {
-                  if (n < rows) {
-                    const float w = sW[c * kRows + n];
+              for (int n = 0; n < kRowsOf; ++n) {
+                if (row_of + n < rows) {
+                  const float w = sW[c * kRows + row_of + n];
 #pragma unroll
-                    for (int b = 0; b < kBlk; ++b) {
-                      const float v = __ldcg(src + n * D + b * 128);
-                      acc[b][n] += w == 0.f ? 0.f : v * w;
-                    }
+                  for (int b = 0; b < kBlk; ++b) {
+                    const float v = __ldcg(src + n * D + b * 128);
+                    acc[b][n] += w == 0.f ? 0.f : v * w;
                   }
                 }
               }
             }
-            named_bar_sync(1, 128);
           }
-          if (kPack == 1 || row_id < 64) {
-#pragma unroll
-            for (int n = 0; n < NR; ++n)
-              if (n < rows) {
-#pragma unroll
-                for (int b = 0; b < kBlk; ++b) reinterpret_cast<T*>(p.out)[out_row(n) + b * 128 + row_id] = from_f<T>(acc[b][n]);
-              }
-          }
-          if (tid == 0) *ticket = 0;
+          named_bar_sync(1, kSoft);
         }
+        if (tid < kRows) {
+          if (p.sinks != nullptr && tid < rows)
+            S += exp2f(p.sinks[cur.head * g + ((int)tid - (int)((tid * inv_g) >> 16) * g)] * kLog2e - (M == -INFINITY ? 0.f : M));
+          sInv[tid] = S == 0.f ? 0.f : 1.f / S;
+        }
+        named_bar_sync(1, kSoft);
+        if (writes) {
+#pragma unroll
+          for (int n = 0; n < kRowsOf; ++n)
+            if (row_of + n < rows) {
+#pragma unroll
+              for (int b = 0; b < kBlk; ++b)
+                reinterpret_cast<T*>(p.out)[out_row(row_of + n) + b * 128] = from_f<T>(acc[b][n] * sInv[row_of + n]);
+            }
+        }
+        if (tid == 0) *ticket = 0;
+        named_bar_sync(1, kSoft);              // the exchange buffers are free for the next item
       }
-      named_bar_sync(1, 128);              // the exchange buffers are free for the next item
     }
   }
 
@@ -842,39 +877,43 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
 }
 
 template <typename T, int D, int NR>
-static int launch_nr(Params p, const CUtensorMap& tm, int grid, int slots, cudaStream_t st) {
+static int launch_nr(Params p, const CUtensorMap& tm, int64_t units, int num_sms, cudaStream_t st) {
+  using L = Layout<T, D, NR>;
   auto kern = kv8_decode_kernel<T, D, NR>;
+  // two CTAs an SM where four operand slots each fit, otherwise one with as many as fit
+  int ctas = L::kCtas, slots = 6;
+  while (slots > 4 && L::smem(slots, p.B) > 113 * 1024) --slots;
+  if (ctas == 1 || L::smem(slots, p.B) > 113 * 1024) {
+    ctas = 1;
+    slots = 10;
+    while (slots > 4 && L::smem(slots, p.B) > 226 * 1024) --slots;
+  }
+  const int grid = (int)(units < (int64_t)num_sms * ctas ? units : (int64_t)num_sms * ctas);
   p.slots = slots;
-  const size_t smem = Layout<T, D>::smem(slots, p.B);
+  const size_t smem = L::smem(slots, p.B);
   cudaError_t e = ensure_dynamic_smem((const void*)kern, (int)smem);
   if (e != cudaSuccess) return (int)e;
-  return (int)launch_pdl(kern, dim3(grid), dim3(kThreads), smem, st, tm, p);
+  return (int)launch_pdl(kern, dim3(grid), dim3(L::kThreads), smem, st, tm, p);
 }
 
 template <typename T, int D>
 static int launch(const Params& p0, const CUtensorMap& tm, int B, int max_rows, int num_sms, int64_t max_tiles, cudaStream_t st) {
   Params p = p0;
-  for (int b0 = 0; b0 < B; b0 += kMaxB) {
-    p.B = B - b0 < kMaxB ? B - b0 : kMaxB;
+  // tiles are counted in 32 bits
+  const int64_t most = 0x7fffffff / ((int64_t)p.Hkv * (p.max_keys / Geo<D>::kKeys + 2));
+  if (most < 1) return 3;
+  const int step = most < kMaxB ? (int)most : kMaxB;
+  for (int b0 = 0; b0 < B; b0 += step) {
+    p.B = B - b0 < step ? B - b0 : step;
     p.block_tables = p0.block_tables + (int64_t)b0 * p.bt_stride;
     p.seq_lens = p0.seq_lens + b0;
     p.qsl = p0.qsl + b0;
     p.tickets = p0.tickets + (int64_t)b0 * p.Hkv;
-    // two CTAs an SM where four operand slots each fit, otherwise one with as many as fit
-    int ctas = 2, slots = 6;
-    while (slots > 4 && Layout<T, D>::smem(slots, p.B) > 113 * 1024) --slots;
-    if (Layout<T, D>::smem(slots, p.B) > 113 * 1024) {
-      ctas = 1;
-      slots = 10;
-      while (slots > 4 && Layout<T, D>::smem(slots, p.B) > 226 * 1024) --slots;
-    }
     const int64_t units = (int64_t)p.B * p.Hkv * (max_tiles < 1 ? 1 : max_tiles);
-    int grid = num_sms * ctas;
-    if (units < grid) grid = (int)units;
     int rc;
-    if (max_rows <= 4) rc = launch_nr<T, D, 4>(p, tm, grid, slots, st);
-    else if (max_rows <= 8) rc = launch_nr<T, D, 8>(p, tm, grid, slots, st);
-    else rc = launch_nr<T, D, 16>(p, tm, grid, slots, st);
+    if (max_rows <= 4) rc = launch_nr<T, D, 4>(p, tm, units, num_sms, st);
+    else if (max_rows <= 8) rc = launch_nr<T, D, 8>(p, tm, units, num_sms, st);
+    else rc = launch_nr<T, D, 16>(p, tm, units, num_sms, st);
     if (rc != 0) return rc;
   }
   return 0;
@@ -900,7 +939,8 @@ extern "C" int b200_kv8_decode(void* out, const void* q, const void* cache, cons
   p.q = q; p.out = out; p.cache = static_cast<const uint8_t*>(cache); p.ws_o = ws_o; p.ws_lse = ws_lse; p.tickets = tickets;
   p.block_tables = block_tables; p.seq_lens = seq_lens; p.qsl = qsl; p.sinks = sinks; p.status = status;
   p.num_blocks = num_blocks; p.bt_stride = bt_stride; p.q_stride = q_stride; p.Hq = Hq; p.Hkv = Hkv; p.block_size = block_size;
-  p.max_blocks = max_blocks; p.window = window; p.early_meta = early_meta; p.min_tiles = 1;
+  p.max_blocks = max_blocks; p.max_keys = (int)((int64_t)max_blocks * block_size < 0x7ffffe00 ? max_blocks * block_size : 0x7ffffe00);
+  p.window = window; p.early_meta = early_meta; p.min_tiles = 1;
   p.scale_log2 = scale * kv8dec::kLog2e;
   const CUtensorMap& tm = *reinterpret_cast<const CUtensorMap*>(tmap);
   const int rows = max_query_len * (Hq / Hkv), keys = D == 64 ? 256 : 128;
