@@ -19,9 +19,9 @@
 // Work: all tiles of all (request, head) items in one line, cut into equal pieces, one a CTA (two CTAs an SM where shared memory lasts), so
 // that uneven requests cost what their sum costs.  Where a cut falls, from the lengths on the device: captured launches adapt.  An item
 // that lies in several CTAs is merged by the last of them to arrive, in the order of the cuts: the result does not depend on who that is.
-// 192 or 320 threads: warp 0 TMA producer (a lane per box of a tile, which looks its block up a tile ahead), warp 1 MMA issuer, the others
-// softmax (thread = row of the tile; TMEM lane = output dim at the end) and queries: four warps, or, where a row of the tile brings 16 scores
-// or more, eight, which share them by query rows (heads of 64: by keys of a row).  What is done once an item is kept short in code as well as in
+// 192, 320 or 576 threads: warp 0 TMA producer (a lane per box of a tile, which looks its block up a tile ahead), warp 1 MMA issuer, the others
+// softmax (thread = row of the tile; TMEM lane = output dim at the end) and queries: four warps for 8 scores a row of the tile at most, as many
+// groups of four as there are eights otherwise, by query rows and, with heads of 64, by keys.  What is done once an item is kept short in code as well as in
 // time: half of a call's time went into it before, most of that into fetching instructions.  Every wait is bounded; on time-out the status word is
 // set and the CTA unwinds.
 #include <cuda.h>
@@ -74,11 +74,11 @@ template <> struct Pieces<__half> { static constexpr int n = 3; };
 template <typename T, int D, int NR> struct Layout {
   using G = Geo<D>;
   static constexpr int P = Pieces<T>::n;
-  static constexpr int kGroups = NR * G::kPack >= 16 ? 2 : 1;  // groups of four softmax warps
+  // groups of four softmax warps; a thread has at most 8 scores of a tile
+  static constexpr int kKeyGroups = G::kPack == 2 && NR >= 8 ? 2 : 1, kRowGroups = NR == 16 ? 2 : 1, kGroups = kKeyGroups * kRowGroups;
   static constexpr int kSoft = 128 * kGroups, kThreads = 64 + kSoft;
-  static constexpr int kCtas = D == 256 || (D == 64 && kGroups == 2) ? 1 : 2;   // an SM at most: shared memory, registers
-  static constexpr int kKeysOf = G::kPack / (G::kPack == 2 ? kGroups : 1);       // keys and query rows of a thread
-  static constexpr int kRowsOf = NR / (G::kPack == 1 ? kGroups : 1);
+  static constexpr int kCtas = D == 256 || (D == 64 && NR == 16) ? 1 : 2;        // an SM at most: shared memory, registers
+  static constexpr int kKeysOf = G::kPack / kKeyGroups, kRowsOf = NR / kRowGroups;       // keys of a row and query rows of a thread
   static constexpr int kNO = G::kNS * P;                       // columns of an O^T accumulator
   static constexpr int kQ = P * G::kBlk * G::kNS * 128;        // queries
   static constexpr int kP = kNO * 128;                         // one weight buffer
@@ -86,7 +86,7 @@ template <typename T, int D, int NR> struct Layout {
   static constexpr int kTmem = kCols <= 64 ? 64 : kCols <= 128 ? 128 : 256;
   static constexpr int kScales = G::kKeys * 4;
   // barriers, factors, flags, exchange buffers
-  static constexpr int kMisc = 4096 + (D == 64 ? kRows * 64 * 4 : 0);
+  static constexpr int kMisc = 4096 + (D == 64 ? kRows * 64 * 4 : 0);      // 2 KB of it for up to 16 softmax warps
   static size_t smem(int slots, int B) {
     return 1024 + (size_t)slots * (G::kOp + kScales) + kQ + 2 * kP + kMisc + (size_t)(B + 1) * 4;
   }
@@ -100,20 +100,10 @@ __device__ __forceinline__ float warp_max_redux(float v) {
   i = i >= 0 ? i : i ^ 0x7fffffff;
   return __int_as_float(i);
 }
-// into the registers themselves: no copy may come before the wait
-__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&r)[8]) { tmem_ld_x8(taddr, r); }
-__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld_x16(taddr, r); }
 __device__ __forceinline__ void tmem_st_x8(uint32_t taddr, const uint32_t (&r)[8]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
                "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                : "memory");
-}
-__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
 }
 __device__ __forceinline__ uint16_t f16x2_to_e4m3x2(__half2 v) {
   uint16_t r;
@@ -200,17 +190,16 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
   uint64_t* o_final = bars + 42;         // a phase per item
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 44);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  volatile int* ok_slot = abort_flag + 1;                    // [8]
-  int* s_last = const_cast<int*>(abort_flag) + 9;
-  uint32_t* sValid = tmem_slot + 12;                         // [16] boxes of a K slot that were read
+  volatile int* ok_slot = abort_flag + 1;                    // [16]
+  int* s_last = const_cast<int*>(abort_flag) + 17;
+  uint32_t* sValid = tmem_slot + 20;                         // [16] boxes of a K slot that were read
   uint32_t* sOdd = sValid + 16;                              // [16] heads of 64: 1 + the row of a K slot whose second key is behind the end
   float* sFactor = reinterpret_cast<float*>(sOdd + 16);      // [2 items][16]
-  float* sMax = sFactor + 2 * kRows;                         // [8 warps][17]
-  float* sSum = sMax + 8 * 17;                               // [8][16]
-  float* sInv = sSum + 8 * kRows;                            // [16]
-  float* sW = sInv + kRows;                                  // [32][16]
-  int* sScan = reinterpret_cast<int*>(sW);                   // [10] (before the first item)
-  float* sHalf = sW + 32 * kRows;                            // [16][64] (heads of 64)
+  float* sMax = sFactor + 2 * kRows;                         // [16 warps][9] maxima of a group's rows, largest v_scale
+  float* sSum = sMax + 16 * 9;                               // [16][8]
+  float* sInv = sSum + 16 * 8;                               // [16]
+  int* sScan = reinterpret_cast<int*>(sInv + kRows);         // [18]
+  float* sHalf = reinterpret_cast<float*>(sScan + 20);       // [16][64] (heads of 64)
   int* sPre = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(bars) + L::kMisc);   // [B + 1]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -429,8 +418,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
     const int wi = warp - 2, tid = wi * 32 + lane, group = wi >> 2, quarter = warp & 3;
     const int row_id = quarter * 32 + lane;          // TMEM lane: row of the tile, output dim
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
-    const int key_of = kPack == 2 && L::kGroups == 2 ? group : 0;        // first key (of a row of the tile) and query row of this thread
-    const int row_of = kPack == 1 && L::kGroups == 2 ? group * kRowsOf : 0;
+    const int row_group = group / L::kKeyGroups, key_of = group % L::kKeyGroups, row_of = row_group * kRowsOf;
     const uint32_t tS = tmem_base + lane_off + key_of * kRows + row_of, tO = tmem_base + 2 * kNS + lane_off + key_of * kRows + row_of;
     const uint32_t inv_g = 65536u / g + 1;           // r / g = r * inv_g >> 16 for r < 16
     const int page_rows = p.block_size / kPack, box_rows = min(kM, page_rows & -page_rows);
@@ -514,9 +502,16 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
 #pragma unroll
       for (int i = 0; i < kRowsOf; ++i) { m_used[i] = -INFINITY; l_part[i] = 0.f; }
       const float* factor = sFactor + (item & 1) * kRows + row_of;
-      const int tile_end = it.tile + it.count;
+      const Walk cur = it;
+      const Request rc = r;
+      it.next();
+      if (it.more()) {
+        r = request_of<D>(p, it.req);
+        q_load(it, r);                       // on their way while this item is worked on
+      }
+      const int tile_end = cur.tile + cur.count;
 #pragma unroll 1
-      for (int i = it.tile; ok && i < tile_end; ++i, ++t) {
+      for (int i = cur.tile; ok && i < tile_end; ++i, ++t) {
         const int buf = t & 1;
         const int kslot = slot, vslot = slot + 1 == ns ? 0 : slot + 1;
         const uint32_t vphase = slot + 1 == ns ? phase ^ 1 : phase;
@@ -529,9 +524,9 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
         slot += 2;
         if (slot >= ns) { slot -= ns; phase ^= 1; }
         tc_fence_after_sync();
-        uint32_t sr[kKeysOf][kRowsOf <= 8 ? 8 : 16];
+        uint32_t sr[kKeysOf][8];
 #pragma unroll
-        for (int q2 = 0; q2 < kKeysOf; ++q2) tmem_ld_cols(tS + buf * kNS + q2 * kRows, sr[q2]);
+        for (int q2 = 0; q2 < kKeysOf; ++q2) tmem_ld_x8(tS + buf * kNS + q2 * kRows, sr[q2]);
         float kscale[kKeysOf], vscale[kKeysOf];
 #pragma unroll
         for (int q2 = 0; q2 < kKeysOf; ++q2) {
@@ -547,15 +542,15 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
           mbar_arrive(&kv_empty[kslot]);
           mbar_arrive(&kv_empty[vslot]);
         }
-        const int key0 = r.kv_begin + i * kKeys;
-        const bool whole = key0 + kKeys <= r.seq_len && (valid & all_boxes) == all_boxes;
-        const bool full = whole && key0 + kKeys - 1 <= r.ctx && (p.window <= 0 || key0 > pos_max - p.window);
+        const int key0 = rc.kv_begin + i * kKeys;
+        const bool whole = key0 + kKeys <= rc.seq_len && (valid & all_boxes) == all_boxes;
+        const bool full = whole && key0 + kKeys - 1 <= rc.ctx && (p.window <= 0 || key0 > pos_max - p.window);
         float sc[kKeysOf][kRowsOf];
         bool need = fail;
 #pragma unroll
         for (int q2 = 0; q2 < kKeysOf; ++q2) {
           const int key = key0 + row_id * kPack + key_of + q2;
-          const bool there = whole || (key < r.seq_len && (valid >> my_box & 1));
+          const bool there = whole || (key < rc.seq_len && (valid >> my_box & 1));
           if (!there) {
             vscale[q2] = 0.f;
             // codes of rows that were not read, or not written, may be anything: zeros, since a weight of zero does not hide a NaN
@@ -574,7 +569,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
             const int row = row_of + n;
             float v = __uint_as_float(sr[q2][n]) * (kscale[q2] * factor[n]);
             if (!full) {
-              const int pos = row < rows ? r.ctx + (int)((row * inv_g) >> 16) : -1;
+              const int pos = row < rows ? rc.ctx + (int)((row * inv_g) >> 16) : -1;
               v = there && key <= pos && (p.window <= 0 || key > pos - p.window) ? v : -INFINITY;
             } else if (NR > 4 && row >= rows) {
               v = -INFINITY;
@@ -588,14 +583,14 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
 #pragma unroll
           for (int n = 0; n < kRowsOf; ++n) {
             const float wm = warp_max_redux(kKeysOf == 2 ? fmaxf(sc[0][n], sc[kKeysOf - 1][n]) : sc[0][n]);
-            if (lane == n) sMax[wi * 17 + n] = wm;
+            if (lane == n) sMax[wi * 9 + n] = wm;
           }
           {
             float vm = 0.f;
 #pragma unroll
             for (int q2 = 0; q2 < kKeysOf; ++q2) vm = fmaxf(vm, is_nan_bits(vscale[q2]) ? 0.f : vscale[q2]);
             vm = warp_max_redux(vm);
-            if (lane == 16) sMax[wi * 17 + 16] = vm;
+            if (lane == 8) sMax[wi * 9 + 8] = vm;
           }
           const bool warp_failed = __any_sync(0xffffffffu, fail);
           if (lane == 0) ok_slot[wi] = warp_failed ? 0 : 1;
@@ -603,7 +598,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
           bool all_ok = true;
           float vm = 0.f;
 #pragma unroll
-          for (int w = 0; w < kWarps; ++w) { all_ok &= ok_slot[w] != 0; vm = fmaxf(vm, sMax[w * 17 + 16]); }
+          for (int w = 0; w < kWarps; ++w) { all_ok &= ok_slot[w] != 0; vm = fmaxf(vm, sMax[w * 9 + 8]); }
           if (!all_ok) { ok = false; break; }
           const float back = vm > vref ? (vref > 0.f ? vref * pow2_inv(vm) : 0.f) : 1.f;
           vref = fmaxf(vref, vm);
@@ -611,10 +606,10 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
           bool rescale = back != 1.f;
 #pragma unroll
           for (int n = 0; n < kRowsOf; ++n) {
-            // keys of a row may be with both groups; rows are with one
-            const float* mx = sMax + (kPack == 1 ? group * 4 * 17 : 0) + n;
-            float top = fmaxf(fmaxf(mx[0], mx[17]), fmaxf(mx[34], mx[51]));
-            if (kPack == 2 && L::kGroups == 2) top = fmaxf(top, fmaxf(fmaxf(mx[68], mx[85]), fmaxf(mx[102], mx[119])));
+            // a group's rows, and the same rows' other keys next to it
+            const float* mx = sMax + row_group * L::kKeyGroups * 4 * 9 + n;
+            float top = fmaxf(fmaxf(mx[0], mx[9]), fmaxf(mx[18], mx[27]));
+            if (L::kKeyGroups == 2) top = fmaxf(top, fmaxf(fmaxf(mx[36], mx[45]), fmaxf(mx[54], mx[63])));
             alpha[n] = 1.f;
             if (top > m_used[n] + kSlack) {            // also the first finite maximum (m_used = -inf)
               alpha[n] = exp2f(m_used[n] - top);       // exp2(-inf) = 0: nothing accumulated yet
@@ -625,7 +620,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
             alpha[n] *= back;
           }
           // every group has its own columns; the waits of its threads agree because they read the same maxima
-          if (rescale && i > it.tile) {
+          if (rescale && i > cur.tile) {
             if (!wait_or_abort(o_done, (t - 1) & 1, ab, 908)) fail = true;
             __syncwarp();
             tc_fence_after_sync();
@@ -633,21 +628,12 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
 #pragma unroll
             for (int c = 0; c < kParts; ++c) {
               const uint32_t at = tO + c / (P * kKeysOf) * kNO + (c / kKeysOf % P * kPack + c % kKeysOf) * kRows;
-              if constexpr (kRowsOf <= 8) {
-                uint32_t o[8];
-                tmem_ld_x8(at, o);
-                tmem_ld_wait();
+              uint32_t o[8];
+              tmem_ld_x8(at, o);
+              tmem_ld_wait();
 #pragma unroll
-                for (int n = 0; n < kRowsOf; ++n) o[n] = __float_as_uint(__uint_as_float(o[n]) * alpha[n]);
-                tmem_st_x8(at, o);
-              } else {
-                uint32_t o[16];
-                tmem_ld_x16(at, o);
-                tmem_ld_wait();
-#pragma unroll
-                for (int n = 0; n < kRowsOf; ++n) o[n] = __float_as_uint(__uint_as_float(o[n]) * alpha[n]);
-                tmem_st_x16(at, o);
-              }
+              for (int n = 0; n < kRowsOf; ++n) o[n] = __float_as_uint(__uint_as_float(o[n]) * alpha[n]);
+              tmem_st_x8(at, o);
             }
             tmem_st_wait();
           }
@@ -689,13 +675,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
       }
       if (fail) ok = false;
       // ---- the next item's queries, so that its first product runs while this one ends: every S of this item has been read
-      const Walk cur = it;
-      const Request rc = r;
-      it.next();
-      if (it.more()) {
-        r = request_of<D>(p, it.req);
-        q_load(it, r);
-      }
+      if (it.more()) q_store(item + 1);
       // ---- row sums
 #pragma unroll
       for (int n = 0; n < kRowsOf; ++n) {
@@ -703,11 +683,10 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
         if (lane == n) {
-          sSum[wi * kRows + n] = v;
-          sMax[wi * 17 + n] = m_used[n];
+          sSum[wi * 8 + n] = v;
+          sMax[wi * 9 + n] = m_used[n];
         }
       }
-      if (it.more()) q_store(item + 1);
       const int first = sPre[cur.req] * p.Hkv + cur.head * cur.n;
       const int c0 = first / share, c1 = (first + cur.n - 1) / share;      // the CTAs that have tiles of this item
       const bool partial = c0 != c1;
@@ -716,11 +695,11 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
       ok = bar_red_or(1, kSoft, !ok) == 0;   // one thread's time-out ends the work of all
       tc_fence_after_sync();
       if (tid < NR) {
-        const int w0 = kPack == 1 ? tid / kRowsOf * 4 : 0, n = tid % kRowsOf;
+        const int w0 = tid / kRowsOf * L::kKeyGroups * 4, n = tid % kRowsOf;
         float sum = 0.f;
-#pragma unroll 1
-        for (int w = w0; w < w0 + (kPack == 1 ? 4 : kWarps); ++w) sum += sSum[w * kRows + n];
-        const float m = sMax[w0 * 17 + n], ms = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int w = 0; w < 4 * L::kKeyGroups; ++w) sum += sSum[(w0 + w) * 8 + n];
+        const float m = sMax[w0 * 9 + n], ms = m == -INFINITY ? 0.f : m;
         float den = sum;
         if (!partial && p.sinks != nullptr && tid < rows)
           den += exp2f(p.sinks[cur.head * g + ((int)tid - (int)((tid * inv_g) >> 16) * g)] * kLog2e - ms + kLift);
@@ -730,8 +709,8 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
       }
       named_bar_sync(1, kSoft);
       // this thread's output dims of its rows: pieces summed; heads of 64: even keys' in lanes 0 .. 63, odd ones' behind
-      constexpr bool kBoth = kPack == 2 && L::kGroups == 1;
-      const bool reads = kPack == 1 || L::kGroups == 1 || (row_id >> 6) == group;
+      constexpr bool kBoth = kPack == 2 && L::kKeyGroups == 1;
+      const bool reads = L::kKeyGroups == 1 || (row_id >> 6) == key_of;
       float o_mine[kBlk][kRowsOf];
 #pragma unroll
       for (int b = 0; b < kBlk; ++b) {
@@ -741,8 +720,8 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
 #pragma unroll
         for (int c = 0; c < P; ++c) {
           const uint32_t at = tO + b * kNO + (c * kPack + (kBoth ? row_id >> 6 : 0)) * kRows;
-          uint32_t o[kRowsOf <= 8 ? 8 : 16];
-          if constexpr (kRowsOf <= 8) tmem_ld_x8(at, o); else tmem_ld_x16(at, o);
+          uint32_t o[8];
+          tmem_ld_x8(at, o);
           tmem_ld_wait();
           const float unit = c == 0 ? 1.f : c == 1 ? 1.f / 32.f : 1.f / 1024.f;
 #pragma unroll
@@ -752,12 +731,12 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
       if constexpr (kPack == 2) {
         if (row_id >= 64 && reads) {
 #pragma unroll
-          for (int n = 0; n < kRowsOf; ++n) sHalf[n * 64 + row_id - 64] = o_mine[0][n];
+          for (int n = 0; n < kRowsOf; ++n) sHalf[(row_of + n) * 64 + row_id - 64] = o_mine[0][n];
         }
         named_bar_sync(1, kSoft);
         if (row_id < 64 && reads) {
 #pragma unroll
-          for (int n = 0; n < kRowsOf; ++n) o_mine[0][n] += sHalf[n * 64 + row_id];
+          for (int n = 0; n < kRowsOf; ++n) o_mine[0][n] += sHalf[(row_of + n) * 64 + row_id];
         }
       }
       auto out_row = [&](int row) {
@@ -791,79 +770,64 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
       }
       named_bar_sync(1, kSoft);
       if (*s_last) {
+        // every thread its dims: a few parts' log-sum-exps and results at a time, all in flight, joined in the order of the parts
         const int n_parts = c1 - c0 + 1;
-        float acc[kBlk][kRowsOf];
+        constexpr int kAtOnce = kRowsOf * kBlk > 8 || L::kGroups > 1 ? 2 : 4;
+        float acc[kBlk][kRowsOf], M[kRowsOf], S[kRowsOf];
 #pragma unroll
-        for (int b = 0; b < kBlk; ++b)
+        for (int n = 0; n < kRowsOf; ++n) {
+          M[n] = -INFINITY;
+          S[n] = 0.f;
 #pragma unroll
-          for (int n = 0; n < kRowsOf; ++n) acc[b][n] = 0.f;
-        float M = -INFINITY, S = 0.f;            // of row tid, for tid < 16; acc is relative to M
+          for (int b = 0; b < kBlk; ++b) acc[b][n] = 0.f;
+        }
+        if (writes) {
 #pragma unroll 1
-        for (int base = 0; base < n_parts; base += 32) {
-          const int cnt = min(32, n_parts - base);
-          auto slot_of = [&](int c) { return 2 * (int64_t)(c0 + base + c) + ((long long)(c0 + base + c) * share >= first ? 0 : 1); };
-          for (int x = tid; x < cnt * kRows; x += kSoft)
-            sW[x] = (x & 15) < rows ? __ldcg(p.ws_lse + slot_of(x >> 4) * kRows + (x & 15)) : -INFINITY;
-          named_bar_sync(1, kSoft);
-          if (tid < kRows) {
-            float top = M;
-#pragma unroll 1
-            for (int c = 0; c < cnt; ++c) top = fmaxf(top, sW[c * kRows + tid]);
-            const float ts = top == -INFINITY ? 0.f : top;
-            const float old = M == -INFINITY ? 0.f : exp2f(M - ts);
-            S *= old;
-#pragma unroll 1
-            for (int c = 0; c < cnt; ++c) {
-              const float v = sW[c * kRows + tid], e = v == -INFINITY ? 0.f : exp2f(v - ts);      // a NaN stays one
-              S += e;
-              sW[c * kRows + tid] = e;
-            }
-            M = top;
-            sInv[tid] = old;
-          }
-          named_bar_sync(1, kSoft);
-          if (writes) {
-            if (base > 0) {
+          for (int base = 0; base < n_parts; base += kAtOnce) {
+            float l[kAtOnce][kRowsOf], v[kAtOnce][kBlk][kRowsOf];
 #pragma unroll
-              for (int n = 0; n < kRowsOf; ++n)
-#pragma unroll
-                for (int b = 0; b < kBlk; ++b) acc[b][n] *= sInv[row_of + n];
-            }
-#pragma unroll 1
-            for (int c = 0; c < cnt; ++c) {
-              const float* src = p.ws_o + (slot_of(c) * kRows + row_of) * D + row_id;
+            for (int u = 0; u < kAtOnce; ++u) {
+              const int c = c0 + min(base + u, n_parts - 1);
+              const int64_t at = (2 * (int64_t)c + ((long long)c * share >= first ? 0 : 1)) * kRows + row_of;
 #pragma unroll
               for (int n = 0; n < kRowsOf; ++n) {
-                if (row_of + n < rows) {
-                  const float w = sW[c * kRows + row_of + n];
+                const bool in = row_of + n < rows && base + u < n_parts;
+                l[u][n] = in ? __ldcg(p.ws_lse + at + n) : -INFINITY;
 #pragma unroll
-                  for (int b = 0; b < kBlk; ++b) {
-                    const float v = __ldcg(src + n * D + b * 128);
-                    acc[b][n] += w == 0.f ? 0.f : v * w;
-                  }
-                }
+                for (int b = 0; b < kBlk; ++b) v[u][b][n] = in ? __ldcg(p.ws_o + (at + n) * D + b * 128 + row_id) : 0.f;
+              }
+            }
+#pragma unroll
+            for (int n = 0; n < kRowsOf; ++n) {
+              float top = M[n];
+#pragma unroll
+              for (int u = 0; u < kAtOnce; ++u) top = fmaxf(top, l[u][n]);
+              const float ts = top == -INFINITY ? 0.f : top, old = exp2f(M[n] - ts);
+              M[n] = top;
+              S[n] *= old;
+#pragma unroll
+              for (int b = 0; b < kBlk; ++b) acc[b][n] *= old;
+#pragma unroll
+              for (int u = 0; u < kAtOnce; ++u) {
+                const float w = exp2f(l[u][n] - ts);       // a NaN stays one; an empty part weighs nothing, and its result is zeros
+                S[n] += w;
+#pragma unroll
+                for (int b = 0; b < kBlk; ++b) acc[b][n] += v[u][b][n] * w;
               }
             }
           }
-          named_bar_sync(1, kSoft);
-        }
-        if (tid < kRows) {
-          if (p.sinks != nullptr && tid < rows)
-            S += exp2f(p.sinks[cur.head * g + ((int)tid - (int)((tid * inv_g) >> 16) * g)] * kLog2e - (M == -INFINITY ? 0.f : M));
-          sInv[tid] = S == 0.f ? 0.f : 1.f / S;
-        }
-        named_bar_sync(1, kSoft);
-        if (writes) {
 #pragma unroll
-          for (int n = 0; n < kRowsOf; ++n)
-            if (row_of + n < rows) {
+          for (int n = 0; n < kRowsOf; ++n) {
+            const int row = row_of + n;
+            if (row >= rows) continue;
+            if (p.sinks != nullptr)
+              S[n] += exp2f(p.sinks[cur.head * g + (row - (int)((row * inv_g) >> 16) * g)] * kLog2e - (M[n] == -INFINITY ? 0.f : M[n]));
+            const float inv = S[n] == 0.f ? 0.f : 1.f / S[n];
 #pragma unroll
-              for (int b = 0; b < kBlk; ++b)
-                reinterpret_cast<T*>(p.out)[out_row(row_of + n) + b * 128] = from_f<T>(acc[b][n] * sInv[row_of + n]);
-            }
+            for (int b = 0; b < kBlk; ++b) reinterpret_cast<T*>(p.out)[out_row(row) + b * 128] = from_f<T>(acc[b][n] * inv);
+          }
         }
         if (tid == 0) *ticket = 0;
-        named_bar_sync(1, kSoft);              // the exchange buffers are free for the next item
       }
     }
   }
