@@ -6,9 +6,9 @@
 //   * Queries: q times a power of two that puts the row's largest element in (128, 256] is the sum of e4m3 pieces, each the rounded rest
 //     of those in front of it.  A piece has four significant bits and rests are signed, so two pieces hold the 8 bits of bf16 and three the
 //     11 of fp16 exactly, down to 2^-18 of the row's largest element.  All pieces add into one accumulator.
-//   * Weights: exp2(s - m) * 2^7 * v_scale / (largest v_scale so far) <= 2^8, in fp16 and then in the same pieces, each rest times 2^5 so that
+//   * Weights: exp2(s - m) * 2^3 * v_scale / (largest v_scale so far) <= 2^8, in fp16 and then in the same pieces, each rest times 2^5 so that
 //     weights far below the largest keep their digits; every piece has accumulator columns of its own.  Two pieces are off by less
-//     than 2^-8 (the rounding of a bf16 weight), three carry the 11 bits of fp16.
+//     than 2^-8 (the rounding of a bf16 weight) and by 2^-18 of the largest, three carry the 11 bits of fp16 and are off by 2^-23 of it.
 // Few query rows and many keys: keys are the UMMA M side, query rows the N side.
 //     S^T[128 rows, 16]        = K[128 rows, 128 B] . Q^T      per piece, K-major as cached
 //     O^T[128 dims, 16 pieces] += V^T[128 dims, 128 rows] . P   V MN-major as cached
@@ -20,9 +20,10 @@
 // that uneven requests cost what their sum costs.  Where a cut falls, from the lengths on the device: captured launches adapt.  An item
 // that lies in several CTAs is merged by the last of them to arrive, in the order of the cuts: the result does not depend on who that is.
 // 192, 320 or 576 threads: warp 0 TMA producer (a lane per box of a tile, which looks its block up a tile ahead), warp 1 MMA issuer, the others
-// softmax (thread = row of the tile; TMEM lane = output dim at the end) and queries: four warps for 8 scores a row of the tile at most, as many
-// groups of four as there are eights otherwise, by query rows and, with heads of 64, by keys.  What is done once an item is kept short in code as well as in
-// time: half of a call's time went into it before, most of that into fetching instructions.  Every wait is bounded; on time-out the status word is
+// softmax (thread = row of the tile; TMEM lane = output dim at the end) and queries: groups of four warps that share the scores of a row by
+// query rows, four a thread (eight of 16 with heads of 64), and with heads of 64 by keys.  What is done once an item is kept short in code as
+// well as in time: half of a call's time went into it before, most of that into fetching instructions.  Merging waits for the end of
+// the CTA's work, where one fence serves both of its cut items.  Every wait is bounded; on time-out the status word is
 // set and the CTA unwinds.
 #include <cuda.h>
 #include <math.h>
@@ -39,8 +40,9 @@ namespace kv8dec {
 constexpr int kM = 128;          // rows of 128 bytes in a tile
 constexpr int kRows = 16;        // query rows, zero padded
 constexpr int kMaxB = 2048;      // requests a launch
-constexpr float kSlack = 1.f;    // the running maximum moves when a score exceeds it by more (log2): weights stay below 2^(7 + 1)
-constexpr float kLift = 7.f;
+// The running maximum moves when a score exceeds it by more than kSlack (log2): weights stay below 2^(kLift + kSlack).  With 7 and 1 every item
+// moved it several times.
+constexpr float kSlack = 5.f, kLift = 3.f;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Params {
@@ -74,11 +76,11 @@ template <> struct Pieces<__half> { static constexpr int n = 3; };
 template <typename T, int D, int NR> struct Layout {
   using G = Geo<D>;
   static constexpr int P = Pieces<T>::n;
-  // groups of four softmax warps; a thread has at most 8 scores of a tile
-  static constexpr int kKeyGroups = G::kPack == 2 && NR >= 8 ? 2 : 1, kRowGroups = NR == 16 ? 2 : 1, kGroups = kKeyGroups * kRowGroups;
+  // groups of four softmax warps
+  static constexpr int kKeyGroups = G::kPack, kRowGroups = NR == 4 ? 1 : NR == 8 || G::kPack == 2 ? 2 : 4, kGroups = kKeyGroups * kRowGroups;
   static constexpr int kSoft = 128 * kGroups, kThreads = 64 + kSoft;
-  static constexpr int kCtas = D == 256 || (D == 64 && NR == 16) ? 1 : 2;        // an SM at most: shared memory, registers
-  static constexpr int kKeysOf = G::kPack / kKeyGroups, kRowsOf = NR / kRowGroups;       // keys of a row and query rows of a thread
+  static constexpr int kCtas = D == 256 || kGroups == 4 ? 1 : 2;        // an SM at most: shared memory, registers
+  static constexpr int kKeysOf = 1, kRowsOf = NR / kRowGroups;          // keys of a row and query rows of a thread
   static constexpr int kNO = G::kNS * P;                       // columns of an O^T accumulator
   static constexpr int kQ = P * G::kBlk * G::kNS * 128;        // queries
   static constexpr int kP = kNO * 128;                         // one weight buffer
@@ -199,7 +201,8 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
   float* sSum = sMax + 16 * 9;                               // [16][8]
   float* sInv = sSum + 16 * 8;                               // [16]
   int* sScan = reinterpret_cast<int*>(sInv + kRows);         // [18]
-  float* sHalf = reinterpret_cast<float*>(sScan + 20);       // [16][64] (heads of 64)
+  int* sPend = sScan + 20;                                   // [2][8] the CTA's cut items: ticket, first unit, its CTAs, rows, output
+  float* sHalf = reinterpret_cast<float*>(sPend + 16);       // [16][64] (heads of 64)
   int* sPre = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(bars) + L::kMisc);   // [B + 1]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -484,6 +487,10 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
       if (lane == 0) mbar_arrive(q_ready);
     };
 
+    auto out_row = [&](int qs, int head0, int row) {
+      const int tok = (int)((row * inv_g) >> 16);
+      return ((int64_t)(qs + tok) * p.Hq + head0 + (row - tok * g)) * D + row_id;
+    };
     int t = 0;                                       // tiles so far
     int slot = 0;
     uint32_t phase = 0;
@@ -494,6 +501,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
       q_load(it, r);
       q_store(0);
     }
+    if (tid < 2) sPend[tid * 8 + 7] = 0;             // no cut item yet
     named_bar_sync(1, kSoft);                        // factors
 #pragma unroll 1
     for (int item = 0; it.more(); ++item) {
@@ -739,10 +747,6 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
           for (int n = 0; n < kRowsOf; ++n) o_mine[0][n] += sHalf[(row_of + n) * 64 + row_id];
         }
       }
-      auto out_row = [&](int row) {
-        const int tok = (int)((row * inv_g) >> 16);
-        return ((int64_t)(rc.qs + tok) * p.Hq + cur.head * g + (row - tok * g)) * D + row_id;
-      };
       const bool writes = (kPack == 1 || row_id < 64) && reads;
       if (writes) {
 #pragma unroll
@@ -754,24 +758,45 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
             for (int b = 0; b < kBlk; ++b) {
               const float v = inv == 0.f ? 0.f : o_mine[b][n] * inv;
               if (partial) p.ws_o[(my_slot * kRows + row) * D + b * 128 + row_id] = v;
-              else reinterpret_cast<T*>(p.out)[out_row(row) + b * 128] = from_f<T>(v);
+              else reinterpret_cast<T*>(p.out)[out_row(rc.qs, cur.head * g, row) + b * 128] = from_f<T>(v);
             }
           }
         }
       }
-      named_bar_sync(1, kSoft);
-      if (!partial) continue;
-      // ---- the last CTA of the item to arrive merges.  The barrier has ordered everyone's stores in front of this thread's release.
-      int* ticket = p.tickets + (int64_t)cur.req * p.Hkv + cur.head;
-      if (tid == 0) {
-        int seen;
-        asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(seen) : "l"(ticket) : "memory");
-        *s_last = seen == c1 - c0;
+      if (partial && tid == 0) {
+        int* pend = sPend + (item == 0 ? 0 : 8);      // the first and the last item of a CTA at most
+        pend[0] = cur.req * p.Hkv + cur.head;
+        pend[1] = first;
+        pend[2] = c0;
+        pend[3] = c1;
+        pend[4] = rows;
+        pend[5] = rc.qs;
+        pend[6] = cur.head * g;
+        pend[7] = 1;
       }
-      named_bar_sync(1, kSoft);
-      if (*s_last) {
+      named_bar_sync(1, kSoft);                        // the exchange buffers are free for the next item
+    }
+    // ---- the last CTA of an item to arrive merges.  The barrier has ordered everyone's stores in front of these threads' releases.
+    if (tid < 64 && lane == 0) {
+      const bool mine = sPend[tid == 0 ? 7 : 15] != 0;
+      int last = 0;
+      if (mine) {
+        const int* pend = sPend + (tid == 0 ? 0 : 8);
+        int seen;
+        asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(seen) : "l"(p.tickets + pend[0]) : "memory");
+        last = seen == pend[3] - pend[2];
+      }
+      s_last[tid >> 5] = last;
+    }
+    named_bar_sync(1, kSoft);
+#pragma unroll 1
+    for (int k = 0; k < 2; ++k) {
+      if (s_last[k] == 0) continue;
+      const int* pend = sPend + k * 8;
+      const int first = pend[1], c0 = pend[2], n_parts = pend[3] - c0 + 1, rows = pend[4], qs = pend[5], head0 = pend[6];
+      const bool writes = (kPack == 1 || row_id < 64) && (L::kKeyGroups == 1 || (row_id >> 6) == key_of);
         // every thread its dims: a few parts' log-sum-exps and results at a time, all in flight, joined in the order of the parts
-        const int n_parts = c1 - c0 + 1;
+        
         constexpr int kAtOnce = kRowsOf * kBlk > 8 || L::kGroups > 1 ? 2 : 4;
         float acc[kBlk][kRowsOf], M[kRowsOf], S[kRowsOf];
 #pragma unroll
@@ -821,14 +846,13 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
             const int row = row_of + n;
             if (row >= rows) continue;
             if (p.sinks != nullptr)
-              S[n] += exp2f(p.sinks[cur.head * g + (row - (int)((row * inv_g) >> 16) * g)] * kLog2e - (M[n] == -INFINITY ? 0.f : M[n]));
+              S[n] += exp2f(p.sinks[head0 + (row - (int)((row * inv_g) >> 16) * g)] * kLog2e - (M[n] == -INFINITY ? 0.f : M[n]));
             const float inv = S[n] == 0.f ? 0.f : 1.f / S[n];
 #pragma unroll
-            for (int b = 0; b < kBlk; ++b) reinterpret_cast<T*>(p.out)[out_row(row) + b * 128] = from_f<T>(acc[b][n] * inv);
+            for (int b = 0; b < kBlk; ++b) reinterpret_cast<T*>(p.out)[out_row(qs, head0, row) + b * 128] = from_f<T>(acc[b][n] * inv);
           }
         }
-        if (tid == 0) *ticket = 0;
-      }
+      if (tid == 0) p.tickets[pend[0]] = 0;
     }
   }
 

@@ -248,11 +248,11 @@ def oracle(b, window=0, sinks=None):
         mag_o = torch.einsum("hij,jhd->ihd", pv.nan_to_num(), v.nan_to_num().abs())
         lim[at:at + n] = mag_o * (eps_p + 2 * worst.T[..., None].nan_to_num() + 2.0 ** -17)
         # Weights far below a row's largest lose digits absolutely, too: exp(s - m) <= 1 for the largest is held in fp16, whose smallest step
-        # is 2^-24 (off by 2^-25), or, times 2^7 and v's scale over the largest one, as e4m3 pieces of which the last of two counts 2^-5:
-        # steps of 2^-9 / 2^5 / 2^7 = 2^-21 (off by 2^-22; three: 2^-27).  The sum of weights is 1 at least, so a result is off by no more
+        # is 2^-24 (off by 2^-25), or, times 2^3 and v's scale over the largest one, as e4m3 pieces of which the last of two counts 2^-5:
+        # steps of 2^-9 / 2^5 / 2^3 = 2^-17 (off by 2^-18; three: 2^-23).  The sum of weights is 1 at least, so a result is off by no more
         # than that times the sum of what the weights multiply, codes times the largest scale.
         if b["q"].dtype != torch.float32 and len(j):
-            unit = 2.0 ** (-22 if b["q"].dtype == torch.bfloat16 else -25)
+            unit = 2.0 ** (-18 if b["q"].dtype == torch.bfloat16 else -23)
             sc = scales[blk, 1, :, j % block].double().nan_to_num().amax(0).repeat_interleave(H // Hkv)
             cd = codes[blk, 1, :, j % block].double().nan_to_num().abs().repeat_interleave(H // Hkv, 1)
             lim[at:at + n] += unit * torch.einsum("ij,jhd->ihd", seen.double(), cd) * sc[:, None]
