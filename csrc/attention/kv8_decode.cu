@@ -21,7 +21,7 @@
 // that lies in several CTAs is merged by the last of them to arrive, in the order of the cuts: the result does not depend on who that is.
 // 192, 320 or 576 threads: warp 0 TMA producer (a lane per box of a tile, which looks its block up a tile ahead), warp 1 MMA issuer, the others
 // softmax (thread = row of the tile; TMEM lane = output dim at the end) and queries: groups of four warps that share the scores of a row by
-// query rows, four a thread (eight of 16 with heads of 64), and with heads of 64 by keys.  What is done once an item is kept short in code as
+// query rows and, with heads of 64, by keys, so that a thread has eight at most.  What is done once an item is kept short in code as
 // well as in time: half of a call's time went into it before, most of that into fetching instructions.  Merging waits for the end of
 // the CTA's work, where one fence serves both of its cut items.  Every wait is bounded; on time-out the status word is
 // set and the CTA unwinds.
@@ -76,8 +76,9 @@ template <> struct Pieces<__half> { static constexpr int n = 3; };
 template <typename T, int D, int NR> struct Layout {
   using G = Geo<D>;
   static constexpr int P = Pieces<T>::n;
-  // groups of four softmax warps
-  static constexpr int kKeyGroups = G::kPack, kRowGroups = NR == 4 ? 1 : NR == 8 || G::kPack == 2 ? 2 : 4, kGroups = kKeyGroups * kRowGroups;
+  // Groups of four softmax warps: heads of 64 a group for the even and one for the odd keys; 16 query rows in halves, and 8 where keys are
+  // halved already.  us with 8 rows in one group and in two, 16 requests of 4096 tokens: heads of 128 30.0 and 31.0, heads of 64 54.0 and 46.7.
+  static constexpr int kKeyGroups = G::kPack, kRowGroups = NR == 16 || (NR == 8 && G::kPack == 2) ? 2 : 1, kGroups = kKeyGroups * kRowGroups;
   static constexpr int kSoft = 128 * kGroups, kThreads = 64 + kSoft;
   static constexpr int kCtas = D == 256 || kGroups == 4 ? 1 : 2;        // an SM at most: shared memory, registers
   static constexpr int kKeysOf = 1, kRowsOf = NR / kRowGroups;          // keys of a row and query rows of a thread
