@@ -83,11 +83,141 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_put_kernel(const T* __restric
   put_row<NI>(x, c, slots[t], h, half, l);
 }
 
+// The common case of the kernel below: heads of 128, rotated whole in halves, 16 bits, 16-byte aligned.  Lane l of a half-warp has columns
+// 4 l .. 4 l + 3 and the same behind 64, so that a column meets its partner in its own thread; pairs of fp32 values go through one instruction; a
+// CTA reads its token's angles and the norms' weights once.  Bound by memory: 8192 tokens x (32 + 2 x 4) heads are 164 MB, 25 us.
+__device__ __forceinline__ uint64_t pk2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 un2(uint64_t r) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(r));
+  return f;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+template <typename T>
+__device__ __forceinline__ void unpack4(uint2 a, uint64_t (&v)[2]) {
+  const T* x = reinterpret_cast<const T*>(&a);
+  v[0] = pk2(to_f(x[0]), to_f(x[1]));
+  v[1] = pk2(to_f(x[2]), to_f(x[3]));
+}
+template <typename T> __device__ __forceinline__ uint32_t round2(uint64_t v);
+template <> __device__ __forceinline__ uint32_t round2<__nv_bfloat16>(uint64_t v) {
+  const float2 f = un2(v);
+  const __nv_bfloat162 r = __floats2bfloat162_rn(f.x, f.y);
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+template <> __device__ __forceinline__ uint32_t round2<__half>(uint64_t v) {
+  const float2 f = un2(v);
+  const __half2 r = __floats2half2_rn(f.x, f.y);
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+template <typename T, bool kNorm>
+__global__ void __launch_bounds__(kWarps * 32) kv8_qkv128_kernel(
+    T* __restrict__ q_out, const T* __restrict__ qkv, const int64_t* __restrict__ positions, const float* __restrict__ cos_sin,
+    const T* __restrict__ q_w, const T* __restrict__ k_w, float eps, int Hq, float gemma, Kv8Cache c,
+    const int64_t* __restrict__ slots, int64_t max_pos, int64_t qkv_stride) {
+  griddep_launch();
+  griddep_wait();
+  const int wid = threadIdx.x >> 5, lane = threadIdx.x & 31, half = lane >> 4, l = lane & 15;
+  const int64_t t = blockIdx.x;
+  const int q_units = (Hq + 1) / 2, units = q_units + c.Hkv;
+  int64_t pos = positions[t];
+  pos = pos < 0 ? 0 : (pos >= max_pos ? max_pos - 1 : pos);
+  const float4 cs4 = *reinterpret_cast<const float4*>(cos_sin + pos * 128 + l * 4);
+  const float4 sn4 = *reinterpret_cast<const float4*>(cos_sin + pos * 128 + 64 + l * 4);
+  const uint64_t cs[2] = {pk2(cs4.x, cs4.y), pk2(cs4.z, cs4.w)}, sn[2] = {pk2(sn4.x, sn4.y), pk2(sn4.z, sn4.w)};
+  const uint64_t minus = pk2(-1.f, -1.f);
+  const int64_t slot = slots[t];
+  const bool keep = slot >= 0 && slot < c.num_blocks * c.block_size;
+  const int64_t blk = keep ? slot / c.block_size : 0;
+  const int off = keep ? (int)(slot - blk * c.block_size) : 0;
+  const T* row = qkv + t * qkv_stride + l * 4;
+  for (int u = blockIdx.y * kWarps + wid; u < units; u += gridDim.y * kWarps) {
+    const bool is_q = u < q_units;
+    const int head = is_q ? 2 * u + half : Hq + (u - q_units) + half * c.Hkv;
+    const bool in = !is_q || head < Hq, turn = is_q || half == 0;
+    const T* src = row + (int64_t)(in ? head : 0) * 128;
+    uint64_t x[2], y[2];               // columns 4 l .. and 64 + 4 l ..
+    unpack4<T>(*reinterpret_cast<const uint2*>(src), x);
+    unpack4<T>(*reinterpret_cast<const uint2*>(src + 64), y);
+    if constexpr (kNorm) {
+      uint64_t sq = mul2(x[0], x[0]);
+      sq = fma2(x[1], x[1], sq);
+      sq = fma2(y[0], y[0], sq);
+      sq = fma2(y[1], y[1], sq);
+      const float2 s2 = un2(sq);
+      float s = s2.x + s2.y;
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      if (turn) {
+        const float inv = rsqrtf(s / 128 + eps);
+        const uint64_t inv2 = pk2(inv, inv), one = pk2(gemma, gemma), ones = pk2(1.f, 1.f);
+        const T* w = (is_q ? q_w : k_w) + l * 4;
+        uint64_t wx[2], wy[2];
+        unpack4<T>(*reinterpret_cast<const uint2*>(w), wx);
+        unpack4<T>(*reinterpret_cast<const uint2*>(w + 64), wy);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          x[j] = mul2(mul2(x[j], inv2), fma2(wx[j], ones, one));
+          y[j] = mul2(mul2(y[j], inv2), fma2(wy[j], ones, one));
+        }
+      }
+    }
+    if (turn) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint64_t a = fma2(x[j], cs[j], mul2(mul2(y[j], sn[j]), minus)), b = fma2(y[j], cs[j], mul2(x[j], sn[j]));
+        x[j] = a;
+        y[j] = b;
+      }
+    }
+    if (is_q) {
+      if (!in) continue;
+      T* dst = q_out + (t * Hq + head) * (int64_t)128 + l * 4;
+      *reinterpret_cast<uint2*>(dst) = make_uint2(round2<T>(x[0]), round2<T>(x[1]));
+      *reinterpret_cast<uint2*>(dst + 64) = make_uint2(round2<T>(y[0]), round2<T>(y[1]));
+      continue;
+    }
+    const float2 f[4] = {un2(x[0]), un2(x[1]), un2(y[0]), un2(y[1])};
+    float amax = 0.f;
+    bool nan = false;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      amax = fmaxf(amax, fmaxf(fabsf(f[j].x), fabsf(f[j].y)));
+      nan |= is_nan_bits(f[j].x) | is_nan_bits(f[j].y);
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    nan = __any_sync(0xffffffffu, nan);
+    if (!keep) continue;                 // padding: the whole warp
+    const float s = kv8_scale(amax), inv = pow2_inv(s);
+    uint8_t* page = c.page(blk, half, u - q_units);
+    uint8_t* dst = c.codes(page, off) + l * 4;
+    const float v[8] = {f[0].x, f[0].y, f[1].x, f[1].y, f[2].x, f[2].y, f[3].x, f[3].y};
+    const uint2 codes = nan ? make_uint2(0, 0) : kv8_pack8(v, inv);
+    *reinterpret_cast<uint32_t*>(dst) = codes.x;
+    *reinterpret_cast<uint32_t*>(dst + 64) = codes.y;
+    if (l == 0) *c.scale(page, off) = nan ? __uint_as_float(0x7fffffffu) : s;
+  }
+}
+
 // A fused qkv row: split, optional RMSNorm of query and key heads, rotation, queries out in T, keys and values into the cache.
 // A warp takes two query heads, or the key and the value of one head; all in fp32 between the load and the one rounding at the
-// end (no rounding to T between norm and rotation, nor in front of the codes).  `kFast`: heads of 128 rotated whole in halves, 16-byte
-// aligned: a column's partner is the lane eight places away.  Otherwise rows meet their partners in shared memory.
-template <typename T, int NI, bool kFast, bool kVec>
+// end (no rounding to T between norm and rotation, nor in front of the codes).  Columns meet their partners in shared memory.
+template <typename T, int NI, bool kVec>
 __global__ void __launch_bounds__(kWarps * 32) kv8_qkv_kernel(
     T* __restrict__ q_out, const T* __restrict__ qkv, const int64_t* __restrict__ positions, const float* __restrict__ cos_sin,
     const T* __restrict__ q_w, const T* __restrict__ k_w, float eps, int Hq, int rot, int neox, float gemma, Kv8Cache c,
@@ -102,17 +232,6 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_qkv_kernel(
   pos = pos < 0 ? 0 : (pos >= max_pos ? max_pos - 1 : pos);
   const float* cs = cos_sin + pos * rot;
   const int64_t slot = slots[t];
-  float cc[8], ss[8];
-  if constexpr (kFast) {
-    // x' = x c - y s on the first half, y' = y c + x s on the second: own * c + partner * (-s or s)
-#pragma unroll
-    for (int j = 0; j < 8; j += 4) {
-      *reinterpret_cast<float4*>(&cc[j]) = *reinterpret_cast<const float4*>(cs + (l & 7) * 8 + j);
-      *reinterpret_cast<float4*>(&ss[j]) = *reinterpret_cast<const float4*>(cs + 64 + (l & 7) * 8 + j);
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) ss[j] = l < 8 ? -ss[j] : ss[j];
-  }
   for (int u = blockIdx.y * kWarps + wid; u < units; u += gridDim.y * kWarps) {
     const bool is_q = u < q_units;
     const int head = is_q ? 2 * u + half : Hq + (u - q_units) + half * c.Hkv;
@@ -140,13 +259,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_qkv_kernel(
         }
       }
     }
-    if constexpr (kFast) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float other = __shfl_xor_sync(0xffffffffu, v[0][j], 8);
-        if (turn) v[0][j] = v[0][j] * cc[j] + other * ss[j];
-      }
-    } else {
+    {
       float* buf = sm_rows + (wid * 2 + half) * D;
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
@@ -276,17 +389,29 @@ extern "C" int b200_kv8_qkv(void* q_out, const void* qkv, const int64_t* positio
   const Kv8Cache c = cache_of(cache, num_blocks, Hkv, block_size, D);
   const int units = (Hq + 1) / 2 + Hkv, esize = dtype == kF32 ? 4 : 2;
   const bool vec = aligned16(qkv) && qkv_stride * esize % 16 == 0 && aligned16(q_w) && aligned16(k_w);
-  const bool fast = vec && D == 128 && rot_dim == 128 && neox && aligned16(cos_sin);
+  const bool fast = vec && D == 128 && rot_dim == 128 && neox && dtype != kF32 && aligned16(cos_sin) && aligned16(q_out) &&
+                    (q_w == nullptr) == (k_w == nullptr);
   // few tokens: a warp per unit, so that a decode step is one turn deep; otherwise a CTA per token, which reads its angles once
   const dim3 grid((unsigned)T_, T_ <= 384 ? (unsigned)((units + kWarps - 1) / kWarps) : 1u);
-  const size_t smem = fast ? 0 : (size_t)kWarps * 2 * D * sizeof(float);
-#define B200_KV8_QKV(NI, FAST, VEC)                                                                                            \
-  B200_DISPATCH_DTYPE(dtype, return (int)launch_pdl(kv8_qkv_kernel<T, NI, FAST, VEC>, grid, dim3(kWarps * 32), smem, st,       \
+  if (fast) {
+#define B200_KV8_QKV128(TT, NORM)                                                                                              \
+  return (int)launch_pdl(kv8_qkv128_kernel<TT, NORM>, grid, dim3(kWarps * 32), 0, st, (TT*)q_out, (const TT*)qkv, positions,   \
+                         cos_sin, (const TT*)q_w, (const TT*)k_w, eps, Hq, gemma ? 1.f : 0.f, c, slots, max_pos, qkv_stride)
+    if (dtype == kBF16) {
+      if (q_w != nullptr) B200_KV8_QKV128(__nv_bfloat16, true);
+      B200_KV8_QKV128(__nv_bfloat16, false);
+    }
+    if (q_w != nullptr) B200_KV8_QKV128(__half, true);
+    B200_KV8_QKV128(__half, false);
+#undef B200_KV8_QKV128
+  }
+  const size_t smem = (size_t)kWarps * 2 * D * sizeof(float);
+#define B200_KV8_QKV(NI, VEC)                                                                                                  \
+  B200_DISPATCH_DTYPE(dtype, return (int)launch_pdl(kv8_qkv_kernel<T, NI, VEC>, grid, dim3(kWarps * 32), smem, st,             \
                                                     (T*)q_out, (const T*)qkv, positions, cos_sin, (const T*)q_w, (const T*)k_w, \
                                                     eps, Hq, rot_dim, neox, gemma ? 1.f : 0.f, c, slots, max_pos, qkv_stride))
-#define B200_KV8_QKV_NI(NI) if (vec) { B200_KV8_QKV(NI, false, true); } else { B200_KV8_QKV(NI, false, false); }
-  if (fast) { B200_KV8_QKV(1, true, true); }
-  else if (D <= 128) { B200_KV8_QKV_NI(1) }
+#define B200_KV8_QKV_NI(NI) if (vec) { B200_KV8_QKV(NI, true); } else { B200_KV8_QKV(NI, false); }
+  if (D <= 128) { B200_KV8_QKV_NI(1) }
   else if (D <= 256) { B200_KV8_QKV_NI(2) }
   else { B200_KV8_QKV_NI(4) }
 #undef B200_KV8_QKV_NI
