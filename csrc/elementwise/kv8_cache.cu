@@ -134,25 +134,34 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_qkv128_kernel(
   const int wid = threadIdx.x >> 5, lane = threadIdx.x & 31, half = lane >> 4, l = lane & 15;
   const int64_t t = blockIdx.x;
   const int q_units = (Hq + 1) / 2, units = q_units + c.Hkv;
+  const T* row = qkv + t * qkv_stride + l * 4;
+  const auto head_of = [&](int u) { return u < q_units ? 2 * u + half : Hq + (u - q_units) + half * c.Hkv; };
+  uint2 xr, yr;                          // of the unit at hand; the next one's are loaded before its arithmetic
+  const auto fetch = [&](int u) {
+    const int head = head_of(u);
+    const T* src = row + (int64_t)(u < q_units && head >= Hq ? 0 : head) * 128;
+    xr = *reinterpret_cast<const uint2*>(src);
+    yr = *reinterpret_cast<const uint2*>(src + 64);
+  };
+  int u = blockIdx.y * kWarps + wid;
+  if (u >= units) return;
+  fetch(u);
   int64_t pos = positions[t];
+  const int64_t slot = slots[t];
   pos = pos < 0 ? 0 : (pos >= max_pos ? max_pos - 1 : pos);
   const float4 cs4 = *reinterpret_cast<const float4*>(cos_sin + pos * 128 + l * 4);
   const float4 sn4 = *reinterpret_cast<const float4*>(cos_sin + pos * 128 + 64 + l * 4);
   const uint64_t cs[2] = {pk2(cs4.x, cs4.y), pk2(cs4.z, cs4.w)}, sn[2] = {pk2(sn4.x, sn4.y), pk2(sn4.z, sn4.w)};
   const uint64_t minus = pk2(-1.f, -1.f);
-  const int64_t slot = slots[t];
-  const bool keep = slot >= 0 && slot < c.num_blocks * c.block_size;
-  const int64_t blk = keep ? slot / c.block_size : 0;
-  const int off = keep ? (int)(slot - blk * c.block_size) : 0;
-  const T* row = qkv + t * qkv_stride + l * 4;
-  for (int u = blockIdx.y * kWarps + wid; u < units; u += gridDim.y * kWarps) {
+  for (; u < units; u += gridDim.y * kWarps) {
     const bool is_q = u < q_units;
-    const int head = is_q ? 2 * u + half : Hq + (u - q_units) + half * c.Hkv;
+    const int head = head_of(u);
     const bool in = !is_q || head < Hq, turn = is_q || half == 0;
-    const T* src = row + (int64_t)(in ? head : 0) * 128;
-    uint64_t x[2], y[2];               // columns 4 l .. and 64 + 4 l ..
-    unpack4<T>(*reinterpret_cast<const uint2*>(src), x);
-    unpack4<T>(*reinterpret_cast<const uint2*>(src + 64), y);
+    uint64_t x[2], y[2];                 // columns 4 l .. and 64 + 4 l ..
+    unpack4<T>(xr, x);
+    unpack4<T>(yr, y);
+    const int next = u + gridDim.y * kWarps;
+    if (next < units) fetch(next);
     if constexpr (kNorm) {
       uint64_t sq = mul2(x[0], x[0]);
       sq = fma2(x[1], x[1], sq);
@@ -202,7 +211,9 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_qkv128_kernel(
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
     nan = __any_sync(0xffffffffu, nan);
-    if (!keep) continue;                 // padding: the whole warp
+    if (slot < 0 || slot >= c.num_blocks * c.block_size) continue;   // padding: the whole warp
+    const int64_t blk = slot >> 32 ? slot / c.block_size : (int64_t)((uint32_t)slot / (uint32_t)c.block_size);
+    const int off = (int)(slot - blk * c.block_size);
     const float s = kv8_scale(amax), inv = pow2_inv(s);
     uint8_t* page = c.page(blk, half, u - q_units);
     uint8_t* dst = c.codes(page, off) + l * 4;
