@@ -5,6 +5,8 @@
 // warp take a token's key and value of the same head, because a NaN in either marks both.
 #include <math.h>
 
+#include <algorithm>
+
 #include "../api.h"
 #include "../common/kv8.cuh"
 #include "../common/launch.cuh"
@@ -83,9 +85,13 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_put_kernel(const T* __restric
   put_row<NI>(x, c, slots[t], h, half, l);
 }
 
-// The common case of the kernel below: heads of 128, rotated whole in halves, 16 bits, 16-byte aligned.  Lane l of a half-warp has columns
-// 4 l .. 4 l + 3 and the same behind 64, so that a column meets its partner in its own thread; pairs of fp32 values go through one instruction; a
-// CTA reads its token's angles and the norms' weights once.  Bound by memory: 8192 tokens x (32 + 2 x 4) heads are 164 MB, 25 us.
+// The common case of the kernel below: heads of 128, rotated whole in halves, 16 bits, 16-byte aligned.  Eight lanes have a head, lane l of
+// them columns 8 l .. 8 l + 7 and the same behind 64, so that a column meets its partner in its own thread.  With w the norm's weight and 1 / n
+// the norm, a column is (x w_x cos - y w_y sin) / n: the products of weights and angles are the token's, not the head's.  A warp takes four
+// heads a step, with copies of the next steps in flight; a token has one warp, or more, up to one a step, where there are too few tokens to
+// fill the GPU's three CTAs of eight warps an SM.  8192 tokens of 32 + 2 x 4 heads, 164 MB, 25 us of memory: 36 us.  48 us with two heads a
+// step and their angles and weights multiplied head by head (twice the instructions); 47 with the next step's loads in registers and two
+// warps a token, 38 with four steps in flight in shared memory, 40 with six; 36 with one warp.
 __device__ __forceinline__ uint64_t pk2(float a, float b) {
   uint64_t r;
   asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
@@ -106,11 +112,15 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
   return d;
 }
+__device__ __forceinline__ void copy16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+}
+constexpr int kRing = 4;
 template <typename T>
-__device__ __forceinline__ void unpack4(uint2 a, uint64_t (&v)[2]) {
+__device__ __forceinline__ void unpack8(uint4 a, uint64_t (&v)[4]) {
   const T* x = reinterpret_cast<const T*>(&a);
-  v[0] = pk2(to_f(x[0]), to_f(x[1]));
-  v[1] = pk2(to_f(x[2]), to_f(x[3]));
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = pk2(to_f(x[2 * j]), to_f(x[2 * j + 1]));
 }
 template <typename T> __device__ __forceinline__ uint32_t round2(uint64_t v);
 template <> __device__ __forceinline__ uint32_t round2<__nv_bfloat16>(uint64_t v) {
@@ -125,102 +135,133 @@ template <> __device__ __forceinline__ uint32_t round2<__half>(uint64_t v) {
 }
 
 template <typename T, bool kNorm>
-__global__ void __launch_bounds__(kWarps * 32) kv8_qkv128_kernel(
+__global__ void __launch_bounds__(kWarps * 32, 3) kv8_qkv128_kernel(
     T* __restrict__ q_out, const T* __restrict__ qkv, const int64_t* __restrict__ positions, const float* __restrict__ cos_sin,
     const T* __restrict__ q_w, const T* __restrict__ k_w, float eps, int Hq, float gemma, Kv8Cache c,
-    const int64_t* __restrict__ slots, int64_t max_pos, int64_t qkv_stride) {
+    const int64_t* __restrict__ slots, int64_t max_pos, int64_t qkv_stride, int64_t tokens, int share) {
   griddep_launch();
   griddep_wait();
-  const int wid = threadIdx.x >> 5, lane = threadIdx.x & 31, half = lane >> 4, l = lane & 15;
-  const int64_t t = blockIdx.x;
-  const int q_units = (Hq + 1) / 2, units = q_units + c.Hkv;
-  const T* row = qkv + t * qkv_stride + l * 4;
-  const auto head_of = [&](int u) { return u < q_units ? 2 * u + half : Hq + (u - q_units) + half * c.Hkv; };
-  uint2 xr, yr;                          // of the unit at hand; the next one's are loaded before its arithmetic
-  const auto fetch = [&](int u) {
-    const int head = head_of(u);
-    const T* src = row + (int64_t)(u < q_units && head >= Hq ? 0 : head) * 128;
-    xr = *reinterpret_cast<const uint2*>(src);
-    yr = *reinterpret_cast<const uint2*>(src + 64);
+  const int lane = threadIdx.x & 31, part = lane >> 3, l = lane & 7;
+  const int64_t w = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5), t = w / share;
+  const int q_units = (Hq + 3) / 4, units = q_units + (c.Hkv + 1) / 2;
+  int u = (int)(w - t * share);
+  if (t >= tokens || u >= units) return;
+  const T* row = qkv + t * qkv_stride + l * 8;
+  // A unit is four query heads, or the keys and values of two.
+  const bool value = part & 1;
+  const auto head_of = [&](int u) { return u < q_units ? 4 * u + part : 2 * (u - q_units) + part / 2; };
+  // Loads of kRing units are in flight a warp; a lane copies to shared memory what it reads there itself.
+  __shared__ uint4 ring[kWarps][kRing][2][32];
+  uint4(*const mine)[2][32] = ring[threadIdx.x >> 5];
+  const auto fetch = [&](int u, int at) {
+    if (u < units) {
+      const int h = head_of(u);
+      const T* src = row + (int64_t)(u < q_units ? min(h, Hq - 1) : Hq + min(h, c.Hkv - 1) + (value ? c.Hkv : 0)) * 128;
+      copy16(&mine[at][0][lane], src);
+      copy16(&mine[at][1][lane], src + 64);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  int u = blockIdx.y * kWarps + wid;
-  if (u >= units) return;
-  fetch(u);
+#pragma unroll
+  for (int i = 0; i < kRing; ++i) fetch(u + i * share, i);
   int64_t pos = positions[t];
   const int64_t slot = slots[t];
   pos = pos < 0 ? 0 : (pos >= max_pos ? max_pos - 1 : pos);
-  const float4 cs4 = *reinterpret_cast<const float4*>(cos_sin + pos * 128 + l * 4);
-  const float4 sn4 = *reinterpret_cast<const float4*>(cos_sin + pos * 128 + 64 + l * 4);
-  const uint64_t cs[2] = {pk2(cs4.x, cs4.y), pk2(cs4.z, cs4.w)}, sn[2] = {pk2(sn4.x, sn4.y), pk2(sn4.z, sn4.w)};
-  const uint64_t minus = pk2(-1.f, -1.f);
-  for (; u < units; u += gridDim.y * kWarps) {
+  const float* angles = cos_sin + pos * 128 + l * 8;
+  uint64_t xc[4], xs[4], yc[4], ys[4];   // weight x cosine and sine of either half, -sine in ys
+  const auto turns = [&](const T* weight) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const float4 cs = reinterpret_cast<const float4*>(angles)[j], sn = reinterpret_cast<const float4*>(angles + 64)[j];
+      xc[2 * j] = yc[2 * j] = pk2(cs.x, cs.y), xc[2 * j + 1] = yc[2 * j + 1] = pk2(cs.z, cs.w);
+      xs[2 * j] = pk2(sn.x, sn.y), xs[2 * j + 1] = pk2(sn.z, sn.w);
+      ys[2 * j] = pk2(-sn.x, -sn.y), ys[2 * j + 1] = pk2(-sn.z, -sn.w);
+    }
+    if constexpr (kNorm) {
+      uint64_t wx[4], wy[4];
+      unpack8<T>(*reinterpret_cast<const uint4*>(weight + l * 8), wx);
+      unpack8<T>(*reinterpret_cast<const uint4*>(weight + l * 8 + 64), wy);
+      const uint64_t ones = pk2(1.f, 1.f), g = pk2(gemma, gemma);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        wx[j] = fma2(wx[j], ones, g);
+        wy[j] = fma2(wy[j], ones, g);
+        xc[j] = mul2(xc[j], wx[j]);
+        xs[j] = mul2(xs[j], wx[j]);
+        yc[j] = mul2(yc[j], wy[j]);
+        ys[j] = mul2(ys[j], wy[j]);
+      }
+    }
+  };
+  bool keys = u >= q_units;
+  turns(keys ? k_w : q_w);
+  int at = 0;
+  for (; u < units; u += share) {
     const bool is_q = u < q_units;
-    const int head = head_of(u);
-    const bool in = !is_q || head < Hq, turn = is_q || half == 0;
-    uint64_t x[2], y[2];                 // columns 4 l .. and 64 + 4 l ..
-    unpack4<T>(xr, x);
-    unpack4<T>(yr, y);
-    const int next = u + gridDim.y * kWarps;
-    if (next < units) fetch(next);
+    const int h = head_of(u);
+    if (kNorm && !is_q && !keys) {
+      keys = true;
+      turns(k_w);
+    }
+    uint64_t x[4], y[4];                 // columns 8 l .. and 64 + 8 l ..
+    asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 1) : "memory");
+    unpack8<T>(mine[at][0][lane], x);
+    unpack8<T>(mine[at][1][lane], y);
+    uint64_t inv2 = 0;
     if constexpr (kNorm) {
       uint64_t sq = mul2(x[0], x[0]);
-      sq = fma2(x[1], x[1], sq);
-      sq = fma2(y[0], y[0], sq);
-      sq = fma2(y[1], y[1], sq);
+#pragma unroll
+      for (int j = 1; j < 4; ++j) sq = fma2(x[j], x[j], sq);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sq = fma2(y[j], y[j], sq);
       const float2 s2 = un2(sq);
       float s = s2.x + s2.y;
 #pragma unroll
-      for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      if (turn) {
-        const float inv = rsqrtf(s / 128 + eps);
-        const uint64_t inv2 = pk2(inv, inv), one = pk2(gemma, gemma), ones = pk2(1.f, 1.f);
-        const T* w = (is_q ? q_w : k_w) + l * 4;
-        uint64_t wx[2], wy[2];
-        unpack4<T>(*reinterpret_cast<const uint2*>(w), wx);
-        unpack4<T>(*reinterpret_cast<const uint2*>(w + 64), wy);
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          x[j] = mul2(mul2(x[j], inv2), fma2(wx[j], ones, one));
-          y[j] = mul2(mul2(y[j], inv2), fma2(wy[j], ones, one));
-        }
-      }
+      for (int o = 4; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      const float inv = rsqrtf(s / 128 + eps);
+      inv2 = pk2(inv, inv);
     }
-    if (turn) {
+    if (is_q || !value) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const uint64_t a = fma2(x[j], cs[j], mul2(mul2(y[j], sn[j]), minus)), b = fma2(y[j], cs[j], mul2(x[j], sn[j]));
+      for (int j = 0; j < 4; ++j) {
+        uint64_t a = fma2(x[j], xc[j], mul2(y[j], ys[j])), b = fma2(y[j], yc[j], mul2(x[j], xs[j]));
+        if constexpr (kNorm) a = mul2(a, inv2), b = mul2(b, inv2);
         x[j] = a;
         y[j] = b;
       }
     }
+    fetch(u + kRing * share, at);
+    at = at + 1 == kRing ? 0 : at + 1;
     if (is_q) {
-      if (!in) continue;
-      T* dst = q_out + (t * Hq + head) * (int64_t)128 + l * 4;
-      *reinterpret_cast<uint2*>(dst) = make_uint2(round2<T>(x[0]), round2<T>(x[1]));
-      *reinterpret_cast<uint2*>(dst + 64) = make_uint2(round2<T>(y[0]), round2<T>(y[1]));
+      if (h >= Hq) continue;
+      T* dst = q_out + (t * Hq + h) * (int64_t)128 + l * 8;
+      *reinterpret_cast<uint4*>(dst) = make_uint4(round2<T>(x[0]), round2<T>(x[1]), round2<T>(x[2]), round2<T>(x[3]));
+      *reinterpret_cast<uint4*>(dst + 64) = make_uint4(round2<T>(y[0]), round2<T>(y[1]), round2<T>(y[2]), round2<T>(y[3]));
       continue;
     }
-    const float2 f[4] = {un2(x[0]), un2(x[1]), un2(y[0]), un2(y[1])};
-    float amax = 0.f;
-    bool nan = false;
+    float f[2][8], amax = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      amax = fmaxf(amax, fmaxf(fabsf(f[j].x), fabsf(f[j].y)));
-      nan |= is_nan_bits(f[j].x) | is_nan_bits(f[j].y);
+      const float2 a = un2(x[j]), b = un2(y[j]);
+      f[0][2 * j] = a.x, f[0][2 * j + 1] = a.y, f[1][2 * j] = b.x, f[1][2 * j + 1] = b.y;
+    }
+    bool nan = false;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      amax = fmaxf(amax, fabsf(f[j >> 3][j & 7]));
+      nan |= is_nan_bits(f[j >> 3][j & 7]);
     }
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    nan = __any_sync(0xffffffffu, nan);
-    if (slot < 0 || slot >= c.num_blocks * c.block_size) continue;   // padding: the whole warp
+    for (int o = 4; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    nan = (__ballot_sync(0xffffffffu, nan) >> (lane & 16) & 0xffffu) != 0;   // in the head's key or its value
+    if (slot < 0 || slot >= c.num_blocks * c.block_size || h >= c.Hkv) continue;
     const int64_t blk = slot >> 32 ? slot / c.block_size : (int64_t)((uint32_t)slot / (uint32_t)c.block_size);
     const int off = (int)(slot - blk * c.block_size);
     const float s = kv8_scale(amax), inv = pow2_inv(s);
-    uint8_t* page = c.page(blk, half, u - q_units);
-    uint8_t* dst = c.codes(page, off) + l * 4;
-    const float v[8] = {f[0].x, f[0].y, f[1].x, f[1].y, f[2].x, f[2].y, f[3].x, f[3].y};
-    const uint2 codes = nan ? make_uint2(0, 0) : kv8_pack8(v, inv);
-    *reinterpret_cast<uint32_t*>(dst) = codes.x;
-    *reinterpret_cast<uint32_t*>(dst + 64) = codes.y;
+    uint8_t* page = c.page(blk, value, h);
+    uint8_t* dst = c.codes(page, off) + l * 8;
+    *reinterpret_cast<uint2*>(dst) = nan ? make_uint2(0, 0) : kv8_pack8(f[0], inv);
+    *reinterpret_cast<uint2*>(dst + 64) = nan ? make_uint2(0, 0) : kv8_pack8(f[1], inv);
     if (l == 0) *c.scale(page, off) = nan ? __uint_as_float(0x7fffffffu) : s;
   }
 }
@@ -405,9 +446,12 @@ extern "C" int b200_kv8_qkv(void* q_out, const void* qkv, const int64_t* positio
   // few tokens: a warp per unit, so that a decode step is one turn deep; otherwise a CTA per token, which reads its angles once
   const dim3 grid((unsigned)T_, T_ <= 384 ? (unsigned)((units + kWarps - 1) / kWarps) : 1u);
   if (fast) {
+    const int steps = (Hq + 3) / 4 + (Hkv + 1) / 2, share = (int)std::max<int64_t>(1, std::min<int64_t>(steps, (148 * 3 * kWarps + T_ - 1) / T_));
+    if (T_ * share > ((int64_t)1 << 33)) return 2;
 #define B200_KV8_QKV128(TT, NORM)                                                                                              \
-  return (int)launch_pdl(kv8_qkv128_kernel<TT, NORM>, grid, dim3(kWarps * 32), 0, st, (TT*)q_out, (const TT*)qkv, positions,   \
-                         cos_sin, (const TT*)q_w, (const TT*)k_w, eps, Hq, gemma ? 1.f : 0.f, c, slots, max_pos, qkv_stride)
+  return (int)launch_pdl(kv8_qkv128_kernel<TT, NORM>, dim3((unsigned)((T_ * share + kWarps - 1) / kWarps)), dim3(kWarps * 32), 0, st, \
+                         (TT*)q_out, (const TT*)qkv, positions, cos_sin, (const TT*)q_w, (const TT*)k_w, eps, Hq, gemma ? 1.f : 0.f,   \
+                         c, slots, max_pos, qkv_stride, T_, share)
     if (dtype == kBF16) {
       if (q_w != nullptr) B200_KV8_QKV128(__nv_bfloat16, true);
       B200_KV8_QKV128(__nv_bfloat16, false);
