@@ -16,6 +16,9 @@ namespace {
 
 constexpr int kWarps = 8;
 
+// a / b of non-negative numbers; a division of 64 bits is some hundred instructions, and few numbers here need it.
+__device__ __forceinline__ int64_t quotient(int64_t a, int b) { return a >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b); }
+
 // elements 8 l .. 8 l + 7 of every 128 of a row of D; zeros behind its end
 template <typename T, int NI, bool kVec>
 __device__ __forceinline__ void load_row(float (&v)[NI][8], const T* src, int D, int l) {
@@ -58,8 +61,9 @@ __device__ __forceinline__ void put_row(const float (&v)[NI][8], const Kv8Cache&
   nan = __any_sync(0xffffffffu, nan);
   if (slot < 0 || slot >= c.num_blocks * c.block_size) return;      // padding: the whole warp
   const float s = kv8_scale(amax), inv = nan ? 0.f : pow2_inv(s);
-  const int off = (int)(slot % c.block_size);
-  uint8_t* page = c.page(slot / c.block_size, half, h);
+  const int64_t blk = quotient(slot, c.block_size);
+  const int off = (int)(slot - blk * c.block_size);
+  uint8_t* page = c.page(blk, half, h);
   uint8_t* dst = c.codes(page, off);
 #pragma unroll
   for (int i = 0; i < NI; ++i)
@@ -78,8 +82,8 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_put_kernel(const T* __restric
   const int64_t row = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
   if (row >= rows) return;
   const int lane = threadIdx.x & 31, half = lane >> 4, l = lane & 15;
-  const int64_t t = row / c.Hkv;
-  const int h = (int)(row % c.Hkv);
+  const int64_t t = quotient(row, c.Hkv);
+  const int h = (int)(row - t * c.Hkv);
   float x[NI][8];
   load_row<T, NI, kVec>(x, (half ? v + t * v_stride : k + t * k_stride) + (int64_t)h * c.D, c.D, l);
   put_row<NI>(x, c, slots[t], h, half, l);
@@ -255,7 +259,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) kv8_qkv128_kernel(
     for (int o = 4; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
     nan = (__ballot_sync(0xffffffffu, nan) >> (lane & 16) & 0xffffu) != 0;   // in the head's key or its value
     if (slot < 0 || slot >= c.num_blocks * c.block_size || h >= c.Hkv) continue;
-    const int64_t blk = slot >> 32 ? slot / c.block_size : (int64_t)((uint32_t)slot / (uint32_t)c.block_size);
+    const int64_t blk = quotient(slot, c.block_size);
     const int off = (int)(slot - blk * c.block_size);
     const float s = kv8_scale(amax), inv = pow2_inv(s);
     uint8_t* page = c.page(blk, value, h);
@@ -368,12 +372,12 @@ __global__ void __launch_bounds__(256) kv_gather_kernel(T* __restrict__ k, T* __
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= chunks) return;
   const int per = c.D / 16, which = blockIdx.y;
-  const int64_t row = i / per, m = row / c.Hkv;
-  const int at = (int)(i % per) * 16, h = (int)(row % c.Hkv);
+  const int64_t row = quotient(i, per), m = quotient(row, c.Hkv);
+  const int at = (int)(i - row * per) * 16, h = (int)(row - m * c.Hkv);
   const int64_t slot = slots[m];
   const bool in = slot >= 0 && slot < c.num_blocks * c.block_size;
-  const int64_t blk = in ? slot / c.block_size : 0;
-  const int off = in ? (int)(slot % c.block_size) : 0;
+  const int64_t blk = in ? quotient(slot, c.block_size) : 0;
+  const int off = in ? (int)(slot - blk * c.block_size) : 0;
   T* dst = (which ? v : k) + row * c.D + at;
   alignas(16) T o[16];
   if (!in) {
