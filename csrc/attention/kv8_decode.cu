@@ -17,7 +17,7 @@
 // Heads of 256: two 128-byte blocks a key, two O^T accumulators.
 //
 // Work: all tiles of all (request, head) items in one line, cut into equal pieces, one a CTA (two CTAs an SM where shared memory lasts), so
-// that uneven requests cost what their sum costs.  Where a cut falls, from the lengths on the device: captured launches adapt.  An item
+// that uneven requests cost what their sum costs.  Cuts come from the lengths on the device: captured launches adapt.  An item
 // that lies in several CTAs is merged by the last of them to arrive, in the order of the cuts: the result does not depend on who that is.
 // 192, 320 or 576 threads: warp 0 TMA producer (a lane per box of a tile, which looks its block up a tile ahead), warp 1 MMA issuer, the others
 // softmax (thread = row of the tile; TMEM lane = output dim at the end) and queries: groups of four warps that share the scores of a row by
@@ -43,6 +43,9 @@ constexpr int kMaxB = 2048;      // requests a launch
 // The running maximum moves when a score exceeds it by more than kSlack (log2): weights stay below 2^(kLift + kSlack).  With 7 and 1 every item
 // moved it several times.
 constexpr float kSlack = 5.f, kLift = 3.f;
+// A cut this close to an item's end moves there (tiles; CTAs of one tile keep theirs): one tile costs less than a merge of 16 rows.  us without
+// and with, 12 requests of 600 tokens, 8 heads of 128: 16 rows 26.5 and 21.8, 8 rows 18.1 and 15.7, 4 rows 14.3 and 13.1; of 2000: 37.6 and 38.0.
+constexpr int kSnap = 1;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Params {
@@ -58,7 +61,7 @@ struct Params {
   const float* sinks;
   int* status;
   int64_t num_blocks, bt_stride, q_stride;
-  int B, Hq, Hkv, block_size, max_blocks, max_keys, window, slots, early_meta, min_tiles;
+  int B, Hq, Hkv, block_size, max_blocks, max_keys, window, slots, early_meta;
   float scale_log2;
 };
 
@@ -115,6 +118,27 @@ __device__ __forceinline__ uint16_t f16x2_to_e4m3x2(__half2 v) {
 }
 __device__ __forceinline__ __half2 as_half2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
 
+// The last request whose tiles start at or before unit `at`: those without tiles lie in front of it.
+__device__ __forceinline__ int request_at(const int* pre, int B, int Hkv, int at) {
+  int a = 0, b = B;
+#pragma unroll 1
+  while (b - a > 1) {
+    const int mid = (a + b) >> 1;
+    if (pre[mid] * Hkv <= at) a = mid; else b = mid;
+  }
+  return a;
+}
+
+// Cut b of the line of units: b * share, moved to the end of an item that is at most `snap` tiles away.
+__device__ __forceinline__ int cut_at(const int* pre, int B, int Hkv, int units, int share, int snap, int b) {
+  const long long p = (long long)share * b;
+  if (p == 0 || p >= units) return p == 0 ? 0 : units;
+  const int at = (int)p, a = request_at(pre, B, Hkv, at), n = pre[a + 1] - pre[a];
+  const int in = (int)((unsigned)(at - pre[a] * Hkv) % (unsigned)n);
+  if (min(in, n - in) > snap) return at;
+  return in <= n - in ? at - in : at + n - in;
+}
+
 // A CTA's share of the line of tiles, item by item.
 struct Walk {
   const int* pre;          // [B + 1] tiles of the requests in front (of one head)
@@ -126,12 +150,7 @@ struct Walk {
     pre = pre_; B = B_; Hkv = Hkv_; at = lo; end = hi;
     count = 0;
     if (at >= end) return;
-    int a = 0, b = B;      // the last request whose tiles start at or before `at`: those without tiles lie in front of it
-#pragma unroll 1
-    while (b - a > 1) {
-      const int mid = (a + b) >> 1;
-      if (pre[mid] * Hkv <= at) a = mid; else b = mid;
-    }
+    const int a = request_at(pre, B, Hkv, at);
     req = a;
     n = pre[a + 1] - pre[a];
     const unsigned in = at - pre[a] * Hkv;
@@ -202,7 +221,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
   float* sSum = sMax + 16 * 9;                               // [16][8]
   float* sInv = sSum + 16 * 8;                               // [16]
   int* sScan = reinterpret_cast<int*>(sInv + kRows);         // [18]
-  int* sPend = sScan + 20;                                   // [2][8] the CTA's cut items: ticket, first unit, its CTAs, rows, output
+  int* sPend = sScan + 20;                                   // [2][8] the CTA's cut items: ticket, its CTAs, rows, output
   float* sHalf = reinterpret_cast<float*>(sPend + 16);       // [16][64] (heads of 64)
   int* sPre = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(bars) + L::kMisc);   // [B + 1]
 
@@ -266,8 +285,9 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
   const uint32_t tmem_base = *tmem_slot;
 
   const int units = sPre[p.B] * p.Hkv;
-  const int share = max((units + (int)gridDim.x - 1) / (int)gridDim.x, p.min_tiles);
-  const int lo = min((long long)units, (long long)share * blockIdx.x), hi = min(units - lo, share) + lo;
+  const int share = max((units + (int)gridDim.x - 1) / (int)gridDim.x, 1);
+  const int snap = share > 1 ? kSnap : 0;
+  const int lo = cut_at(sPre, p.B, p.Hkv, units, share, snap, blockIdx.x), hi = cut_at(sPre, p.B, p.Hkv, units, share, snap, blockIdx.x + 1);
   const int n_tiles = hi - lo;
   Walk it;
   it.start(sPre, p.B, p.Hkv, lo, hi);
@@ -697,9 +717,10 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
         }
       }
       const int first = sPre[cur.req] * p.Hkv + cur.head * cur.n;
-      const int c0 = first / share, c1 = (first + cur.n - 1) / share;      // the CTAs that have tiles of this item
-      const bool partial = c0 != c1;
-      const int64_t my_slot = 2 * (int64_t)blockIdx.x + ((long long)blockIdx.x * share >= first ? 0 : 1);
+      // the CTAs that have tiles of this item: its cuts lie more than `snap` from its ends
+      const int c0 = (first + snap) / share, c1 = cur.n > 2 * snap + 1 ? (first + cur.n - snap - 1) / share : 0;
+      const bool partial = c0 < c1;
+      const int64_t my_slot = 2 * (int64_t)blockIdx.x + ((int)blockIdx.x == c0 ? 1 : 0);
       if (ok && !wait_or_abort(o_final, item & 1, ab, 907)) ok = false;
       ok = bar_red_or(1, kSoft, !ok) == 0;   // one thread's time-out ends the work of all
       tc_fence_after_sync();
@@ -767,12 +788,11 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
       if (partial && tid == 0) {
         int* pend = sPend + (item == 0 ? 0 : 8);      // the first and the last item of a CTA at most
         pend[0] = cur.req * p.Hkv + cur.head;
-        pend[1] = first;
-        pend[2] = c0;
-        pend[3] = c1;
-        pend[4] = rows;
-        pend[5] = rc.qs;
-        pend[6] = cur.head * g;
+        pend[1] = c0;
+        pend[2] = c1;
+        pend[3] = rows;
+        pend[4] = rc.qs;
+        pend[5] = cur.head * g;
         pend[7] = 1;
       }
       named_bar_sync(1, kSoft);                        // the exchange buffers are free for the next item
@@ -785,7 +805,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
         const int* pend = sPend + (tid == 0 ? 0 : 8);
         int seen;
         asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(seen) : "l"(p.tickets + pend[0]) : "memory");
-        last = seen == pend[3] - pend[2];
+        last = seen == pend[2] - pend[1];
       }
       s_last[tid >> 5] = last;
     }
@@ -794,7 +814,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
     for (int k = 0; k < 2; ++k) {
       if (s_last[k] == 0) continue;
       const int* pend = sPend + k * 8;
-      const int first = pend[1], c0 = pend[2], n_parts = pend[3] - c0 + 1, rows = pend[4], qs = pend[5], head0 = pend[6];
+      const int c0 = pend[1], n_parts = pend[2] - c0 + 1, rows = pend[3], qs = pend[4], head0 = pend[5];
       const bool writes = (kPack == 1 || row_id < 64) && (L::kKeyGroups == 1 || (row_id >> 6) == key_of);
         // every thread its dims: a few parts' log-sum-exps and results at a time, all in flight, joined in the order of the parts
         
@@ -814,7 +834,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
 #pragma unroll
             for (int u = 0; u < kAtOnce; ++u) {
               const int c = c0 + min(base + u, n_parts - 1);
-              const int64_t at = (2 * (int64_t)c + ((long long)c * share >= first ? 0 : 1)) * kRows + row_of;
+              const int64_t at = (2 * (int64_t)c + (c == c0 ? 1 : 0)) * kRows + row_of;
 #pragma unroll
               for (int n = 0; n < kRowsOf; ++n) {
                 const bool in = row_of + n < rows && base + u < n_parts;
@@ -929,7 +949,7 @@ extern "C" int b200_kv8_decode(void* out, const void* q, const void* cache, cons
   p.block_tables = block_tables; p.seq_lens = seq_lens; p.qsl = qsl; p.sinks = sinks; p.status = status;
   p.num_blocks = num_blocks; p.bt_stride = bt_stride; p.q_stride = q_stride; p.Hq = Hq; p.Hkv = Hkv; p.block_size = block_size;
   p.max_blocks = max_blocks; p.max_keys = (int)((int64_t)max_blocks * block_size < 0x7ffffe00 ? max_blocks * block_size : 0x7ffffe00);
-  p.window = window; p.early_meta = early_meta; p.min_tiles = 1;
+  p.window = window; p.early_meta = early_meta;
   p.scale_log2 = scale * kv8dec::kLog2e;
   const CUtensorMap& tm = *reinterpret_cast<const CUtensorMap*>(tmap);
   const int rows = max_query_len * (Hq / Hkv), keys = D == 64 ? 256 : 128;
