@@ -167,6 +167,37 @@ def test_fused_write(device, dt, H, Hkv, D, rot, neox, norm, gemma, block, T):
     assert (raw == 0x33).all()
 
 
+@gpu
+@pytest.mark.parametrize("H,Hkv,norm", [(32, 4, True), (7, 3, False), (1, 1, True)])
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+def test_fused_write_of_many_tokens(dt, H, Hkv, norm):
+    """The same bits as in small calls; a NaN or an infinity in a key or value marks its token and head alone."""
+    T, D, block = 3700, 128, 16
+    g = torch.Generator().manual_seed(H)
+    qkv = torch.randn(T, (H + 2 * Hkv) * D, generator=g).to(DT[dt])
+    x = qkv.view(T, H + 2 * Hkv, D)
+    x[10, H, 5] = math.nan                       # key
+    x[11, H + 2 * Hkv - 1, 127] = math.nan       # value
+    x[12, H + Hkv, 64] = math.inf                # value: saturates
+    qkv = qkv.cuda()
+    w = [(1 + 0.1 * torch.randn(D, generator=g)).to(DT[dt]).cuda() if norm else None for _ in range(2)]
+    angle = torch.rand(T, 64, generator=g) * 6.3
+    cs = torch.cat([angle.cos(), angle.sin()], -1).cuda()
+    pos = torch.arange(T).cuda()
+    slots = torch.randperm(T + 60, generator=g)[:T].cuda()
+    caches = [new_cache((T + 60 + block) // block, Hkv, block, D, "cuda", 0x11) for _ in range(2)]
+    q = ops.qkv_split_norm_rope_cache(qkv, pos, cs, *w, 1e-6, H, Hkv, D, True, caches[0], slots)
+    parts = [ops.qkv_split_norm_rope_cache(qkv[i:i + 370], pos[i:i + 370], cs, *w, 1e-6, H, Hkv, D, True, caches[1], slots[i:i + 370])
+             for i in range(0, T, 370)]
+    assert torch.equal(q, torch.cat(parts)) and torch.equal(*caches)
+    k, v = ops.gather_kv_cache(caches[0], slots)
+    nan = (k.isnan() | v.isnan()).any(-1).cpu()
+    want = torch.zeros(T, Hkv, dtype=torch.bool)
+    want[10, 0] = want[11, Hkv - 1] = True
+    assert torch.equal(nan, want)
+    assert float(v[12, 0, 64]) == 448 * 128
+
+
 @pytest.mark.parametrize("device", DEVICES)
 def test_blocks_move_whole(device):
     k, v = special_rows(32, 2, 64, torch.bfloat16)
@@ -356,6 +387,67 @@ def test_rows_of_no_request_stay(D, dt):
         ops.paged_attention(q, b["cache"], b["table"], b["lens"], b["qsl"] + 4, b["scale"], b["max_q"], b["max_len"], out=out)
         check(out[4:4 + T], b)
         assert (out[:4] == 5).all() and (out[4 + T:] == 5).all()
+
+
+@gpu
+@pytest.mark.parametrize("D,new", [(128, 40), (128, 200), (64, 70), (64, 300), (256, 30)])
+@pytest.mark.parametrize("window", [1, 5, 130, 700])
+def test_windows_of_prompts(D, new, window):
+    """Windows inside a tile, over several and beyond the start, with a context; both prompt kernels."""
+    b = batch([new, 17, new + 1], [0, 600, 333], 4, 2, D, 32, torch.bfloat16, "cuda", seed=new)
+    check(attend(b, window), b, window)
+
+
+@gpu
+@pytest.mark.parametrize("new", [1, 9])
+def test_more_requests_than_a_launch_takes(new):
+    """4100 requests are three launches of 2048 at most, each with items that are cut."""
+    n = [new if i % 5 else 0 for i in range(4100)]
+    n[2047] = n[2048] = new
+    b = batch(n, [(17 * i) % 50 if i % 1000 else 900 for i in range(4100)], 2, 1, 64, 16, torch.bfloat16, "cuda")
+    check(attend(b), b)
+
+
+@gpu
+def test_long_bounds_and_wide_tables():
+    """Lengths far below what the call allows for: the scratch of a prompt is that of a few requests at a time."""
+    b = batch([70, 1, 300, 90, 5], [600, 20, 0, 130, 64], 8, 4, 128, 64, torch.bfloat16, "cuda")
+    want = attend(b)
+    check(want, b)
+    table = torch.full((5, 4000), -1, dtype=torch.int32, device="cuda")
+    table[:, :b["table"].shape[1]] = b["table"]
+    got = ops.paged_attention(b["q"], b["cache"], table, b["lens"], b["qsl"], b["scale"], b["max_q"], 250000)
+    check(got, b)
+    # the decode kernel cuts its line of tiles by the lengths, not by their bound
+    b = batch([1, 1, 2], [600, 20, 4000], 4, 2, 128, 64, torch.bfloat16, "cuda")
+    got = ops.paged_attention(b["q"], b["cache"], b["table"], b["lens"], b["qsl"], b["scale"], b["max_q"], 250000)
+    check(got, b)
+
+
+@gpu
+@pytest.mark.parametrize("D", [64, 128, 256, 96])
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+@pytest.mark.parametrize("new,context", [([1, 2, 1], [400, 37, 3]), ([50, 3], [30, 0]), ([300, 20], [100, 4])])
+def test_queries_that_are_not_numbers(D, dt, new, context):
+    """A NaN or an infinity in a query is its row's alone."""
+    b = batch(new, context, 4, 2, D, 64, DT[dt], "cuda", seed=5)
+    bad = torch.zeros(b["q"].shape[:2], dtype=torch.bool)
+    bad[0, 1] = bad[2, 3] = bad[-1, 0] = True
+    q = b["q"].clone()
+    q[0, 1, 3], q[2, 3, D - 1], q[-1, 0, 0] = math.nan, math.inf, -math.inf
+    got = attend({**b, "q": q}).cpu()
+    assert got[bad].isnan().all()
+    got[bad] = attend(b).cpu()[bad]
+    check(got, b)
+
+
+@gpu
+def test_items_around_the_cuts():
+    """One to many tiles a request and every number of requests up to 40: cuts on, next to and far from the ends of items."""
+    for n in (1, 2, 3, 7, 19, 40):
+        b = batch([1 + (i % 2) for i in range(n)], [(389 * i) % 1900 for i in range(n)], 8, 2, 128, 64, torch.bfloat16, "cuda", seed=n)
+        check(attend(b), b)
+        assert torch.equal(attend(b), attend(b))
 
 
 def test_refusals():

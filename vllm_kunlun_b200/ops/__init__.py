@@ -125,7 +125,8 @@ def mrope(q, k, positions3, cos_sin_cache, head_dim, sections, interleaved=False
 
 
 def reshape_and_cache(k, v, kv_cache, slot_mapping):
-    """Keys and values ``[T, kv_heads, head_dim]`` to their slots; negative slots are padding.  ``kv_cache``: in the type of ``k``,
+    """Keys and values ``[T, kv_heads, head_dim]`` to their slots; negative slots are padding, and a slot that
+    is given twice has no defined contents.  ``kv_cache``: in the type of ``k``,
     ``[blocks, 2, kv_heads, block_size, head_dim]``, or in 8 bits, ``uint8 [blocks, 2, kv_heads, block_size, head_dim + 4]``
     (:func:`reference.attention.kv8_rows` says what that holds; 4 more bytes a row for its scale)."""
     if kv_cache.dtype == torch.uint8:
