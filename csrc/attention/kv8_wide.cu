@@ -443,7 +443,7 @@ kv8_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
   }
 }
 
-// Keys (in T) and values (in fp16) of tile blockIdx.x (128 keys) of a request and head, as far as the call needs it.  Rows that were not
+// Keys (in T, even blockIdx.x) or values (in fp16, odd) of a tile of 128 keys of a request and head, as far as the call needs it.  Rows that were not
 // written, or whose block is outside the pool: zeros; a NaN stays one in the key and is a zero in the value, since a weight of zero would
 // not hide it.  A thread takes 16 codes of a row at a time.
 template <typename T, int D>
@@ -453,7 +453,7 @@ kv8_widen_kernel(T* __restrict__ k, __half* __restrict__ v, uint8_t* __restrict_
                  const int* __restrict__ qsl, int window) {
   griddep_launch();
   griddep_wait();
-  const int tile = blockIdx.x, h = blockIdx.y, req = blockIdx.z, key0 = tile * kTile;
+  const int tile = blockIdx.x >> 1, which = blockIdx.x & 1, h = blockIdx.y, req = blockIdx.z, key0 = tile * kTile;
   const int q_len = qsl[req + 1] - qsl[req], seq_len = seq_lens[req], ctx = seq_len - q_len;
   const int first = window > 0 ? max(0, ctx - window + 1) / kTile : 0;
   // a request whose rows see nothing has its first tile read all the same
@@ -465,43 +465,40 @@ kv8_widen_kernel(T* __restrict__ k, __half* __restrict__ v, uint8_t* __restrict_
     const int b = bi < max_blocks ? bt[bi] : -1;
     return b >= 0 && b < c.num_blocks ? b : -1;
   };
-  if (h == 0 && threadIdx.x < 32) {
+  if (h == 0 && which == 0 && threadIdx.x < 32) {
     const uint32_t bits = __ballot_sync(0xffffffffu, threadIdx.x < 8 && block_of(key0 + threadIdx.x * 16) >= 0);
     if (threadIdx.x == 0) valid[(int64_t)req * (rows / kTile) + tile] = (uint8_t)bits;
   }
   constexpr int kPer = D / 16, kSteps = kTile * kPer / 256;
   const int64_t out0 = (((int64_t)req * c.Hkv + h) * rows + key0) * D;
+  uint4 codes[kSteps];
+  float scale[kSteps];
 #pragma unroll
-  for (int which = 0; which < 2; ++which) {
-    uint4 codes[kSteps];
-    float scale[kSteps];
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-      const int x = i * 256 + threadIdx.x, key = key0 + x / kPer, b = block_of(key);
-      codes[i] = make_uint4(0, 0, 0, 0);
-      scale[i] = 0.f;
-      if (b >= 0) {
-        uint8_t* page = c.page(b, which, h);
-        const int off = key % c.block_size;
-        codes[i] = *reinterpret_cast<const uint4*>(c.codes(page, off) + x % kPer * 16);
-        scale[i] = *c.scale(page, off);
-      }
+  for (int i = 0; i < kSteps; ++i) {
+    const int x = i * 256 + threadIdx.x, key = key0 + x / kPer, b = block_of(key);
+    codes[i] = make_uint4(0, 0, 0, 0);
+    scale[i] = 0.f;
+    if (b >= 0) {
+      uint8_t* page = c.page(b, which, h);
+      const int off = key % c.block_size;
+      codes[i] = *reinterpret_cast<const uint4*>(c.codes(page, off) + x % kPer * 16);
+      scale[i] = *c.scale(page, off);
     }
+  }
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-      const int x = i * 256 + threadIdx.x;
-      const uint32_t in[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
-      const float f = which && is_nan_bits(scale[i]) ? 0.f : scale[i];
-      uint32_t y[8];
+  for (int i = 0; i < kSteps; ++i) {
+    const int x = i * 256 + threadIdx.x;
+    const uint32_t in[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
+    const float f = which && is_nan_bits(scale[i]) ? 0.f : scale[i];
+    uint32_t y[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float2 a = e4m3x2_to_float2((uint16_t)(in[j / 2] >> (16 * (j & 1))));
-        y[j] = which ? pack2<__half>(a.x * f, a.y * f) : pack2<T>(a.x * f, a.y * f);
-      }
-      uint4* dst = which ? reinterpret_cast<uint4*>(v + out0 + (int64_t)x * 16) : reinterpret_cast<uint4*>(k + out0 + (int64_t)x * 16);
-      dst[0] = make_uint4(y[0], y[1], y[2], y[3]);
-      dst[1] = make_uint4(y[4], y[5], y[6], y[7]);
+    for (int j = 0; j < 8; ++j) {
+      const float2 a = e4m3x2_to_float2((uint16_t)(in[j / 2] >> (16 * (j & 1))));
+      y[j] = which ? pack2<__half>(a.x * f, a.y * f) : pack2<T>(a.x * f, a.y * f);
     }
+    uint4* dst = which ? reinterpret_cast<uint4*>(v + out0 + (int64_t)x * 16) : reinterpret_cast<uint4*>(k + out0 + (int64_t)x * 16);
+    dst[0] = make_uint4(y[0], y[1], y[2], y[3]);
+    dst[1] = make_uint4(y[4], y[5], y[6], y[7]);
   }
 }
 
@@ -509,7 +506,7 @@ template <typename T, int D>
 static int launch_wide(const Params& p, const Scratch& w, const CUtensorMap& tmQ, const CUtensorMap& tmK, const CUtensorMap& tmV,
                        int64_t items, cudaStream_t st) {
   const Kv8Cache c{const_cast<uint8_t*>(p.cache), p.num_blocks, p.Hkv, p.block_size, D};
-  cudaError_t e = launch_pdl(kv8_widen_kernel<T, D>, dim3(w.rows / kTile, p.Hkv, p.B), dim3(256), 0, st, (T*)w.k, (__half*)w.v,
+  cudaError_t e = launch_pdl(kv8_widen_kernel<T, D>, dim3(2 * (w.rows / kTile), p.Hkv, p.B), dim3(256), 0, st, (T*)w.k, (__half*)w.v,
                              (uint8_t*)w.valid, w.rows, c, p.block_tables, p.bt_stride, p.max_blocks, p.seq_lens, p.qsl, p.window);
   if (e != cudaSuccess) return (int)e;
   auto kern = kv8_wide_kernel<T, D>;
