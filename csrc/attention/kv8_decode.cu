@@ -84,7 +84,7 @@ template <typename T, int D, int NR> struct Layout {
   static constexpr int kKeyGroups = G::kPack, kRowGroups = NR == 16 || (NR == 8 && G::kPack == 2) ? 2 : 1, kGroups = kKeyGroups * kRowGroups;
   static constexpr int kSoft = 128 * kGroups, kThreads = 64 + kSoft;
   static constexpr int kCtas = D == 256 || kGroups == 4 ? 1 : 2;        // an SM at most: shared memory, registers
-  static constexpr int kKeysOf = 1, kRowsOf = NR / kRowGroups;          // keys of a row and query rows of a thread
+  static constexpr int kRowsOf = NR / kRowGroups;                       // query rows of a thread
   static constexpr int kNO = G::kNS * P;                       // columns of an O^T accumulator
   static constexpr int kQ = P * G::kBlk * G::kNS * 128;        // queries
   static constexpr int kP = kNO * 128;                         // one weight buffer
@@ -114,6 +114,12 @@ __device__ __forceinline__ void tmem_st_x8(uint32_t taddr, const uint32_t (&r)[8
 __device__ __forceinline__ uint16_t f16x2_to_e4m3x2(__half2 v) {
   uint16_t r;
   asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(*reinterpret_cast<const uint32_t*>(&v)));
+  return r;
+}
+// 2^x, results below 2^-126 as zero, which is far below what a weight's pieces hold
+__device__ __forceinline__ float fast_exp2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
 __device__ __forceinline__ __half2 as_half2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
@@ -193,7 +199,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
   using G = Geo<D>;
   using L = Layout<T, D, NR>;
   constexpr int P = L::P, kPack = G::kPack, kBlk = G::kBlk, kKeys = G::kKeys, kNS = G::kNS, kNO = L::kNO, kSoft = L::kSoft, kWarps = kSoft / 32;
-  constexpr int kKeysOf = L::kKeysOf, kRowsOf = L::kRowsOf, kThreads = L::kThreads;
+  constexpr int kRowsOf = L::kRowsOf, kThreads = L::kThreads;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int ns = p.slots;
@@ -448,7 +454,9 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
     const int page_rows = p.block_size / kPack, box_rows = min(kM, page_rows & -page_rows);
     const uint32_t all_boxes = (1u << (kM / box_rows)) - 1;              // 16 boxes at most
     const int my_box = row_id / box_rows;
-    const int p_off = row_id & 15, p_ch = row_id >> 4;
+    // byte `row_id` of the thread's first row of P; 16-byte chunks are swizzled by the row's number, of which the thread's part is below 8
+    uint8_t* sW = sP + (key_of * kRows + row_of) * 128 + (row_id & 15);
+    const int p_ch = (row_id >> 4) ^ (row_of & 7);
 
     // ---- queries in pieces: 8 elements a thread and step, lanes of a row next to one another
     constexpr int kLanes = D / 8, kQSteps = (NR * kLanes + kSoft - 1) / kSoft;
@@ -527,9 +535,11 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
 #pragma unroll 1
     for (int item = 0; it.more(); ++item) {
       const int rows = r.q_len * g, pos_max = r.ctx + r.q_len - 1;
-      float m_used[kRowsOf], l_part[kRowsOf], vref = 0.f;
+      // weights are 2^(score + base), base = kLift - the reference maximum; rows of `unset` have seen no score yet
+      float base[kRowsOf], l_part[kRowsOf], vref = 0.f;
+      uint32_t unset = (1u << kRowsOf) - 1;
 #pragma unroll
-      for (int i = 0; i < kRowsOf; ++i) { m_used[i] = -INFINITY; l_part[i] = 0.f; }
+      for (int i = 0; i < kRowsOf; ++i) { base[i] = kLift; l_part[i] = 0.f; }
       const float* factor = sFactor + (item & 1) * kRows + row_of;
       const Walk cur = it;
       const Request rc = r;
@@ -539,6 +549,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
         q_load(it, r);                       // on their way while this item is worked on
       }
       const int tile_end = cur.tile + cur.count;
+      bool unset_any = true;
 #pragma unroll 1
       for (int i = cur.tile; ok && i < tile_end; ++i, ++t) {
         const int buf = t & 1;
@@ -553,16 +564,13 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
         slot += 2;
         if (slot >= ns) { slot -= ns; phase ^= 1; }
         tc_fence_after_sync();
-        uint32_t sr[kKeysOf][8];
-#pragma unroll
-        for (int q2 = 0; q2 < kKeysOf; ++q2) tmem_ld_x8(tS + buf * kNS + q2 * kRows, sr[q2]);
-        float kscale[kKeysOf], vscale[kKeysOf];
-#pragma unroll
-        for (int q2 = 0; q2 < kKeysOf; ++q2) {
-          kscale[q2] = sScale[kslot * kKeys + row_id * kPack + key_of + q2];
-          vscale[q2] = sScale[vslot * kKeys + row_id * kPack + key_of + q2];
-        }
+        uint32_t sr[8];
+        tmem_ld_x8(tS + buf * kNS, sr);
+        float kscale = sScale[kslot * kKeys + row_id * kPack + key_of], vscale = sScale[vslot * kKeys + row_id * kPack + key_of];
         const uint32_t valid = sValid[kslot];
+        float fac[kRowsOf];
+#pragma unroll
+        for (int n = 0; n < kRowsOf; n += 4) *reinterpret_cast<float4*>(fac + n) = *reinterpret_cast<const float4*>(factor + n);
         tmem_ld_wait();
         tc_fence_before_sync();
         __syncwarp();
@@ -574,53 +582,50 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
         const int key0 = rc.kv_begin + i * kKeys;
         const bool whole = key0 + kKeys <= rc.seq_len && (valid & all_boxes) == all_boxes;
         const bool full = whole && key0 + kKeys - 1 <= rc.ctx && (p.window <= 0 || key0 > pos_max - p.window);
-        float sc[kKeysOf][kRowsOf];
-        bool need = fail;
+        float y[kRowsOf];                    // log2 of the weights
+        bool need = fail || unset_any;
+        if (is_nan_bits(vscale)) {           // the row's key gives NaN to those who see it, then, and the value nothing to the others
+          kscale = vscale;
+          vscale = 0.f;
+        }
+        if (full) {
+          // rows behind the request's have queries of zeros and go along
 #pragma unroll
-        for (int q2 = 0; q2 < kKeysOf; ++q2) {
-          const int key = key0 + row_id * kPack + key_of + q2;
+          for (int n = 0; n < kRowsOf; ++n) y[n] = fmaf(__uint_as_float(sr[n]), kscale * fac[n], base[n]);
+        } else {
+          const int key = key0 + row_id * kPack + key_of;
           const bool there = whole || (key < rc.seq_len && (valid >> my_box & 1));
           if (!there) {
-            vscale[q2] = 0.f;
+            vscale = 0.f;
             // codes of rows that were not read, or not written, may be anything: zeros, since a weight of zero does not hide a NaN
             uint8_t* v = smem + vslot * G::kOp + row_id * 128;
 #pragma unroll
             for (int c = 0; c < 8 / kPack; ++c) {
 #pragma unroll
               for (int b = 0; b < kBlk; ++b)
-                *reinterpret_cast<uint4*>(v + b * (kM * 128) + (((kPack == 2 ? (key_of + q2) * 4 + c : c) ^ (row_id & 7)) << 4)) =
+                *reinterpret_cast<uint4*>(v + b * (kM * 128) + (((kPack == 2 ? key_of * 4 + c : c) ^ (row_id & 7)) << 4)) =
                     make_uint4(0, 0, 0, 0);
             }
           }
-          need |= vscale[q2] > vref;
 #pragma unroll
           for (int n = 0; n < kRowsOf; ++n) {
-            const int row = row_of + n;
-            float v = __uint_as_float(sr[q2][n]) * (kscale[q2] * factor[n]);
-            if (!full) {
-              const int pos = row < rows ? rc.ctx + (int)((row * inv_g) >> 16) : -1;
-              v = there && key <= pos && (p.window <= 0 || key > pos - p.window) ? v : -INFINITY;
-            } else if (NR > 4 && row >= rows) {
-              v = -INFINITY;
-            }
-            sc[q2][n] = v;
-            need |= v > m_used[n] + kSlack;
+            const int row = row_of + n, pos = row < rows ? rc.ctx + (int)((row * inv_g) >> 16) : -1;
+            const bool seen = there && key <= pos && (p.window <= 0 || key > pos - p.window);
+            y[n] = seen ? fmaf(__uint_as_float(sr[n]), kscale * fac[n], base[n]) : -INFINITY;
           }
         }
+        need |= vscale > vref;
+#pragma unroll
+        for (int n = 0; n < kRowsOf; ++n) need |= y[n] > kLift + kSlack;
         if (bar_red_or(1, kSoft, need)) {
           // ---- rare after the first tiles: move the reference maxima and the reference scale, rescale O^T
 #pragma unroll
           for (int n = 0; n < kRowsOf; ++n) {
-            const float wm = warp_max_redux(kKeysOf == 2 ? fmaxf(sc[0][n], sc[kKeysOf - 1][n]) : sc[0][n]);
+            const float wm = warp_max_redux(y[n]);
             if (lane == n) sMax[wi * 9 + n] = wm;
           }
-          {
-            float vm = 0.f;
-#pragma unroll
-            for (int q2 = 0; q2 < kKeysOf; ++q2) vm = fmaxf(vm, is_nan_bits(vscale[q2]) ? 0.f : vscale[q2]);
-            vm = warp_max_redux(vm);
-            if (lane == 8) sMax[wi * 9 + 8] = vm;
-          }
+          const float wv = warp_max_redux(vscale);
+          if (lane == 8) sMax[wi * 9 + 8] = wv;
           const bool warp_failed = __any_sync(0xffffffffu, fail);
           if (lane == 0) ok_slot[wi] = warp_failed ? 0 : 1;
           named_bar_sync(1, kSoft);
@@ -640,23 +645,26 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
             float top = fmaxf(fmaxf(mx[0], mx[9]), fmaxf(mx[18], mx[27]));
             if (L::kKeyGroups == 2) top = fmaxf(top, fmaxf(fmaxf(mx[36], mx[45]), fmaxf(mx[54], mx[63])));
             alpha[n] = 1.f;
-            if (top > m_used[n] + kSlack) {            // also the first finite maximum (m_used = -inf)
-              alpha[n] = exp2f(m_used[n] - top);       // exp2(-inf) = 0: nothing accumulated yet
-              m_used[n] = top;
+            const bool first = unset >> n & 1;
+            if (top > kLift + kSlack || (first && top > -INFINITY)) {
+              alpha[n] = first ? 0.f : exp2f(kLift - top);       // nothing was added yet
+              base[n] -= top - kLift;
+              y[n] -= top - kLift;
               l_part[n] *= alpha[n];
+              unset &= ~(1u << n);
               rescale = true;
             }
             alpha[n] *= back;
           }
+          unset_any = (unset & (rows - row_of >= kRowsOf ? ~0u : (1u << max(0, rows - row_of)) - 1)) != 0;
           // every group has its own columns; the waits of its threads agree because they read the same maxima
           if (rescale && i > cur.tile) {
             if (!wait_or_abort(o_done, (t - 1) & 1, ab, 908)) fail = true;
             __syncwarp();
             tc_fence_after_sync();
-            constexpr int kParts = kBlk * P * kKeysOf;
 #pragma unroll
-            for (int c = 0; c < kParts; ++c) {
-              const uint32_t at = tO + c / (P * kKeysOf) * kNO + (c / kKeysOf % P * kPack + c % kKeysOf) * kRows;
+            for (int c = 0; c < kBlk * P; ++c) {
+              const uint32_t at = tO + c / P * kNO + c % P * kPack * kRows;
               uint32_t o[8];
               tmem_ld_x8(at, o);
               tmem_ld_wait();
@@ -670,29 +678,20 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
         }
         const float to_ref = vref > 0.f ? pow2_inv(vref) : 0.f;
         if (!fail) {
-          uint8_t* wbuf = sP + buf * L::kP + p_off;
+          uint8_t* wbuf = sW + buf * L::kP;
+          const float vs = vscale * to_ref;
 #pragma unroll
-          for (int q2 = 0; q2 < kKeysOf; ++q2) {
-            const float vs = vscale[q2] * to_ref;
+          for (int n = 0; n < kRowsOf; n += 2) {
+            const float x0 = fast_exp2(y[n]), x1 = fast_exp2(y[n + 1]);
+            l_part[n] += x0;
+            l_part[n + 1] += x1;
+            __half2 rest = __floats2half2_rn(x0 * vs, x1 * vs);
 #pragma unroll
-            for (int n = 0; n < kRowsOf; n += 2) {
-              float w[2];
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const float m = m_used[n + e] == -INFINITY ? 0.f : m_used[n + e];
-                const float x = exp2f(sc[q2][n + e] - m + kLift);
-                l_part[n + e] += x;
-                w[e] = x > 0.f ? x * vs : x;         // a masked key's scale may be a NaN
-              }
-              __half2 rest = __floats2half2_rn(w[0], w[1]);
-#pragma unroll
-              for (int c = 0; c < P; ++c) {
-                const uint16_t code = f16x2_to_e4m3x2(rest);
-                const int rr = (c * kPack + key_of + q2) * kRows + row_of + n;
-                wbuf[rr * 128 + ((p_ch ^ (rr & 7)) << 4)] = (uint8_t)code;
-                wbuf[(rr + 1) * 128 + ((p_ch ^ ((rr + 1) & 7)) << 4)] = (uint8_t)(code >> 8);
-                if (c + 1 < P) rest = __hmul2(__hsub2(rest, as_half2(e4m3x2_to_f16x2(code))), __float2half2_rn(32.f));
-              }
+            for (int c = 0; c < P; ++c) {
+              const uint16_t code = f16x2_to_e4m3x2(rest);
+              wbuf[(c * kPack * kRows + n) * 128 + ((p_ch ^ n) << 4)] = (uint8_t)code;
+              wbuf[(c * kPack * kRows + n + 1) * 128 + ((p_ch ^ (n + 1)) << 4)] = (uint8_t)(code >> 8);
+              if (c + 1 < P) rest = __hmul2(__hsub2(rest, as_half2(e4m3x2_to_f16x2(code))), __float2half2_rn(32.f));
             }
           }
         }
@@ -713,7 +712,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
         for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
         if (lane == n) {
           sSum[wi * 8 + n] = v;
-          sMax[wi * 9 + n] = m_used[n];
+          sMax[wi * 9 + n] = base[n];
         }
       }
       const int first = sPre[cur.req] * p.Hkv + cur.head * cur.n;
@@ -729,13 +728,13 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
         float sum = 0.f;
 #pragma unroll
         for (int w = 0; w < 4 * L::kKeyGroups; ++w) sum += sSum[(w0 + w) * 8 + n];
-        const float m = sMax[w0 * 9 + n], ms = m == -INFINITY ? 0.f : m;
+        const float lift = sMax[w0 * 9 + n];
         float den = sum;
         if (!partial && p.sinks != nullptr && tid < rows)
-          den += exp2f(p.sinks[cur.head * g + ((int)tid - (int)((tid * inv_g) >> 16) * g)] * kLog2e - ms + kLift);
+          den += exp2f(p.sinks[cur.head * g + ((int)tid - (int)((tid * inv_g) >> 16) * g)] * kLog2e + lift);
         // vref comes with the weights' scale; a row that saw nothing gives zeros, a NaN stays one
         sInv[tid] = !ok || den == 0.f ? 0.f : vref / den;
-        if (partial) p.ws_lse[my_slot * kRows + tid] = !ok || sum == 0.f ? -INFINITY : ms + log2f(sum) - kLift;
+        if (partial) p.ws_lse[my_slot * kRows + tid] = !ok || sum == 0.f ? -INFINITY : log2f(sum) - lift;
       }
       named_bar_sync(1, kSoft);
       // this thread's output dims of its rows: pieces summed; heads of 64: even keys' in lanes 0 .. 63, odd ones' behind
