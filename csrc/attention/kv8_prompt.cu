@@ -10,6 +10,8 @@
 // buffer and the tensor core's.  Every stored value is an exact fp16 number (common/kv8.cuh): its scale is gone then, and P rounds to 11 bits.
 // What bounds it: per tile the tensor core needs 1024 cycles, the special-function units as many (128 x 128 exponentials at 16 a cycle),
 // shared memory a little more for two tiles than both (1216 a tile: operands, TMA, widening, scales).
+// Measured, us, beside the kernel that widens first (kv8_wide.cu), 32 / 8 heads of 128: 17 new tokens (one tile) behind 16000: 37 and 52; 60 (two): 52
+// and 63; 128 (four): 95 and 91; 300 (ten): 313 and 233; 12 x 30 tokens without context: 12 and 16.  So it takes up to two tiles.
 //
 // A row is (token, head of a group): a tile holds 128 / g tokens of all g heads of one key / value head, so that a few new tokens fill it,
 // and K and V are read and converted once for the group.  A persistent CTA works on two tiles ("streams") of consecutive tokens that read

@@ -11,6 +11,8 @@
 // so there is one stream with two S buffers of N = 64 keys; S(i + 2) is issued behind P.V(i), the softmax of tile i + 1 meanwhile.
 // What bounds it: per 128 keys and tile the tensor core needs 1024 cycles (2048 with heads of 256), the special-function units 1024.
 // Widening reads D + 4 and writes 2 D bytes a row; what it writes mostly stays in L2.
+// Measured, bf16, 32 / 8 heads of 128: 4 prompts of 2048 tokens 180 us (137 GFLOP of visible scores and values: 760 TFLOP/s); 4096 tokens behind 28672
+// 1.83 ms (2.06 TFLOP: 1120 TFLOP/s, 0.69 of what a library product reaches).  Widening inside for every pair of tiles: 239 us and 2.87 ms.
 // Warp 0 TMA producer, warp 1 MMA issuer, warps 4-7 and 8-11 softmax and epilogue (thread = row).  The grid has a CTA per item, in descending
 // order of row blocks; a CTA that is done takes the next pending one's item (cluster launch control).  Every wait is bounded; on time-out the
 // status word is set and the CTA unwinds.

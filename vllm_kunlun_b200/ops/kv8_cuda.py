@@ -43,7 +43,9 @@ def _attend(out, q, kv_cache, block_tables, seq_lens, query_start_loc, scale, ma
                                 window, scale, stable_metadata)
             return
         if D in (64, 128, 256) and group <= 128 and scale > 0:
-            # widened once for all query tiles where more than one pair of them (128 // group tokens each) reads the same keys
+            # widened once for all query tiles where more than one pair of them (128 // group tokens each) reads the same keys.
+            # us widened inside and first, 32 / 8 heads of 128 behind 16000 tokens: one tile 37 / 52, two 52 / 63, four 95 / 91,
+            # ten 313 / 233.  Heads of 256 have no kernel that widens inside.
             wide = D == 256 or max_query_len > 2 * (128 // group)
             _ext.C().kv8_prompt(out, q, kv_cache, block_tables, seq_lens, query_start_loc, sinks, max_query_len, max_seq_len, window,
                                 scale, wide)
