@@ -399,6 +399,14 @@ def test_windows_of_prompts(D, new, window):
 
 
 @gpu
+@pytest.mark.parametrize("new", [1, 30, 300])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 + 5, 2 ** 40])
+def test_windows_wider_than_any_length(new, window):
+    b = batch([new, 2], [300, 7], 4, 2, 128, 64, torch.bfloat16, "cuda")
+    assert torch.equal(attend(b, window), attend(b))
+
+
+@gpu
 @pytest.mark.parametrize("new", [1, 9])
 def test_more_requests_than_a_launch_takes(new):
     """4100 requests are three launches of 2048 at most, each with items that are cut."""

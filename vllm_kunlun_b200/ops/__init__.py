@@ -257,8 +257,8 @@ def paged_attention(q, kv_cache, block_tables, seq_lens, query_start_loc, scale:
                                            sinks)
         from .kv8_cuda import paged_attention_kv8
         return paged_attention_kv8(out, q, kv_cache, block_tables, seq_lens, query_start_loc, scale, max_query_len, max_seq_len,
-                                   window or 0, sinks, workspace, num_decodes, decode_query_len, num_decode_tokens,
-                                   stable_metadata)
+                                   min(window or 0, 1 << 30), sinks, workspace, num_decodes, decode_query_len, num_decode_tokens,
+                                   stable_metadata)    # a wider window hides nothing: lengths are below that
     if q.is_cuda:
         if out is None:
             out = torch.empty(q.shape[0], q.shape[1], kv_cache.shape[-1], dtype=q.dtype, device=q.device)
