@@ -109,10 +109,18 @@ __device__ __forceinline__ float warp_max_redux(float v) {
   i = i >= 0 ? i : i ^ 0x7fffffff;
   return __int_as_float(i);
 }
-__device__ __forceinline__ void tmem_st_x8(uint32_t taddr, const uint32_t (&r)[8]) {
+// The columns of a thread's rows and no others: the columns next to them are another group's, which may be writing them.
+__device__ __forceinline__ void tmem_ld_rows(uint32_t taddr, uint32_t (&r)[8]) { tmem_ld_x8(taddr, r); }
+__device__ __forceinline__ void tmem_ld_rows(uint32_t taddr, uint32_t (&r)[4]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_st_rows(uint32_t taddr, const uint32_t (&r)[8]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
                "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                : "memory");
+}
+__device__ __forceinline__ void tmem_st_rows(uint32_t taddr, const uint32_t (&r)[4]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
 }
 __device__ __forceinline__ uint16_t f16x2_to_e4m3x2(__half2 v) {
   uint16_t r;
@@ -567,8 +575,8 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
         slot += 2;
         if (slot >= ns) { slot -= ns; phase ^= 1; }
         tc_fence_after_sync();
-        uint32_t sr[8];
-        tmem_ld_x8(tS + buf * kNS, sr);
+        uint32_t sr[kRowsOf];
+        tmem_ld_rows(tS + buf * kNS, sr);
         float kscale = sScale[kslot * kKeys + row_id * kPack + key_of], vscale = sScale[vslot * kKeys + row_id * kPack + key_of];
         const uint32_t valid = sValid[kslot];
         float fac[kRowsOf];
@@ -668,12 +676,12 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
 #pragma unroll
             for (int c = 0; c < kBlk * P; ++c) {
               const uint32_t at = tO + c / P * kNO + c % P * kPack * kRows;
-              uint32_t o[8];
-              tmem_ld_x8(at, o);
+              uint32_t o[kRowsOf];
+              tmem_ld_rows(at, o);
               tmem_ld_wait();
 #pragma unroll
               for (int n = 0; n < kRowsOf; ++n) o[n] = __float_as_uint(__uint_as_float(o[n]) * alpha[n]);
-              tmem_st_x8(at, o);
+              tmem_st_rows(at, o);
             }
             tmem_st_wait();
           }
@@ -752,8 +760,8 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
 #pragma unroll
         for (int c = 0; c < P; ++c) {
           const uint32_t at = tO + b * kNO + (c * kPack + (kBoth ? row_id >> 6 : 0)) * kRows;
-          uint32_t o[8];
-          tmem_ld_x8(at, o);
+          uint32_t o[kRowsOf];
+          tmem_ld_rows(at, o);
           tmem_ld_wait();
           const float unit = c == 0 ? 1.f : c == 1 ? 1.f / 32.f : 1.f / 1024.f;
 #pragma unroll

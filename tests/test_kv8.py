@@ -450,6 +450,25 @@ def test_queries_that_are_not_numbers(D, dt, new, context):
 
 
 @gpu
+@pytest.mark.parametrize("D,group", [(64, 2), (64, 5), (64, 8), (64, 16), (128, 4), (128, 8), (128, 13), (256, 3), (256, 8), (256, 16)])
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+def test_maxima_that_keep_moving(D, group, dt):
+    """Keys that grow tile by tile: every tile rescales what the ones in front of it left, for all rows of a head at once."""
+    lens = [900 + 61 * i for i in range(24)]
+    b = batch([1] * 24, [n - 1 for n in lens], 2 * group, 2, D, 64, DT[dt], "cpu", seed=group)
+    scales = ra.kv8_views(b["cache"])[1]
+    for r, n in enumerate(lens):
+        j = torch.arange(n)
+        scales[b["table"][r].long()[j // 64], 0, :, j % 64] *= torch.exp2((j // 256).float())[:, None]
+    for name in ("q", "cache", "table", "lens", "qsl"):
+        b[name] = b[name].cuda()
+    first = attend(b)
+    check(first, b)
+    for _ in range(20):
+        assert torch.equal(attend(b), first)
+
+
+@gpu
 def test_items_around_the_cuts():
     """One to many tiles a request and every number of requests up to 40: cuts on, next to and far from the ends of items."""
     for n in (1, 2, 3, 7, 19, 40):
