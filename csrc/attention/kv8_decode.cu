@@ -6,9 +6,14 @@
 //   * Queries: q times a power of two that puts the row's largest element in (128, 256] is the sum of e4m3 pieces, each the rounded rest
 //     of those in front of it.  A piece has four significant bits and rests are signed, so two pieces hold the 8 bits of bf16 and three the
 //     11 of fp16 exactly, down to 2^-18 of the row's largest element.  All pieces add into one accumulator.
-//   * Weights: exp2(s - m) * 2^3 * v_scale / (largest v_scale so far) <= 2^8, in fp16 and then in the same pieces, each rest times 2^5 so that
-//     weights far below the largest keep their digits; every piece has accumulator columns of its own.  Two pieces are off by less
-//     than 2^-8 (the rounding of a bf16 weight) and by 2^-18 of the largest, three carry the 11 bits of fp16 and are off by 2^-23 of it.
+//   * Weights: exp2(s - m) * 2^lift * v_scale / (largest v_scale so far), in fp16 and then in three pieces; each rest is multiplied up so that
+//     weights far below the largest keep their digits, and every piece has accumulator columns of its own.  The many keys behind one that
+//     holds most of a row count together however little each weighs, so the range matters as much as the digits.  bf16: e5m2 pieces, rests
+//     times 2^3, weights up to 2^15: off by 2^-9, and by half the last piece's smallest step, 2^-30 of the largest.  fp16: e4m3 pieces, rests
+//     times 2^5, weights up to 2^8: 2^-12, and 2^-25 of the largest, the smallest step of the prompt kernels' fp16 weights.  Two e4m3
+//     pieces for bf16 (off by 2^-8, and by 2^-18 of the largest: 32768 keys just below that, 12 % of a row, count as nothing) are no faster:
+//     16 x 4096 tokens of 32 / 8 heads of 128 33.9 us, with three pieces 34.1; 48 ragged requests 62.4 and 62.7; 64 requests of two tokens
+//     behind 4095, 64 / 8 heads of 64, 215 and 213.
 // Few query rows and many keys: keys are the UMMA M side, query rows the N side.
 //     S^T[128 rows, 16]        = K[128 rows, 128 B] . Q^T      per piece, K-major as cached
 //     O^T[128 dims, 16 pieces] += V^T[128 dims, 128 rows] . P   V MN-major as cached
@@ -43,9 +48,6 @@ namespace kv8dec {
 constexpr int kM = 128;          // rows of 128 bytes in a tile
 constexpr int kRows = 16;        // query rows, zero padded
 constexpr int kMaxB = 2048;      // requests a launch
-// The running maximum moves when a score exceeds it by more than kSlack (log2): weights stay below 2^(kLift + kSlack).  With 7 and 1 every item
-// moved it several times.
-constexpr float kSlack = 5.f, kLift = 3.f;
 // A cut this close to an item's end moves there (tiles; CTAs of one tile keep theirs): one tile costs less than a merge of 16 rows.  us without
 // and with, 12 requests of 600 tokens, 8 heads of 128: 16 rows 26.5 and 21.8, 8 rows 18.1 and 15.7, 4 rows 14.3 and 13.1; of 2000: 37.6 and 38.0.
 constexpr int kSnap = 1;
@@ -75,20 +77,30 @@ template <int D> struct Geo {
   static constexpr int kOp = kBlk * kM * 128;          // codes of K or V of a tile
   static constexpr int kNS = kRows * kPack;            // columns of S^T
 };
+// Pieces of a query (q) and of a weight (w; the rest times kStep from one to the next).  The running maximum moves when a score exceeds it by
+// more than kSlack (log2): weights stay below 2^(kLift + kSlack).
 template <typename T> struct Pieces;
-template <> struct Pieces<__nv_bfloat16> { static constexpr int n = 2; };
-template <> struct Pieces<__half> { static constexpr int n = 3; };
+template <> struct Pieces<__nv_bfloat16> {
+  static constexpr int q = 2, w = 3;
+  static constexpr bool kE5 = true;
+  static constexpr float kStep = 8.f, kLift = 7.f, kSlack = 8.f;
+};
+template <> struct Pieces<__half> {
+  static constexpr int q = 3, w = 3;
+  static constexpr bool kE5 = false;
+  static constexpr float kStep = 32.f, kLift = 5.f, kSlack = 3.f;
+};
 
 template <typename T, int D, int NR> struct Layout {
   using G = Geo<D>;
-  static constexpr int P = Pieces<T>::n;
+  static constexpr int P = Pieces<T>::q, W = Pieces<T>::w;
   // Groups of four softmax warps: heads of 64 a group for the even and one for the odd keys; 16 query rows in halves, and 8 where keys are
   // halved already.  us with 8 rows in one group and in two, 16 requests of 4096 tokens: heads of 128 30.0 and 31.0, heads of 64 54.0 and 46.7.
   static constexpr int kKeyGroups = G::kPack, kRowGroups = NR == 16 || (NR == 8 && G::kPack == 2) ? 2 : 1, kGroups = kKeyGroups * kRowGroups;
   static constexpr int kSoft = 128 * kGroups, kThreads = 64 + kSoft;
   static constexpr int kCtas = D == 256 || kGroups == 4 ? 1 : 2;        // an SM at most: shared memory, registers
   static constexpr int kRowsOf = NR / kRowGroups;                       // query rows of a thread
-  static constexpr int kNO = G::kNS * P;                       // columns of an O^T accumulator
+  static constexpr int kNO = G::kNS * W;                       // columns of an O^T accumulator
   static constexpr int kQ = P * G::kBlk * G::kNS * 128;        // queries
   static constexpr int kP = kNO * 128;                         // one weight buffer
   static constexpr int kCols = 2 * G::kNS + G::kBlk * kNO;
@@ -127,6 +139,13 @@ __device__ __forceinline__ uint16_t f16x2_to_e4m3x2(__half2 v) {
   asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(*reinterpret_cast<const uint32_t*>(&v)));
   return r;
 }
+__device__ __forceinline__ uint16_t f16x2_to_e5m2x2(__half2 v) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e5m2x2.f16x2 %0, %1;" : "=h"(r) : "r"(*reinterpret_cast<const uint32_t*>(&v)));
+  return r;
+}
+// an e5m2 number is the upper byte of the same fp16 number
+__device__ __forceinline__ uint32_t e5m2x2_to_f16x2(uint16_t v) { return __byte_perm(v, 0, 0x1404); }
 // 2^x, results below 2^-126 as zero, which is far below what a weight's pieces hold
 __device__ __forceinline__ float fast_exp2(float x) {
   float r;
@@ -209,8 +228,10 @@ __global__ void __launch_bounds__((Layout<T, D, NR>::kThreads), (Layout<T, D, NR
 kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ Params p) {
   using G = Geo<D>;
   using L = Layout<T, D, NR>;
-  constexpr int P = L::P, kPack = G::kPack, kBlk = G::kBlk, kKeys = G::kKeys, kNS = G::kNS, kNO = L::kNO, kSoft = L::kSoft, kWarps = kSoft / 32;
+  constexpr int P = L::P, W = L::W, kPack = G::kPack, kBlk = G::kBlk, kKeys = G::kKeys, kNS = G::kNS, kNO = L::kNO, kSoft = L::kSoft, kWarps = kSoft / 32;
   constexpr int kRowsOf = L::kRowsOf, kThreads = L::kThreads;
+  using Pc = Pieces<T>;
+  constexpr float kLift = Pc::kLift, kSlack = Pc::kSlack;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int ns = p.slots;
@@ -381,7 +402,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
     // ------------------------------------------------------------------ MMA issuer
     if (elect_one() && n_tiles > 0) {
       constexpr uint32_t idesc_s = umma_idesc(kM, kNS, 0, 0, 0, 0);     // A = K (K-major), B = Q^T (K-major)
-      constexpr uint32_t idesc_o = umma_idesc(kM, kNO, 0, 0, 1, 0);     // A = V (MN-major), B = P (K-major)
+      constexpr uint32_t idesc_o = umma_idesc(kM, kNO, 0, Pc::kE5 ? 1 : 0, 1, 0);     // A = V (e4m3, MN-major), B = P (K-major)
       const uint32_t tS = tmem_base, tO = tmem_base + 2 * kNS;
       const uint32_t q_addr = smem_u32(sQ), p_addr = smem_u32(sP), kv_addr = smem_u32(smem);
       // S of the next tile and P.V of the current one are independent: whichever is ready is issued
@@ -674,8 +695,8 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
             __syncwarp();
             tc_fence_after_sync();
 #pragma unroll
-            for (int c = 0; c < kBlk * P; ++c) {
-              const uint32_t at = tO + c / P * kNO + c % P * kPack * kRows;
+            for (int c = 0; c < kBlk * W; ++c) {
+              const uint32_t at = tO + c / W * kNO + c % W * kPack * kRows;
               uint32_t o[kRowsOf];
               tmem_ld_rows(at, o);
               tmem_ld_wait();
@@ -698,11 +719,14 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
             l_part[n + 1] += x1;
             __half2 rest = __floats2half2_rn(x0 * vs, x1 * vs);
 #pragma unroll
-            for (int c = 0; c < P; ++c) {
-              const uint16_t code = f16x2_to_e4m3x2(rest);
+            for (int c = 0; c < W; ++c) {
+              const uint16_t code = Pc::kE5 ? f16x2_to_e5m2x2(rest) : f16x2_to_e4m3x2(rest);
               wbuf[(c * kPack * kRows + n) * 128 + ((p_ch ^ n) << 4)] = (uint8_t)code;
               wbuf[(c * kPack * kRows + n + 1) * 128 + ((p_ch ^ (n + 1)) << 4)] = (uint8_t)(code >> 8);
-              if (c + 1 < P) rest = __hmul2(__hsub2(rest, as_half2(e4m3x2_to_f16x2(code))), __float2half2_rn(32.f));
+              if (c + 1 < W) {
+                const uint32_t wide = Pc::kE5 ? e5m2x2_to_f16x2(code) : e4m3x2_to_f16x2(code);
+                rest = __hmul2(__hsub2(rest, as_half2(wide)), __float2half2_rn(Pc::kStep));
+              }
             }
           }
         }
@@ -758,12 +782,12 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
         for (int n = 0; n < kRowsOf; ++n) o_mine[b][n] = 0.f;
         if (!ok) continue;
 #pragma unroll
-        for (int c = 0; c < P; ++c) {
+        for (int c = 0; c < W; ++c) {
           const uint32_t at = tO + b * kNO + (c * kPack + (kBoth ? row_id >> 6 : 0)) * kRows;
           uint32_t o[kRowsOf];
           tmem_ld_rows(at, o);
           tmem_ld_wait();
-          const float unit = c == 0 ? 1.f : c == 1 ? 1.f / 32.f : 1.f / 1024.f;
+          const float unit = c == 0 ? 1.f : c == 1 ? 1.f / Pc::kStep : 1.f / (Pc::kStep * Pc::kStep);
 #pragma unroll
           for (int n = 0; n < kRowsOf; ++n) o_mine[b][n] += __uint_as_float(o[n]) * unit;
         }

@@ -1,0 +1,125 @@
+"""Decode attention over the 8-bit cache where weights and values of a row lie far apart, against 64-bit results.
+
+Limits.  With p the softmax weights, s a value row's scale and c its codes, an output may be off by
+
+* the score's error (fp32 sums of D products; queries in e4m3 pieces whose last step is 2^-18 of the row's largest element), which
+  multiplies weights by at most ``1 + 2 * off``,
+* the rounding of a weight: 2^-8 of it for bf16 queries (three e5m2 pieces take 2^-9, the fp16 number in front of them 2^-11), 2^-11 + 2^-12
+  of it for fp16 (an fp16 number and three e4m3 pieces),
+* for weights that are tiny beside the row's largest, half a step of the last piece: no more than ``FLOOR`` times the largest ``p * s`` (or the
+  largest ``p`` times the largest ``s``, see ``spread``) per key, times that key's codes,
+* and one rounding at the end, half a unit of the type.
+"""
+import math
+
+import pytest
+import torch
+
+from vllm_kunlun_b200 import ops
+from vllm_kunlun_b200.ops.reference import attention as ra
+
+pytestmark = pytest.mark.gpu
+DT = {"bf16": torch.bfloat16, "fp16": torch.float16}
+UNIT = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+ROUND = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11 + 2.0 ** -12}
+FLOOR = 2.0 ** -25
+BLOCK = 64
+
+
+def pool(k, v):
+    """An 8-bit cache of whole blocks holding ``k, v [n, heads, D]`` in the order of ``table``, and that table."""
+    n, H, D = k.shape
+    blocks = -(-n // BLOCK)
+    table = torch.randperm(blocks, generator=torch.Generator().manual_seed(n)).cuda()
+    cache = torch.zeros(blocks, 2, H, BLOCK, D + 4, dtype=torch.uint8, device="cuda")
+    codes, scales = ra.kv8_views(cache)
+    c, s = ra.kv8_rows(k, v)
+    pad = blocks * BLOCK - n
+    c = torch.nn.functional.pad(c.view(torch.uint8), (0, 0, 0, 0, 0, 0, 0, pad)).view(blocks, BLOCK, 2, H, D).permute(0, 2, 3, 1, 4)
+    s = torch.nn.functional.pad(s, (0, 0, 0, 0, 0, pad)).view(blocks, BLOCK, 2, H).permute(0, 2, 3, 1)
+    codes.view(torch.uint8)[table] = c
+    scales[table] = s
+    return cache, table.int()[None]
+
+
+def stored(k, v):
+    """Codes and scales as the cache holds them, in 64 bits: ``(ck, sk, cv, sv)``, ``[n, heads, D]`` and ``[n, heads, 1]``."""
+    c, s = ra.kv8_rows(k, v)
+    return c[:, 0].double(), s[:, 0, :, None].double(), c[:, 1].double(), s[:, 1, :, None].double()
+
+
+def results(q, k, v, window=0, spread=False):
+    """What the last ``len(q)`` tokens' queries give, the weights, and how far a result may be off; ``[new, H, D]``, ``[H, new, n]``.
+    ``spread``: weights share one reference for values of all scales, otherwise a small ``p`` of a large value has its digits too."""
+    ck, sk, cv, sv = stored(k, v)
+    g, n, D = q.shape[1] // k.shape[1], len(k), q.shape[2]
+    kk, vv, cc, ss = (x.repeat_interleave(g, 1) for x in (ck * sk, cv * sv, cv, sv))
+    x, scale = q.double(), D ** -0.5
+    pos = torch.arange(n - len(q), n, device="cuda")[:, None]
+    j = torch.arange(n, device="cuda")
+    seen = j <= pos
+    if window:
+        seen &= j > pos - window
+    s = (torch.einsum("ihd,jhd->hij", x, kk) * scale).masked_fill(~seen, -math.inf)
+    mag = torch.einsum("ihd,jhd->hij", x.abs(), kk.abs()) * scale
+    off = (D + 8) * 2.0 ** -24 * mag + 2.0 ** -18 * x.abs().amax(-1).T[:, :, None] * kk.abs().sum(-1).T[:, None] * scale
+    off = torch.where(seen, off, 0.0).amax(2).T[..., None]
+    p = torch.softmax(s, 2)
+    out = torch.einsum("hij,jhd->ihd", p, vv)
+    lim = torch.einsum("hij,jhd->ihd", p, vv.abs()) * (ROUND[q.dtype] + 2 * off + 2.0 ** -17)
+    s_seen = torch.where(seen[None], ss[:, :, 0].T[:, None], 0.0)                 # [H, new, n]
+    top = p.amax(2) * s_seen.amax(2) if spread else (p * s_seen).amax(2)
+    lim += FLOOR * top.T[..., None] * torch.einsum("ij,jhd->ihd", seen.double(), cc.abs())
+    return out, p, lim
+
+
+def attend(q, k, v, window=0, requests=1):
+    """``[requests, new, H, D]``: so many requests of the same tokens, over the same blocks."""
+    cache, table = pool(k, v)
+    n, new = len(k), len(q)
+    lens = torch.full((requests,), n, dtype=torch.int32, device="cuda")
+    qsl = torch.arange(requests + 1, device="cuda").int() * new
+    out = ops.paged_attention(q.repeat(requests, 1, 1), cache, table.repeat(requests, 1), lens, qsl, q.shape[2] ** -0.5, new, n,
+                              window or None)
+    return out.double().unflatten(0, (requests, new))
+
+
+def compare(got, want, lim, dt):
+    """Element by element, and every row as a whole to 2^-7: two roundings to bf16."""
+    d = (got - want).abs()
+    over = (d - lim - UNIT[dt] * want.abs() * 1.001 - (2.0 ** -25 if dt == torch.float16 else 0)).amax()
+    rows = d.norm(dim=-1) / want.norm(dim=-1)
+    assert float(rows.max()) <= 2.0 ** -7, f"a row is off by {float(rows.max()):.2%}"
+    assert float(over) <= 0, f"{float(over)} over"
+
+
+def rows_of(n, new, H, Hkv, D, dt, seed):
+    """Queries, keys and values with components in common, so that sums over many keys do not cancel."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    q = torch.randn(new, H, D, generator=g, device="cuda")
+    k = torch.randn(n, Hkv, D, generator=g, device="cuda")
+    v = 1 + 0.5 * torch.randn(n, Hkv, D, generator=g, device="cuda")
+    return q.to(dt), k, v
+
+
+@pytest.mark.parametrize("n,share", [(4096, 0.95), (8192, 0.8), (8192, 0.95), (8192, 0.99), (16384, 0.9), (32768, 0.8), (32768, 0.9),
+                                     (32768, 0.97)])
+@pytest.mark.parametrize("D,group", [(64, 4), (64, 16), (128, 4), (128, 8), (128, 16), (256, 4), (256, 8)])
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+@pytest.mark.parametrize("size", [0.05, 1.0])
+def test_a_key_that_holds_most_of_a_row(n, share, D, group, dt, size):
+    """The first key has ``share`` of every row's weight and a value of ``size``: the others, each tiny beside it, keep their part, in a
+    row that is cut into many pieces (one request) and in rows that are not (many)."""
+    q, k, v = rows_of(n, 1, group, 1, D, DT[dt], n + group)
+    k[:, :, 0] = 0
+    k[0] = 0
+    k[0, 0, 0] = 16.0                        # a power of two: its code is exact
+    v[0] *= size
+    ck, sk, _, _ = stored(k, v)
+    s = torch.einsum("hd,jd->hj", q[0].double(), (ck * sk)[1:, 0]) * D ** -0.5
+    # the first element of a query meets the first key alone
+    q[0, :, 0] = ((torch.logsumexp(s, 1) + math.log(share / (1 - share))) / (16.0 * D ** -0.5)).to(q.dtype)
+    want, p, lim = results(q, k, v)
+    assert (p[:, 0, 0] - share).abs().max() < 0.03
+    for requests in (1, 300):
+        compare(attend(q, k, v, requests=requests), want, lim, q.dtype)
