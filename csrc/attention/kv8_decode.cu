@@ -6,8 +6,9 @@
 //   * Queries: q times a power of two that puts the row's largest element in (128, 256] is the sum of e4m3 pieces, each the rounded rest
 //     of those in front of it.  A piece has four significant bits and rests are signed, so two pieces hold the 8 bits of bf16 and three the
 //     11 of fp16 exactly, down to 2^-18 of the row's largest element.  All pieces add into one accumulator.
-//   * Weights: exp2(s - m) * 2^lift * v_scale / (largest v_scale so far), in fp16 and then in three pieces; each rest is multiplied up so that
-//     weights far below the largest keep their digits, and every piece has accumulator columns of its own.  The many keys behind one that
+//   * Weights: exp2(s - m) * v_scale * 2^lift, m the largest s + log2(v_scale) that the row has seen, so that neither a heavy key with a small
+//     value nor a light or hidden one with a large value takes the others' digits.  In fp16 and then in three pieces; each rest is multiplied
+//     up so that weights far below the largest keep theirs, and every piece has accumulator columns of its own.  The many keys behind one that
 //     holds most of a row count together however little each weighs, so the range matters as much as the digits.  bf16: e5m2 pieces, rests
 //     times 2^3, weights up to 2^15: off by 2^-9, and by half the last piece's smallest step, 2^-30 of the largest.  fp16: e4m3 pieces, rests
 //     times 2^5, weights up to 2^8: 2^-12, and 2^-25 of the largest, the smallest step of the prompt kernels' fp16 weights.  Two e4m3
@@ -255,8 +256,8 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
   uint32_t* sValid = tmem_slot + 20;                         // [16] boxes of a K slot that were read
   uint32_t* sOdd = sValid + 16;                              // [16] heads of 64: 1 + the row of a K slot whose second key is behind the end
   float* sFactor = reinterpret_cast<float*>(sOdd + 16);      // [2 items][16]
-  float* sMax = sFactor + 2 * kRows;                         // [16 warps][9] maxima of a group's rows, largest v_scale
-  float* sSum = sMax + 16 * 9;                               // [16][8]
+  float* sMax = sFactor + 2 * kRows;                         // [16 warps][8] maxima of a group's rows
+  float* sSum = sMax + 16 * 8;                               // [16][8]
   float* sInv = sSum + 16 * 8;                               // [16]
   int* sScan = reinterpret_cast<int*>(sInv + kRows);         // [18]
   int* sPend = sScan + 20;                                   // [2][8] the CTA's cut items: ticket, its CTAs, rows, output
@@ -567,8 +568,8 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
 #pragma unroll 1
     for (int item = 0; it.more(); ++item) {
       const int rows = r.q_len * g, pos_max = r.ctx + r.q_len - 1;
-      // weights are 2^(score + base), base = kLift - the reference maximum; rows of `unset` have seen no score yet
-      float base[kRowsOf], l_part[kRowsOf], vref = 0.f;
+      // weights are 2^(score + base) * v_scale, base = kLift - the reference maximum; rows of `unset` have seen no score yet
+      float base[kRowsOf], l_part[kRowsOf];
       uint32_t unset = (1u << kRowsOf) - 1;
 #pragma unroll
       for (int i = 0; i < kRowsOf; ++i) { base[i] = kLift; l_part[i] = 0.f; }
@@ -614,7 +615,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
         const int key0 = rc.kv_begin + i * kKeys;
         const bool whole = key0 + kKeys <= rc.seq_len && (valid & all_boxes) == all_boxes;
         const bool full = whole && key0 + kKeys - 1 <= rc.ctx && (p.window <= 0 || key0 > pos_max - p.window);
-        float y[kRowsOf];                    // log2 of the weights
+        float y[kRowsOf];                    // log2 of the weights without the values' scale
         bool need = fail || unset_any;
         if (is_nan_bits(vscale)) {           // the row's key gives NaN to those who see it, then, and the value nothing to the others
           kscale = vscale;
@@ -646,36 +647,32 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
             y[n] = seen ? fmaf(__uint_as_float(sr[n]), kscale * fac[n], base[n]) : -INFINITY;
           }
         }
-        need |= vscale > vref;
+        // log2 of the scale, a power of two; 2^-15 is the smallest that is written
+        const float lv = fmaxf((float)((int)(__float_as_uint(vscale) >> 23) - 127), -15.f), limit = kLift + kSlack - lv;
 #pragma unroll
-        for (int n = 0; n < kRowsOf; ++n) need |= y[n] > kLift + kSlack;
+        for (int n = 0; n < kRowsOf; ++n) need |= y[n] > limit;
         if (bar_red_or(1, kSoft, need)) {
-          // ---- rare after the first tiles: move the reference maxima and the reference scale, rescale O^T
+          // ---- rare after the first tiles: move the reference maxima, rescale O^T
 #pragma unroll
           for (int n = 0; n < kRowsOf; ++n) {
-            const float wm = warp_max_redux(y[n]);
-            if (lane == n) sMax[wi * 9 + n] = wm;
+            const float wm = warp_max_redux(y[n] + lv);
+            if (lane == n) sMax[wi * 8 + n] = wm;
           }
-          const float wv = warp_max_redux(vscale);
-          if (lane == 8) sMax[wi * 9 + 8] = wv;
           const bool warp_failed = __any_sync(0xffffffffu, fail);
           if (lane == 0) ok_slot[wi] = warp_failed ? 0 : 1;
           named_bar_sync(1, kSoft);
           bool all_ok = true;
-          float vm = 0.f;
 #pragma unroll
-          for (int w = 0; w < kWarps; ++w) { all_ok &= ok_slot[w] != 0; vm = fmaxf(vm, sMax[w * 9 + 8]); }
+          for (int w = 0; w < kWarps; ++w) all_ok &= ok_slot[w] != 0;
           if (!all_ok) { ok = false; break; }
-          const float back = vm > vref ? (vref > 0.f ? vref * pow2_inv(vm) : 0.f) : 1.f;
-          vref = fmaxf(vref, vm);
           float alpha[kRowsOf];
-          bool rescale = back != 1.f;
+          bool rescale = false;
 #pragma unroll
           for (int n = 0; n < kRowsOf; ++n) {
             // a group's rows, and the same rows' other keys next to it
-            const float* mx = sMax + row_group * L::kKeyGroups * 4 * 9 + n;
-            float top = fmaxf(fmaxf(mx[0], mx[9]), fmaxf(mx[18], mx[27]));
-            if (L::kKeyGroups == 2) top = fmaxf(top, fmaxf(fmaxf(mx[36], mx[45]), fmaxf(mx[54], mx[63])));
+            const float* mx = sMax + row_group * L::kKeyGroups * 4 * 8 + n;
+            float top = fmaxf(fmaxf(mx[0], mx[8]), fmaxf(mx[16], mx[24]));
+            if (L::kKeyGroups == 2) top = fmaxf(top, fmaxf(fmaxf(mx[32], mx[40]), fmaxf(mx[48], mx[56])));
             alpha[n] = 1.f;
             const bool first = unset >> n & 1;
             if (top > kLift + kSlack || (first && top > -INFINITY)) {
@@ -686,7 +683,6 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
               unset &= ~(1u << n);
               rescale = true;
             }
-            alpha[n] *= back;
           }
           unset_any = (unset & (rows - row_of >= kRowsOf ? ~0u : (1u << max(0, rows - row_of)) - 1)) != 0;
           // every group has its own columns; the waits of its threads agree because they read the same maxima
@@ -708,16 +704,14 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
           }
           named_bar_sync(1, kSoft);          // sMax has been read
         }
-        const float to_ref = vref > 0.f ? pow2_inv(vref) : 0.f;
         if (!fail) {
           uint8_t* wbuf = sW + buf * L::kP;
-          const float vs = vscale * to_ref;
 #pragma unroll
           for (int n = 0; n < kRowsOf; n += 2) {
             const float x0 = fast_exp2(y[n]), x1 = fast_exp2(y[n + 1]);
             l_part[n] += x0;
             l_part[n + 1] += x1;
-            __half2 rest = __floats2half2_rn(x0 * vs, x1 * vs);
+            __half2 rest = __floats2half2_rn(x0 * vscale, x1 * vscale);
 #pragma unroll
             for (int c = 0; c < W; ++c) {
               const uint16_t code = Pc::kE5 ? f16x2_to_e5m2x2(rest) : f16x2_to_e4m3x2(rest);
@@ -747,7 +741,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
         for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
         if (lane == n) {
           sSum[wi * 8 + n] = v;
-          sMax[wi * 9 + n] = base[n];
+          sMax[wi * 8 + n] = base[n];
         }
       }
       const int first = sPre[cur.req] * p.Hkv + cur.head * cur.n;
@@ -763,12 +757,12 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
         float sum = 0.f;
 #pragma unroll
         for (int w = 0; w < 4 * L::kKeyGroups; ++w) sum += sSum[(w0 + w) * 8 + n];
-        const float lift = sMax[w0 * 9 + n];
+        const float lift = sMax[w0 * 8 + n];
         float den = sum;
         if (!partial && p.sinks != nullptr && tid < rows)
           den += exp2f(p.sinks[cur.head * g + ((int)tid - (int)((tid * inv_g) >> 16) * g)] * kLog2e + lift);
-        // vref comes with the weights' scale; a row that saw nothing gives zeros, a NaN stays one
-        sInv[tid] = !ok || den == 0.f ? 0.f : vref / den;
+        // a row that saw nothing gives zeros, a NaN stays one
+        sInv[tid] = !ok || den == 0.f ? 0.f : 1.f / den;
         if (partial) p.ws_lse[my_slot * kRows + tid] = !ok || sum == 0.f ? -INFINITY : log2f(sum) - lift;
       }
       named_bar_sync(1, kSoft);

@@ -6,8 +6,8 @@ Limits.  With p the softmax weights, s a value row's scale and c its codes, an o
   multiplies weights by at most ``1 + 2 * off``,
 * the rounding of a weight: 2^-8 of it for bf16 queries (three e5m2 pieces take 2^-9, the fp16 number in front of them 2^-11), 2^-11 + 2^-12
   of it for fp16 (an fp16 number and three e4m3 pieces),
-* for weights that are tiny beside the row's largest, half a step of the last piece: no more than ``FLOOR`` times the largest ``p * s`` (or the
-  largest ``p`` times the largest ``s``, see ``spread``) per key, times that key's codes,
+* for weights that are tiny beside the row's largest, half a step of the last piece: no more than ``FLOOR`` times the largest ``p * s`` that
+  the row sees per key, times that key's codes,
 * and one rounding at the end, half a unit of the type.
 """
 import math
@@ -48,9 +48,8 @@ def stored(k, v):
     return c[:, 0].double(), s[:, 0, :, None].double(), c[:, 1].double(), s[:, 1, :, None].double()
 
 
-def results(q, k, v, window=0, spread=False):
-    """What the last ``len(q)`` tokens' queries give, the weights, and how far a result may be off; ``[new, H, D]``, ``[H, new, n]``.
-    ``spread``: weights share one reference for values of all scales, otherwise a small ``p`` of a large value has its digits too."""
+def results(q, k, v, window=0):
+    """What the last ``len(q)`` tokens' queries give, the weights, and how far a result may be off; ``[new, H, D]``, ``[H, new, n]``."""
     ck, sk, cv, sv = stored(k, v)
     g, n, D = q.shape[1] // k.shape[1], len(k), q.shape[2]
     kk, vv, cc, ss = (x.repeat_interleave(g, 1) for x in (ck * sk, cv * sv, cv, sv))
@@ -67,8 +66,7 @@ def results(q, k, v, window=0, spread=False):
     p = torch.softmax(s, 2)
     out = torch.einsum("hij,jhd->ihd", p, vv)
     lim = torch.einsum("hij,jhd->ihd", p, vv.abs()) * (ROUND[q.dtype] + 2 * off + 2.0 ** -17)
-    s_seen = torch.where(seen[None], ss[:, :, 0].T[:, None], 0.0)                 # [H, new, n]
-    top = p.amax(2) * s_seen.amax(2) if spread else (p * s_seen).amax(2)
+    top = (p * ss[:, :, 0].T[:, None]).amax(2)
     lim += FLOOR * top.T[..., None] * torch.einsum("ij,jhd->ihd", seen.double(), cc.abs())
     return out, p, lim
 
@@ -123,3 +121,38 @@ def test_a_key_that_holds_most_of_a_row(n, share, D, group, dt, size):
     assert (p[:, 0, 0] - share).abs().max() < 0.03
     for requests in (1, 300):
         compare(attend(q, k, v, requests=requests), want, lim, q.dtype)
+
+
+@pytest.mark.parametrize("size,others", [(2.0 ** 10, 1.0), (2.0 ** 13, 1.0), (6e4, 1.0), (6e4, 2.0 ** -8)])
+@pytest.mark.parametrize("D,group", [(64, 2), (64, 8), (128, 4), (128, 8), (256, 2), (256, 8)])
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+@pytest.mark.parametrize("where", ["in front of the window", "a later token", "hardly any weight", "a small scale of its own"])
+def test_a_value_far_larger_than_the_others(where, dt, D, group, size, others):
+    """A row that does not see the large value, or gives it next to no weight, has its result from the others."""
+    n, new, window = 3000, 2, 0
+    q, k, v = rows_of(n, new, group, 1, D, DT[dt], D + group)
+    v *= others                                        # 2^-8: the smallest scale of the format, beside its largest
+    big = torch.ones(D, device="cuda") * size
+    check = slice(None)
+    if where == "in front of the window":
+        window = 700                                   # the first row's window starts at 2299; tiles start at multiples of 128 or 256
+        v[2290:2299, 0] = big
+    elif where == "a later token":
+        v[n - 1, 0] = big
+        check = slice(0, 1)                            # the second row sees it
+    elif where == "hardly any weight":
+        k[:, :, 0] = 0
+        k[100, 0] = 0
+        k[100, 0, 0] = -256.0
+        q[..., 0] = 60.0 * D ** 0.5 / 256              # its score is -60, the others' are around 0
+        v[100, 0] = big
+    else:
+        v[5:900] *= 2.0 ** -20                         # small, large and ordinary ones in one tile, the large one with no weight
+        k[:, :, 0] = 0
+        k[100, 0] = 0
+        k[100, 0, 0] = -256.0
+        q[..., 0] = 60.0 * D ** 0.5 / 256
+        v[100, 0] = big
+    want, p, lim = results(q, k, v, window)
+    for requests in (1, 300):
+        compare(attend(q, k, v, window, requests)[:, check], want[check], lim[check], q.dtype)
