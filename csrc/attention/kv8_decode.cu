@@ -401,6 +401,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
+    if (p.early_meta) griddep_wait();        // as the queries' warps do: the limit of the waits below is for this kernel's own work alone
     if (elect_one() && n_tiles > 0) {
       constexpr uint32_t idesc_s = umma_idesc(kM, kNS, 0, 0, 0, 0);     // A = K (K-major), B = Q^T (K-major)
       constexpr uint32_t idesc_o = umma_idesc(kM, kNO, 0, Pc::kE5 ? 1 : 0, 1, 0);     // A = V (e4m3, MN-major), B = P (K-major)

@@ -156,3 +156,34 @@ def test_a_value_far_larger_than_the_others(where, dt, D, group, size, others):
     want, p, lim = results(q, k, v, window)
     for requests in (1, 300):
         compare(attend(q, k, v, window, requests)[:, check], want[check], lim[check], q.dtype)
+
+
+@pytest.mark.parametrize("D", [128])
+def test_a_kernel_in_front_that_takes_its_time(D):
+    """A decode call that starts while the kernel in front of it runs on: its bounded waits do not count that kernel's time (three
+    seconds of attention over 2^27 keys of one block)."""
+    from vllm_kunlun_b200.ops import gemm_cuda
+    q, k, v = rows_of(500, 1, 4, 2, D, torch.bfloat16, D)
+    cache, table = pool(k, v)
+    lens, qsl = torch.tensor([500], dtype=torch.int32, device="cuda"), torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+
+    def step():
+        return ops.paged_attention(q, cache, table, lens, qsl, D ** -0.5, 1, 500, stable_metadata=True)
+
+    want = step()
+    block, n = 1 << 16, 1 << 27
+    slow = torch.zeros(1, 2, 1, block, 20, dtype=torch.uint8, device="cuda")
+    blocks = torch.zeros(1, n // block, dtype=torch.int32, device="cuda")
+    long_lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    one = torch.zeros(1, 1, 16, device="cuda")
+    ops.paged_attention(one, slow, blocks, lens, qsl, 1.0, 1, 500)                # loads the kernel
+    torch.cuda.synchronize()
+    start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    start.record()
+    ops.paged_attention(one, slow, blocks, long_lens, qsl, 1.0, 1, n)
+    got = step()
+    end.record()
+    torch.cuda.synchronize()
+    gemm_cuda.check_status()
+    assert torch.equal(got, want)
+    assert start.elapsed_time(end) > 100, "the kernel in front was over too soon to show anything"
