@@ -457,7 +457,8 @@ kv8_widen_kernel(T* __restrict__ k, __half* __restrict__ v, uint8_t* __restrict_
   griddep_wait();
   const int tile = blockIdx.x >> 1, which = blockIdx.x & 1, h = blockIdx.y, req = blockIdx.z, key0 = tile * kTile;
   const int q_len = qsl[req + 1] - qsl[req], seq_len = seq_lens[req], ctx = seq_len - q_len;
-  const int first = window > 0 ? max(0, ctx - window + 1) / kTile : 0;
+  // the attention kernel's first tile: the last one there is where the window lies behind all that the block tables name
+  const int first = window > 0 ? min(max(0, ctx - window + 1), rows - 1) / kTile : 0;
   // a request whose rows see nothing has its first tile read all the same
   if (q_len <= 0 || tile < first || key0 >= max(seq_len, 1)) return;
   const int* bt = block_tables + (int64_t)req * bt_stride;
