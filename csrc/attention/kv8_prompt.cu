@@ -447,7 +447,8 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         uint4 x[D / 8];
 #pragma unroll
         for (int c = 0; c < D / 8; ++c) x[c] = *reinterpret_cast<const uint4*>(q + (c >> 3) * (kTile * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
-        // magnitudes compare as integers.  Infinities and NaN, and what is too large for its scale to be a number: NaN
+        // magnitudes compare as integers.  Infinities and NaN, and what is too large for its scale to be a number: NaN in every piece, so
+        // that the row's scores are NaN before keys that it does not see are taken out
         uint32_t top = 0;
 #pragma unroll
         for (int c = 0; c < D / 8; ++c)
@@ -456,7 +457,8 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         const float amax = to_f(__builtin_bit_cast(T, (uint16_t)t16));
         const bool bad = !row_ok || !(amax <= 8.5e37f);
         const float up2 = pow2_ceil(bad ? 1.f : fmaxf(amax, 1e-30f)), up = 256.f * pow2_inv(up2);
-        sc = bad ? __uint_as_float(0x7fffffffu) : up2 * (1.f / 256.f) * p.scale_log2;
+        const __half2 instead = __float2half2_rn(row_ok ? __uint_as_float(0x7fffffffu) : 0.f);      // of the elements of a bad row
+        sc = up2 * (1.f / 256.f) * p.scale_log2;
         if (bar_red_or(1 + s, 128, late)) { fail = true; break; }     // also: rows of pieces and of queries overlap
 #pragma unroll
         for (int c = 0; c < D / 16; ++c) {
@@ -465,7 +467,7 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             const float lo = to_f(__builtin_bit_cast(T, (uint16_t)in[j])), hi = to_f(__builtin_bit_cast(T, (uint16_t)(in[j] >> 16)));
-            rest[j] = bad ? __float2half2_rn(0.f) : __floats2half2_rn(lo * up, hi * up);
+            rest[j] = bad ? instead : __floats2half2_rn(lo * up, hi * up);
           }
 #pragma unroll
           for (int k = 0; k < C::P; ++k) {

@@ -28,3 +28,22 @@ def test_requests_longer_than_their_block_table(D, new, window, lengths):
     for _ in range(3):
         leave_nan_behind()
         check(attend(b, window), b, window)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256, 96])
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+@pytest.mark.parametrize("new,lengths,window", [(2, (1, 90), 0), (40, (12, 90), 0), (300, (12, 400), 0), (300, (12, 400), 5)])
+def test_queries_that_are_not_numbers_and_see_nothing(D, dt, new, lengths, window):
+    """A row in front of its request's first key gives zeros whatever its query holds."""
+    b = batch([new, new], [0, 64], 4, 2, D, 64, DT[dt], "cuda", seed=new)
+    b["lens"] = torch.tensor(lengths, dtype=torch.int32, device="cuda")         # more queries than keys in the first request
+    b["max_len"] = max(lengths)
+    q = b["q"].clone()
+    blind = new - lengths[0]
+    q[0, 1, 3], q[blind - 1, 3, D - 1] = math.nan, math.inf
+    q[blind, 0, 0] = -math.inf
+    got = attend({**b, "q": q}, window).cpu()
+    assert (got[:blind] == 0).all()
+    assert got[blind, 1:].isfinite().all()
+    got[blind, 0] = attend(b, window).cpu()[blind, 0]
+    check(got, b, window)
