@@ -24,7 +24,7 @@ kv8_generic_kernel(T* __restrict__ out, const T* __restrict__ q, Kv8Cache c, con
   const int D = c.D;
   float* sq = sm_gen;                       // [D]
   float* so = sq + D;                       // [kGenWarps][D]
-  float* sml = so + kGenWarps * D;          // [kGenWarps][2]
+  float* sml = so + kGenWarps * D;          // [kGenWarps][3]
   griddep_launch();
   griddep_wait();
   const int t = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -42,6 +42,7 @@ kv8_generic_kernel(T* __restrict__ out, const T* __restrict__ q, Kv8Cache c, con
   const int* bt = block_tables + (int64_t)req * bt_stride;
   const int64_t to_v = (int64_t)c.Hkv * c.page_bytes();
   float m = -INFINITY, l = 0.f, acc[ND][4];
+  bool sees = false;                        // any key
 #pragma unroll
   for (int i = 0; i < ND; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
   for (int k0 = first + warp * 32; k0 <= pos; k0 += kGenWarps * 32) {
@@ -70,6 +71,7 @@ kv8_generic_kernel(T* __restrict__ out, const T* __restrict__ q, Kv8Cache c, con
         vs = *c.scale(page + to_v, off);
       }
     }
+    sees |= __any_sync(0xffffffffu, row >= 0);
     if (__any_sync(0xffffffffu, is_nan_bits(s))) l = NAN;
     const float mn = fmaxf(m, warp_max(s));
     if (mn == -INFINITY) continue;
@@ -105,16 +107,16 @@ kv8_generic_kernel(T* __restrict__ out, const T* __restrict__ q, Kv8Cache c, con
       for (int j = 0; j < 4; ++j) so[warp * D + d + j] = acc[i][j];
     }
   }
-  if (lane == 0) { sml[warp * 2] = m; sml[warp * 2 + 1] = l; }
+  if (lane == 0) { sml[warp * 3] = m; sml[warp * 3 + 1] = l; sml[warp * 3 + 2] = sees; }
   __syncthreads();
   float M = sinks != nullptr ? sinks[h] : -INFINITY;
 #pragma unroll
-  for (int w = 0; w < kGenWarps; ++w) M = fmaxf(M, sml[w * 2]);
+  for (int w = 0; w < kGenWarps; ++w) { M = fmaxf(M, sml[w * 3]); sees |= sml[w * 3 + 2] != 0.f; }
   const float Ms = M == -INFINITY ? 0.f : M;
   float den = sinks != nullptr ? expf(sinks[h] - Ms) : 0.f, wg[kGenWarps];
 #pragma unroll
-  for (int w = 0; w < kGenWarps; ++w) { wg[w] = expf(sml[w * 2] - Ms); den += is_nan_bits(sml[w * 2 + 1]) ? NAN : sml[w * 2 + 1] * wg[w]; }
-  const float inv = den == 0.f ? 0.f : 1.f / den;      // NaN stays NaN
+  for (int w = 0; w < kGenWarps; ++w) { wg[w] = expf(sml[w * 3] - Ms); den += is_nan_bits(sml[w * 3 + 1]) ? NAN : sml[w * 3 + 1] * wg[w]; }
+  const float inv = den == 0.f ? (sees ? NAN : 0.f) : 1.f / den;      // NaN stays NaN; keys with scores of -inf alone give one
   for (int d = tid; d < D; d += kGenWarps * 32) {
     float a = 0.f;
 #pragma unroll
@@ -133,7 +135,7 @@ extern "C" int b200_kv8_attention_generic(void* out, const void* q, const void* 
   using namespace b200;
   if (B == 0 || T_ == 0) return 0;
   if (Hq % Hkv || Hq > 65535 || window < 0 || D % 16 || D < 16 || D > 512 || block_size % 4 || T_ > 0x7fffffff) return 2;
-  const size_t smem = (size_t)(D + kGenWarps * (D + 2)) * sizeof(float);
+  const size_t smem = (size_t)(D + kGenWarps * (D + 3)) * sizeof(float);
   const Kv8Cache c{static_cast<uint8_t*>(const_cast<void*>(cache)), num_blocks, Hkv, block_size, D};
   const dim3 grid((unsigned)T_, Hq);
 #define B200_KV8_GEN(ND)                                                                                                         \

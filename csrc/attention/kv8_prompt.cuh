@@ -18,6 +18,7 @@ constexpr int kTile = 128, kPage = 64;
 constexpr int kTmemCols = 512;
 constexpr float kMaxSlack = 8.f;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLowest = -3e38f;         // log-sum-exp of a split whose scores are all -inf; one without keys has -inf
 
 struct Params {
   void* out;                // [T, Hq, D]

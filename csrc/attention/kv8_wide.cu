@@ -318,6 +318,7 @@ kv8_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       const uint8_t* there = w.valid + (int64_t)it.req * (w.rows / kTile);
       uint32_t valid_next = there[it.key0 / kTile];
       float m_used = -INFINITY, l_sum = 0.f;
+      bool sees = false;               // any key
       for (int i = 0; i < n; ++i, ++tc) {
         const int key0 = it.key0 + i * kN;
         constexpr uint32_t kAll = kN == kTile ? 255u : 15u;
@@ -336,8 +337,12 @@ kv8_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                                (p.window <= 0 || key0 > pos_last - p.window);
         if (!full_tile) {
           const int hi = min(pos, it.seq_len - 1) - key0, lo = p.window > 0 ? pos - p.window + 1 - key0 : 0;
+          const int a = max(lo, 0), b = min(hi, kN - 1);
+          if (a <= b) sees |= (valid & (2u << (b >> 4)) - (1u << (a >> 4))) != 0;
 #pragma unroll
           for (int e = 0; e < kN; ++e) v[e] = (e <= hi && e >= lo && (valid >> (e >> 4) & 1u)) ? v[e] : 0xff800000u;   // -inf
+        } else {
+          sees = true;
         }
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -405,8 +410,11 @@ kv8_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       float den = l_sum;
       const float ms = m_used == -INFINITY ? 0.f : m_used;
       if (p.splits == 1 && p.sinks != nullptr) den += exp2f(p.sinks[it.head * p.g + r_head] * kLog2e - ms);
-      const float inv = den == 0.f ? 0.f : 1.f / den;      // a NaN stays one
-      if (p.splits > 1 && row_ok) p.ws_lse[(int64_t)it.split * p.T * p.Hq + orow] = den == 0.f ? -INFINITY : ms + log2f(den);
+      // A NaN stays one.  A row that sees no key gives zeros; one whose scores are all -inf (its query is not finite) NaN, but as a split only if
+      // no other has more.
+      const float inv = den == 0.f ? (sees ? NAN : 0.f) : 1.f / den;
+      if (p.splits > 1 && row_ok)
+        p.ws_lse[(int64_t)it.split * p.T * p.Hq + orow] = den != 0.f ? ms + log2f(den) : sees ? kLowest : -INFINITY;
 #pragma unroll 1
       for (int c = 0; c < D; c += 64) {
         uint32_t o[64];

@@ -47,3 +47,19 @@ def test_queries_that_are_not_numbers_and_see_nothing(D, dt, new, lengths, windo
     assert got[blind, 1:].isfinite().all()
     got[blind, 0] = attend(b, window).cpu()[blind, 0]
     check(got, b, window)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256, 96])
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+@pytest.mark.parametrize("new,context,window", [(2, 0, 0), (40, 0, 0), (300, 0, 0), (300, 0, 1), (60, 5000, 1), (60, 5000, 0)])
+def test_infinite_queries(D, dt, new, context, window):
+    """A query with an infinity gives NaN, the one whose scores are all minus infinity (a single visible key, one sign) like the others."""
+    b = batch([new], [context], 4, 2, D, 64, DT[dt], "cuda", seed=new + context)
+    q = b["q"].clone()
+    for h in range(4):
+        q[h % 2, h, 0] = math.inf if h & 2 else -math.inf
+    got = attend({**b, "q": q}, window).cpu()
+    for h in range(4):
+        assert got[h % 2, h].isnan().all()
+        got[h % 2, h] = attend(b, window).cpu()[h % 2, h]
+    check(got, b, window)
