@@ -668,6 +668,7 @@ extern "C" int b200_kv8_prompt(void* out, const void* cache, const void* tmQ, co
   p.seq_lens = seq_lens; p.qsl = qsl; p.sinks = sinks; p.status = status; p.num_blocks = num_blocks; p.bt_stride = bt_stride;
   p.T = T_; p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.g = Hq / Hkv; p.block_size = block_size; p.max_blocks = max_blocks; p.window = window;
   p.max_keys = 0x7fffff80;
+  p.span = 0x7fffffff;
   p.toks = kv8prompt::kTile / p.g; p.splits = splits; p.scale_log2 = scale * kv8prompt::kLog2e;
   const int64_t tiles = (int64_t)B * Hkv * ((max_query_len + p.toks - 1) / p.toks);
   p.single = tiles * splits <= num_sms;

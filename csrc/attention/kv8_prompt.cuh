@@ -36,6 +36,7 @@ struct Params {
   int single;               // one stream a CTA
   int row_blocks, splits;
   int max_keys;             // no key is looked for from here on (a multiple of 128)
+  int span;                 // nor so many behind the request's first tile
   int take;                 // CTAs may be pending: whoever is done takes their items
   float scale_log2;
 };
@@ -130,9 +131,14 @@ template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi
 // One work item: what the two streams of a CTA share and their own rows.
 struct Item {
   int req, qs, q_len, ctx, seq_len, key0, head, split;     // key0: first key of the first tile
+  int origin;                                              // first_key of the request
   int tok0[2], toks[2], n[2];                              // per stream: first token within the request, tokens, key tiles
   int n_max;
 };
+// The first key that a request's queries read, rounded down to tiles of 128: a window hides what is in front of it.
+__device__ __forceinline__ int first_key(int ctx, int window, int max_keys) {
+  return window > 0 ? min(max(0, ctx - window + 1), max_keys - 1) / kTile * kTile : 0;
+}
 // Items are ordered by descending row block, so by descending number of key tiles for prompts of one length.
 template <int kKeys>       // keys of a tile
 __device__ __forceinline__ void get_item(const Params& p, int idx, Item& it) {
@@ -144,6 +150,7 @@ __device__ __forceinline__ void get_item(const Params& p, int idx, Item& it) {
   it.q_len = p.qsl[it.req + 1] - it.qs;
   it.seq_len = p.seq_lens[it.req];
   it.ctx = it.seq_len - it.q_len;
+  it.origin = first_key(it.ctx, p.window, p.max_keys);
   const int step = p.single ? p.toks : 2 * p.toks;
   int all[2];
   int kv_begin = 0;
@@ -152,9 +159,10 @@ __device__ __forceinline__ void get_item(const Params& p, int idx, Item& it) {
     it.tok0[s] = rb * step + s * p.toks;
     it.toks[s] = (s == 1 && p.single) ? 0 : max(0, min(p.toks, it.q_len - it.tok0[s]));
     // a window hides everything in front of the first token's first visible key (whole tiles of it)
-    if (s == 0 && p.window > 0) kv_begin = min(max(0, it.ctx + it.tok0[0] - p.window + 1), p.max_keys - 1) / kKeys * kKeys;
+    if (s == 0 && p.window > 0)
+      kv_begin = it.origin + min(min(max(0, it.ctx + it.tok0[0] - p.window + 1), p.max_keys - 1) - it.origin, p.span - 1) / kKeys * kKeys;
     // keys visible to the tile end with the position of its last token; rows that see nothing have a tile all the same
-    const int kv_end = min(min(it.seq_len, p.max_keys), it.ctx + it.tok0[s] + it.toks[s]);
+    const int kv_end = it.origin + min(min(min(it.seq_len, p.max_keys), it.ctx + it.tok0[s] + it.toks[s]) - it.origin, p.span);
     all[s] = it.toks[s] > 0 ? max(1, (kv_end - kv_begin + kKeys - 1) / kKeys) : 0;
   }
   const int each = (max(all[0], all[1]) + p.splits - 1) / p.splits, first = it.split * each;

@@ -1186,7 +1186,9 @@ void kv8_prompt(at::Tensor out, const at::Tensor& q, const at::Tensor& cache, co
   const float* sk = sinks.has_value() ? sinks->data_ptr<float>() : nullptr;
   // rows per request and head: no more than the block tables can name
   const int64_t longest = std::max<int64_t>(1, std::min(max_seq_len, block_tables.size(1) * cache.size(3)));
-  const int64_t rows = wide ? (longest + 127) / 128 * 128 : 0;
+  const int64_t max_keys = (longest + 127) / 128 * 128;
+  // with a window those that the queries can see, from a multiple of 128 on
+  const int64_t rows = !wide ? 0 : window > 0 ? std::min(max_keys, (window + max_query_len + 127 + 127) / 128 * 128) : max_keys;
   const int64_t per = Hkv * rows * D * 2;
   const int64_t group = wide ? std::min(B, std::max<int64_t>(1, kKv8Scratch / (2 * per))) : B;
   at::Tensor o, lse, wk, wv, ok;
@@ -1213,7 +1215,7 @@ void kv8_prompt(at::Tensor out, const at::Tensor& q, const at::Tensor& cache, co
     const int* sl = seq_lens.data_ptr<int>() + b0;
     const int* ql = qsl.data_ptr<int>() + b0;
     if (wide)
-      rc = b200_kv8_wide(out.data_ptr(), cache.data_ptr(), tq.b, tk.b, tv.b, wk.data_ptr(), wv.data_ptr(), ok.data_ptr(), (int)rows, bt, sl,
+      rc = b200_kv8_wide(out.data_ptr(), cache.data_ptr(), tq.b, tk.b, tv.b, wk.data_ptr(), wv.data_ptr(), ok.data_ptr(), (int)rows, (int)max_keys, bt, sl,
                          ql, sk, po, pl, splits, s.status.data_ptr<int>(), T, n, (int)Hq, (int)Hkv, (int)D, (int)cache.size(3),
                          (int)block_tables.size(1), block_tables.stride(0), cache.size(0), (int)max_query_len, (int)window, (float)scale,
                          dtype_code(q), s.num_sms, stream());

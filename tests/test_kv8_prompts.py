@@ -63,3 +63,32 @@ def test_infinite_queries(D, dt, new, context, window):
         assert got[h % 2, h].isnan().all()
         got[h % 2, h] = attend(b, window).cpu()[h % 2, h]
     check(got, b, window)
+
+
+def scratch_of(f):
+    """What ``f`` gives, and the bytes that it holds at most on top of that."""
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    out = f()
+    torch.cuda.synchronize()
+    return out, torch.cuda.max_memory_allocated() - before - out.numel() * out.element_size()
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("new,window", [(300, 128), (300, 1000), (1, 128), (500, 1)])
+def test_windows_behind_long_contexts(D, new, window):
+    """Only what the window leaves is widened, at any place; the keys in front of it do not matter."""
+    group = 8 if new > 1 else 32                   # one token of 32 heads a group is a prompt
+    b = batch([new, new, new], [2000, 2100, 2303], 2 * group, 2, D, 64, torch.bfloat16, "cuda", seed=new)
+    want = attend(b, window)
+    check(want, b, window)
+    front = 200_064 // 64                          # even: bits are the same only where tiles of 128 keys start at the same keys
+    table = torch.zeros(3, front + b["table"].shape[1], dtype=torch.int32, device="cuda")
+    for r, shift in enumerate((front, front - 2, front // 2 * 2 - 100)):           # whole tiles of 128 keys in front
+        table[r, shift:shift + b["table"].shape[1]] = b["table"][r]
+        b["lens"][r] += 64 * shift
+    b["table"], b["max_len"] = table, int(b["lens"].max())
+    got, scratch = scratch_of(lambda: attend(b, window))
+    assert torch.equal(got, want)
+    assert scratch < 3 * 2 * D * 4 * (window + new + 256) + 3 * new * 2 * group * (D + 1) * 4 * 32 + (1 << 20)
