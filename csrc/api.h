@@ -171,7 +171,7 @@ int b200_kv8_decode(void* out, const void* q, const void* cache, const void* tma
                     cudaStream_t st);
 int b200_kv8_wide(void* out, const void* cache, const void* tmQ, const void* tmK, const void* tmV, void* wide_k, void* wide_v, void* valid,
                   int rows, int max_keys, const int* block_tables, const int* seq_lens, const int* qsl, const float* sinks, float* ws_o,
-                  float* ws_lse, int splits, int* status, int64_t T, int B, int Hq, int Hkv, int D, int block_size, int max_blocks, int64_t bt_stride,
+                  float* ws_lse, int splits, int* status, int64_t T, int B, int Hq, int Hkv, int head0, int heads, int D, int block_size, int max_blocks, int64_t bt_stride,
                   int64_t num_blocks, int max_query_len, int window, float scale, int dtype, int num_sms, cudaStream_t st);
 int b200_kv8_attention_generic(void* out, const void* q, const void* cache, const int* block_tables, const int* seq_lens,
                                const int* qsl, const float* sinks, int64_t T, int B, int Hq, int Hkv, int D, int block_size,

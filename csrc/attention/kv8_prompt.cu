@@ -631,7 +631,7 @@ static int launch(const Params& p, const CUtensorMap& tmQ, const CUtensorMap& tm
   if (e != cudaSuccess || p.splits == 1) return (int)e;
   const int64_t rows = p.T * p.Hq;
   return (int)launch_pdl(kv8_join_kernel<T, D>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, (T*)p.out, (const float*)p.ws_o,
-                         (const float*)p.ws_lse, p.sinks, rows, p.Hq, p.splits, p.qsl, p.B);
+                         (const float*)p.ws_lse, p.sinks, rows, p.Hq, 0, p.Hq, p.splits, p.qsl, p.B);
 }
 
 }  // namespace kv8prompt
@@ -667,6 +667,7 @@ extern "C" int b200_kv8_prompt(void* out, const void* cache, const void* tmQ, co
   p.out = out; p.ws_o = ws_o; p.ws_lse = ws_lse; p.cache = static_cast<const uint8_t*>(cache); p.block_tables = block_tables;
   p.seq_lens = seq_lens; p.qsl = qsl; p.sinks = sinks; p.status = status; p.num_blocks = num_blocks; p.bt_stride = bt_stride;
   p.T = T_; p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.g = Hq / Hkv; p.block_size = block_size; p.max_blocks = max_blocks; p.window = window;
+  p.heads = Hkv;
   p.max_keys = 0x7fffff80;
   p.span = 0x7fffffff;
   p.toks = kv8prompt::kTile / p.g; p.splits = splits; p.scale_log2 = scale * kv8prompt::kLog2e;

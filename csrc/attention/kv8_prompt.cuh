@@ -32,6 +32,7 @@ struct Params {
   int* status;
   int64_t num_blocks, bt_stride, T;
   int B, Hq, Hkv, g, block_size, max_blocks, window;
+  int head0, heads;         // key / value heads that this launch works on
   int toks;                 // tokens of a tile
   int single;               // one stream a CTA
   int row_blocks, splits;
@@ -142,9 +143,9 @@ __device__ __forceinline__ int first_key(int ctx, int window, int max_keys) {
 // Items are ordered by descending row block, so by descending number of key tiles for prompts of one length.
 template <int kKeys>       // keys of a tile
 __device__ __forceinline__ void get_item(const Params& p, int idx, Item& it) {
-  const int heads = p.Hkv * p.splits, per = p.B * heads, rb = p.row_blocks - 1 - idx / per, rem = idx % per;
+  const int heads = p.heads * p.splits, per = p.B * heads, rb = p.row_blocks - 1 - idx / per, rem = idx % per;
   it.req = rem / heads;
-  it.head = rem % heads / p.splits;
+  it.head = p.head0 + rem % heads / p.splits;
   it.split = rem % p.splits;
   it.qs = p.qsl[it.req];
   it.q_len = p.qsl[it.req + 1] - it.qs;
@@ -196,12 +197,12 @@ __device__ __forceinline__ int taken_cta(uint32_t src) {
 template <typename T, int D>
 __global__ void __launch_bounds__(256)
 kv8_join_kernel(T* __restrict__ out, const float* __restrict__ ws_o, const float* __restrict__ ws_lse, const float* __restrict__ sinks,
-                int64_t rows, int Hq, int splits, const int* __restrict__ qsl, int B) {
+                int64_t rows, int Hq, int head0, int heads, int splits, const int* __restrict__ qsl, int B) {
   griddep_launch();
   griddep_wait();
   const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
-  if (row >= rows || row / Hq < qsl[0] || row / Hq >= qsl[B]) return;
+  if (row >= rows || row / Hq < qsl[0] || row / Hq >= qsl[B] || row % Hq < head0 || row % Hq >= head0 + heads) return;
   constexpr int N = D / 32;
   const float mine = lane < splits ? ws_lse[lane * rows + row] : -INFINITY;      // at most 32 splits
   const float M = warp_max(mine), Ms = M == -INFINITY ? 0.f : M;

@@ -41,7 +41,7 @@ template <typename T> struct Fmt;
 template <> struct Fmt<__nv_bfloat16> { static constexpr uint32_t v = 1; };
 template <> struct Fmt<__half> { static constexpr uint32_t v = 0; };
 
-// Where the widened rows are: [B][Hkv][rows][D], rows a multiple of 128 from the request's first_key on, and which 16 keys of every 128 are there.
+// Where the widened rows are: [B][heads][rows][D], rows a multiple of 128 from the request's first_key on, and which 16 keys of every 128 are there.
 struct Scratch {
   const void* k;
   const void* v;
@@ -156,7 +156,7 @@ kv8_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 tma_load_3d(sQ + s * C::kQ + h * (kTile * 128), &tmQ, q_full, h * 64, it.head * p.g, it.qs + it.tok0[s]);
             }
           ++qc;
-          const int row0 = (it.req * p.Hkv + it.head) * w.rows + it.key0 - it.origin;
+          const int row0 = (it.req * p.heads + it.head - p.head0) * w.rows + it.key0 - it.origin;
           for (int j = 0; ok && j <= n_max; ++j) {      // K(0), K(1), V(0), K(2), V(1), ...
             if (j == n_max - 1 && p.take && !ask()) { ok = false; break; }
             if (j < n_max) {
@@ -461,10 +461,10 @@ template <typename T, int D>
 __global__ void __launch_bounds__(256)
 kv8_widen_kernel(T* __restrict__ k, __half* __restrict__ v, uint8_t* __restrict__ valid, int rows, Kv8Cache c,
                  const int* __restrict__ block_tables, int64_t bt_stride, int max_blocks, const int* __restrict__ seq_lens,
-                 const int* __restrict__ qsl, int window, int max_keys) {
+                 const int* __restrict__ qsl, int window, int max_keys, int head0) {
   griddep_launch();
   griddep_wait();
-  const int tile = blockIdx.x >> 1, which = blockIdx.x & 1, h = blockIdx.y, req = blockIdx.z;
+  const int tile = blockIdx.x >> 1, which = blockIdx.x & 1, h = head0 + blockIdx.y, req = blockIdx.z;
   const int q_len = qsl[req + 1] - qsl[req], seq_len = seq_lens[req], first = first_key(seq_len - q_len, window, max_keys);
   // a request whose rows see nothing has its first tile read all the same
   if (q_len <= 0 || (tile > 0 && tile * kTile >= min(seq_len, max_keys) - first)) return;
@@ -476,12 +476,12 @@ kv8_widen_kernel(T* __restrict__ k, __half* __restrict__ v, uint8_t* __restrict_
     const int b = bi < max_blocks ? bt[bi] : -1;
     return b >= 0 && b < c.num_blocks ? b : -1;
   };
-  if (h == 0 && which == 0 && threadIdx.x < 32) {
+  if (blockIdx.y == 0 && which == 0 && threadIdx.x < 32) {
     const uint32_t bits = __ballot_sync(0xffffffffu, threadIdx.x < 8 && block_of(key0 + threadIdx.x * 16) >= 0);
     if (threadIdx.x == 0) valid[(int64_t)req * (rows / kTile) + tile] = (uint8_t)bits;
   }
   constexpr int kPer = D / 16, kSteps = kTile * kPer / 256;
-  const int64_t out0 = (((int64_t)req * c.Hkv + h) * rows + tile * kTile) * D;
+  const int64_t out0 = (((int64_t)req * gridDim.y + blockIdx.y) * rows + tile * kTile) * D;
   uint4 codes[kSteps];
   float scale[kSteps];
 #pragma unroll
@@ -517,9 +517,9 @@ template <typename T, int D>
 static int launch_wide(const Params& p, const Scratch& w, const CUtensorMap& tmQ, const CUtensorMap& tmK, const CUtensorMap& tmV,
                        int64_t items, cudaStream_t st) {
   const Kv8Cache c{const_cast<uint8_t*>(p.cache), p.num_blocks, p.Hkv, p.block_size, D};
-  cudaError_t e = launch_pdl(kv8_widen_kernel<T, D>, dim3(2 * (w.rows / kTile), p.Hkv, p.B), dim3(256), 0, st, (T*)w.k, (__half*)w.v,
+  cudaError_t e = launch_pdl(kv8_widen_kernel<T, D>, dim3(2 * (w.rows / kTile), p.heads, p.B), dim3(256), 0, st, (T*)w.k, (__half*)w.v,
                              (uint8_t*)w.valid, w.rows, c, p.block_tables, p.bt_stride, p.max_blocks, p.seq_lens, p.qsl, p.window,
-                             p.max_keys);
+                             p.max_keys, p.head0);
   if (e != cudaSuccess) return (int)e;
   auto kern = kv8_wide_kernel<T, D>;
   e = ensure_dynamic_smem((const void*)kern, (int)Wide<D>::kSmem);
@@ -528,39 +528,42 @@ static int launch_wide(const Params& p, const Scratch& w, const CUtensorMap& tmQ
   if (e != cudaSuccess || p.splits == 1) return (int)e;
   const int64_t rows = p.T * p.Hq;
   return (int)launch_pdl(kv8_join_kernel<T, D>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, (T*)p.out, (const float*)p.ws_o,
-                         (const float*)p.ws_lse, p.sinks, rows, p.Hq, p.splits, p.qsl, p.B);
+                         (const float*)p.ws_lse, p.sinks, rows, p.Hq, p.head0 * p.g, p.heads * p.g, p.splits, p.qsl, p.B);
 }
 
 }  // namespace kv8prompt
 }  // namespace b200
 
-// Prompt attention over the 8-bit cache through scratch: wide_k, wide_v [B][Hkv][rows][D] 16-bit and valid [B][rows / 128] bytes.  max_keys: the
+// Prompt attention over the 8-bit cache through scratch, for key / value heads head0 .. head0 + heads - 1: wide_k, wide_v
+// [B][heads][rows][D] 16-bit and valid [B][rows / 128] bytes.  max_keys: the
 // longest request rounded up to 128; rows: the same, or with a window no less than window + max_query_len + 127 rounded down to it.  `tmQ` as for b200_kv8_prompt, `tmK` / `tmV`: the scratch as 2-D with boxes of 64 columns and 128 (heads of
 // 256: 64) and 64 rows.  splits and its scratch as for b200_kv8_prompt.  Returns 3 for shapes it does not serve.
 extern "C" int b200_kv8_wide(void* out, const void* cache, const void* tmQ, const void* tmK, const void* tmV, void* wide_k, void* wide_v,
                              void* valid, int rows, int max_keys, const int* block_tables, const int* seq_lens, const int* qsl, const float* sinks,
-                             float* ws_o, float* ws_lse, int splits, int* status, int64_t T_, int B, int Hq, int Hkv, int D,
-                             int block_size, int max_blocks, int64_t bt_stride, int64_t num_blocks, int max_query_len, int window,
+                             float* ws_o, float* ws_lse, int splits, int* status, int64_t T_, int B, int Hq, int Hkv, int head0, int heads,
+                             int D, int block_size, int max_blocks, int64_t bt_stride, int64_t num_blocks, int max_query_len, int window,
                              float scale, int dtype, int num_sms, cudaStream_t st) {
   using namespace b200;
   if (B == 0 || max_query_len <= 0 || T_ == 0) return 0;
   if (Hq % Hkv || Hq / Hkv > kv8prompt::kTile || block_size % 16 || (D != 64 && D != 128 && D != 256) ||
       (dtype != kBF16 && dtype != kF16) || window < 0 || num_sms < 1 || splits < 1 || splits > 32 || !(scale > 0.f) || rows < 128 ||
-      rows % 128 || max_keys < rows || max_keys % 128 || max_keys > 0x7fffff80 || (int64_t)B * Hkv * rows > 0x7fffffff || B > 65535 || Hkv > 65535)
+      rows % 128 || max_keys < rows || max_keys % 128 || max_keys > 0x7fffff80 || (int64_t)B * heads * rows > 0x7fffffff || B > 65535 || heads > 65535 ||
+      head0 < 0 || heads < 1 || head0 + heads > Hkv)
     return 3;
   if (splits > 1 && (ws_o == nullptr || ws_lse == nullptr)) return 2;
   kv8prompt::Params p = {};
   p.out = out; p.ws_o = ws_o; p.ws_lse = ws_lse; p.cache = static_cast<const uint8_t*>(cache); p.block_tables = block_tables;
   p.seq_lens = seq_lens; p.qsl = qsl; p.sinks = sinks; p.status = status; p.num_blocks = num_blocks; p.bt_stride = bt_stride;
   p.T = T_; p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.g = Hq / Hkv; p.block_size = block_size; p.max_blocks = max_blocks; p.window = window;
+  p.head0 = head0; p.heads = heads;
   p.max_keys = max_keys;
   p.span = rows;
   p.toks = kv8prompt::kTile / p.g; p.splits = splits; p.scale_log2 = scale * kv8prompt::kLog2e;
-  const int64_t tiles = (int64_t)B * Hkv * ((max_query_len + p.toks - 1) / p.toks);
+  const int64_t tiles = (int64_t)B * heads * ((max_query_len + p.toks - 1) / p.toks);
   p.single = D == 256 || tiles * splits <= num_sms;
   const int step = p.single ? p.toks : 2 * p.toks;
   p.row_blocks = (max_query_len + step - 1) / step;
-  const int64_t items = (int64_t)B * Hkv * splits * p.row_blocks;
+  const int64_t items = (int64_t)B * heads * splits * p.row_blocks;
   if (items > (1 << 30)) return 3;
   p.take = items > num_sms;
   const kv8prompt::Scratch w{wide_k, wide_v, static_cast<const uint8_t*>(valid), rows};

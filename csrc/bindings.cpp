@@ -1167,11 +1167,11 @@ void kv8_decode(at::Tensor out, const at::Tensor& q, const at::Tensor& cache, co
         "kv8_decode");
 }
 // More rows than that: prompts and chunks.  `wide`: keys and values of all requests in 16 bits first (scratch), otherwise widened by the
-// attention kernel.  The scratch is bounded: a batch that needs more is worked on request by request group.
-constexpr int64_t kKv8Scratch = 1LL << 30;
+// attention kernel.  The scratch is `scratch` bytes, or one head's keys and values of one request: a call that needs more is worked on in
+// groups of requests, and of heads of one request.
 void kv8_prompt(at::Tensor out, const at::Tensor& q, const at::Tensor& cache, const at::Tensor& block_tables,
                 const at::Tensor& seq_lens, const at::Tensor& qsl, const c10::optional<at::Tensor>& sinks, int64_t max_query_len,
-                int64_t max_seq_len, int64_t window, double scale, bool wide) {
+                int64_t max_seq_len, int64_t window, double scale, bool wide, int64_t scratch) {
   check_kv8_attention(out, q, cache, block_tables, seq_lens, qsl, sinks);
   if (q.size(0) == 0 || seq_lens.size(0) == 0) return;
   c10::cuda::CUDAGuard guard(q.device());
@@ -1189,22 +1189,25 @@ void kv8_prompt(at::Tensor out, const at::Tensor& q, const at::Tensor& cache, co
   const int64_t max_keys = (longest + 127) / 128 * 128;
   // with a window those that the queries can see, from a multiple of 128 on
   const int64_t rows = !wide ? 0 : window > 0 ? std::min(max_keys, (window + max_query_len + 127 + 127) / 128 * 128) : max_keys;
-  const int64_t per = Hkv * rows * D * 2;
-  const int64_t group = wide ? std::min(B, std::max<int64_t>(1, kKv8Scratch / (2 * per))) : B;
+  const int64_t per = rows * D * 4;        // a head's keys and values of a request
+  const int64_t heads = wide ? std::min(Hkv, std::max<int64_t>(1, scratch / per)) : Hkv;
+  const int64_t group = wide ? std::min(B, std::max<int64_t>(1, scratch / (per * Hkv))) : B;
   at::Tensor o, lse, wk, wv, ok;
   if (wide) {
-    wk = at::empty({group, Hkv, rows, D}, q.options());
-    wv = at::empty({group, Hkv, rows, D}, q.options().dtype(at::kHalf));
+    wk = at::empty({group, heads, rows, D}, q.options());
+    wv = at::empty({group, heads, rows, D}, q.options().dtype(at::kHalf));
     ok = at::empty({group, rows / 128}, q.options().dtype(at::kByte));
-    rc = b200_encode_tmap_2d(tk.b, wk.data_ptr(), group * Hkv * rows, D, D * 2, D == 256 ? 64 : 128, 64, 2);
-    if (rc == 0) rc = b200_encode_tmap_2d(tv.b, wv.data_ptr(), group * Hkv * rows, D, D * 2, 64, 64, 2);
+    rc = b200_encode_tmap_2d(tk.b, wk.data_ptr(), group * heads * rows, D, D * 2, D == 256 ? 64 : 128, 64, 2);
+    if (rc == 0) rc = b200_encode_tmap_2d(tv.b, wv.data_ptr(), group * heads * rows, D, D * 2, 64, 64, 2);
     TORCH_CHECK(rc == 0, "tensor map encode failed: ", rc);
   } else {
     tk = kv8_tmap(cache, (int)D, 64);
   }
-  for (int64_t b0 = 0; b0 < B; b0 += group) {
-    const int n = (int)std::min(group, B - b0);
-    const int splits = b200_kv8_prompt_splits(n, (int)Hq, (int)Hkv, (int)max_query_len, max_seq_len, (int)window, s.num_sms);
+  const int64_t parts = (Hkv + heads - 1) / heads;        // of the heads; all of them where there are groups of requests
+  for (int64_t i = 0; i < (B + group - 1) / group * parts; ++i) {
+    const int64_t b0 = i / parts * group, h0 = i % parts * heads;
+    const int n = (int)std::min(group, B - b0), nh = (int)std::min(heads, Hkv - h0);
+    const int splits = b200_kv8_prompt_splits(n, (int)(nh * g), nh, (int)max_query_len, max_seq_len, (int)window, s.num_sms);
     if (splits > 1 && (!o.defined() || o.size(0) < splits)) {
       o = at::empty({splits, T, Hq, D}, q.options().dtype(at::kFloat));
       lse = at::empty({splits, T, Hq}, q.options().dtype(at::kFloat));
@@ -1216,9 +1219,9 @@ void kv8_prompt(at::Tensor out, const at::Tensor& q, const at::Tensor& cache, co
     const int* ql = qsl.data_ptr<int>() + b0;
     if (wide)
       rc = b200_kv8_wide(out.data_ptr(), cache.data_ptr(), tq.b, tk.b, tv.b, wk.data_ptr(), wv.data_ptr(), ok.data_ptr(), (int)rows, (int)max_keys, bt, sl,
-                         ql, sk, po, pl, splits, s.status.data_ptr<int>(), T, n, (int)Hq, (int)Hkv, (int)D, (int)cache.size(3),
-                         (int)block_tables.size(1), block_tables.stride(0), cache.size(0), (int)max_query_len, (int)window, (float)scale,
-                         dtype_code(q), s.num_sms, stream());
+                         ql, sk, po, pl, splits, s.status.data_ptr<int>(), T, n, (int)Hq, (int)Hkv, (int)h0, nh, (int)D,
+                         (int)cache.size(3), (int)block_tables.size(1), block_tables.stride(0), cache.size(0), (int)max_query_len,
+                         (int)window, (float)scale, dtype_code(q), s.num_sms, stream());
     else
       rc = b200_kv8_prompt(out.data_ptr(), cache.data_ptr(), tq.b, tk.b, bt, sl, ql, sk, po, pl, splits, s.status.data_ptr<int>(), T, n,
                            (int)Hq, (int)Hkv, (int)D, (int)cache.size(3), (int)block_tables.size(1), block_tables.stride(0),

@@ -140,6 +140,9 @@ class ModelRunner:
             reserve = int(total * (1 - self.cfg.cache.gpu_memory_utilization))
             # activations for the largest step: a few [T, max(inter, vocab-shard)] buffers
             act = self.max_tokens * 16 * self.cfg.model.hidden_size * 2 + (2 << 30)
+            if self.cfg.cache.cache_dtype == "fp8_e4m3":
+                from ..ops.kv8_cuda import SCRATCH      # what a prompt widens at a time
+                act += SCRATCH
             budget = max(0, free - reserve - act)
             need = self.max_bs * self.max_blocks_per_seq
             n = int(max(16, min(budget // per, need + 64)))

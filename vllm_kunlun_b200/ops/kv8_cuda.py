@@ -14,6 +14,8 @@ from . import _ext
 # B200_KV8_UMMA=0 keeps every call on the generic kernel
 TENSOR_CORES = [os.environ.get("B200_KV8_UMMA", "1") != "0"]
 DECODE_ROWS = 16                # query rows (heads of a group x query tokens) that the decode kernel takes
+# Bytes of keys and values that a prompt call widens at a time: all requests, some of them, or some heads of one (one head at least)
+SCRATCH = 1 << 30
 
 
 def paged_attention_kv8(out, q, kv_cache, block_tables, seq_lens, query_start_loc, scale: float, max_query_len: int,
@@ -48,6 +50,6 @@ def _attend(out, q, kv_cache, block_tables, seq_lens, query_start_loc, scale, ma
             # ten 313 / 233.  Heads of 256 have no kernel that widens inside.
             wide = D == 256 or max_query_len > 2 * (128 // group)
             _ext.C().kv8_prompt(out, q, kv_cache, block_tables, seq_lens, query_start_loc, sinks, max_query_len, max_seq_len, window,
-                                scale, wide)
+                                scale, wide, SCRATCH)
             return
     _ext.C().kv8_attention_generic(out, q, kv_cache, block_tables, seq_lens, query_start_loc, sinks, window, scale)
