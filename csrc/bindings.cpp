@@ -14,6 +14,7 @@
 #include <algorithm>
 #include <atomic>
 #include <mutex>
+#include <map>
 #include <unordered_map>
 
 #include "api.h"
@@ -75,6 +76,7 @@ struct GemmState {
   std::mutex mu;
   std::unordered_map<TmapKey, Tmap, TmapHash> cache;
   at::Tensor ws, counters, status;
+  std::map<int, at::Tensor> other_status;      // status words of devices other than the one above
   int num_sms = 0;
   int64_t launches = 0;
 };
@@ -573,13 +575,20 @@ void gemm_decode_fp8(at::Tensor out, const at::Tensor& xq, const at::Tensor& w, 
 int64_t gemm_status() {
   GemmState& gs = gemm_state();
   if (!gs.status.defined()) return 0;
-  return gs.status.item<int>();
+  int code = gs.status.item<int>();
+  for (const auto& it : gs.other_status)
+    if (code == 0) code = it.second.item<int>();
+  return code;
 }
-// The GEMM status word itself (one int32 on the device), for callers that copy it to the host with other results.
-c10::optional<at::Tensor> gemm_status_tensor() {
+// The status word itself (one int32 on the device), for callers that copy it to the host with other results: that of the device
+// of this number, or of the first one that was used.
+c10::optional<at::Tensor> gemm_status_tensor(c10::optional<int64_t> device) {
   GemmState& gs = gemm_state();
   if (!gs.status.defined()) return c10::nullopt;
-  return gs.status;
+  if (!device.has_value() || *device == gs.status.device().index()) return gs.status;
+  const auto it = gs.other_status.find((int)*device);
+  if (it == gs.other_status.end()) return c10::nullopt;
+  return it->second;
 }
 void gemm_clear_tmap_cache() { gemm_state().cache.clear(); }
 
@@ -1118,7 +1127,11 @@ Kv8State& kv8_state(GemmState& gs, const at::Tensor& like) {      // under gs.mu
       gs.counters = at::zeros({1 << 16}, like.options().dtype(at::kInt));
       gs.status = at::zeros({1}, like.options().dtype(at::kInt));
     }
-    s.status = gs.status.device() == like.device() ? gs.status : at::zeros({1}, like.options().dtype(at::kInt));
+    if (gs.status.device() == like.device()) {
+      s.status = gs.status;
+    } else {
+      s.status = gs.other_status[like.device().index()] = at::zeros({1}, like.options().dtype(at::kInt));
+    }
   }
   return s;
 }
@@ -2311,7 +2324,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("launch_count", &launch_count);
   m.def("gemm", &gemm);
   m.def("gemm_status", &gemm_status);
-  m.def("gemm_status_tensor", &gemm_status_tensor);
+  m.def("gemm_status_tensor", &gemm_status_tensor, py::arg("device") = py::none());
   m.def("gemm_decode", &gemm_decode);
   m.def("gemm_decode_fp8", &gemm_decode_fp8);
   m.def("gemm_decode_qkv", &gemm_decode_qkv);

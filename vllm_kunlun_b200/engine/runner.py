@@ -542,9 +542,14 @@ class ModelRunner:
                 words.append(("ep_a2a", a2a.h.status_tensor()))
             from ..ops import _ext
             if _ext.available():
-                gs = _ext.C().gemm_status_tensor()
+                C = _ext.C()
+                gs = C.gemm_status_tensor()
                 if gs is not None:
                     words.append(("gemm", gs))
+                    here = torch.cuda.current_device() if self.device.index is None else self.device.index
+                    # attention over the 8-bit cache has a word per device
+                    if gs.device.index != here and (own := C.gemm_status_tensor(here)) is not None:
+                        words.append(("kv8", own))
             self._status_cache = words
         return self._status_cache
 
