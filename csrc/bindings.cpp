@@ -608,7 +608,8 @@ void grouped_gemm_impl(at::Tensor out, const at::Tensor& x, const at::Tensor& w,
   TORCH_CHECK(x.is_cuda() && w.is_cuda() && x.dim() == 2 && (w.dim() == 3 || w.dim() == 2));
   TORCH_CHECK(x.stride(1) == 1 && w.is_contiguous() && out.stride(1) == 1);
   const bool fp8 = x.element_size() == 1;
-  TORCH_CHECK(w.element_size() == x.element_size());
+  // wider rows would never fill the stages that the kernel waits for
+  TORCH_CHECK(w.element_size() == x.element_size() && x.element_size() <= 2, "grouped GEMM: rows of 8 or 16 bits, not ", x.scalar_type());
   const int E = w.dim() == 3 ? w.size(0) : 1;
   const int N = w.size(-2), K = w.size(-1), M = x.size(0);
   TORCH_CHECK(x.size(1) == K && out.size(0) == M && out.size(1) == (out_scale ? N / 2 : N));

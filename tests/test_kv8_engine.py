@@ -196,3 +196,15 @@ def test_bf16_models_on_the_gpu(monkeypatch, name, head_dim):
                                                                                         dtype=dtype)] * 2)
     empty = generate(model(name, head_dim, **size), "fp8_e4m3", weights=weights)[1]
     assert float(((empty[0] - want[0]).norm(dim=-1) / want[0].norm(dim=-1)).max()) > 2.0 ** -2
+
+
+@gpu
+def test_experts_of_other_types_are_refused():
+    """Rows of 32 bits: an error, not a wait that gives up."""
+    from vllm_kunlun_b200.ops import _ext
+    x, w = torch.zeros(4, 64, device="cuda"), torch.zeros(2, 64, 64, device="cuda")
+    lod = torch.tensor([0, 2, 4], dtype=torch.int32, device="cuda")
+    bias = torch.zeros(2, 64, device="cuda")
+    for out in (torch.zeros(4, 64, device="cuda"), torch.zeros(4, 64, dtype=torch.bfloat16, device="cuda")):
+        with pytest.raises(RuntimeError, match="8 or 16 bits"):
+            _ext.C().grouped_gemm(out, x, w, lod, bias, None, None, 0, 0)
