@@ -153,7 +153,7 @@ int b200_kv8_put(const void* k, const void* v, void* cache, const int64_t* slots
                  int64_t num_blocks, int64_t k_stride, int64_t v_stride, int dtype, cudaStream_t st);
 int b200_kv8_qkv(void* q_out, const void* qkv, const int64_t* positions, const float* cos_sin, const void* q_w, const void* k_w,
                  float eps, int64_t T, int Hq, int Hkv, int D, int rot_dim, int neox, int gemma, void* cache, const int64_t* slots,
-                 int block_size, int64_t num_blocks, int64_t max_pos, int64_t qkv_stride, int dtype, cudaStream_t st);
+                 int block_size, int64_t num_blocks, int64_t max_pos, int64_t qkv_stride, int dtype, int num_sms, cudaStream_t st);
 // rows of either cache (eight = 0: one in the type of `dtype`, [num_blocks][2][Hkv][block_size][D]) to k, v [M, Hkv, D]
 int b200_kv_gather(void* k, void* v, const void* cache, const int64_t* slots, int64_t M, int Hkv, int D, int block_size,
                    int64_t num_blocks, int eight, int dtype, cudaStream_t st);

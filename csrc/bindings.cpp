@@ -971,7 +971,7 @@ void kv8_qkv(at::Tensor q_out, const at::Tensor& qkv, const at::Tensor& position
   check(b200_kv8_qkv(q_out.data_ptr(), qkv.data_ptr(), positions.data_ptr<int64_t>(), cos_sin.data_ptr<float>(), opt_ptr(q_w),
                      opt_ptr(k_w), (float)eps, T, (int)Hq, (int)Hkv, (int)D, (int)cos_sin.size(1), neox, gemma, cache.data_ptr(),
                      slots.data_ptr<int64_t>(), (int)cache.size(3), cache.size(0), cos_sin.size(0), qkv.stride(0),
-                     dtype_code(qkv), stream()), "kv8_qkv");
+                     dtype_code(qkv), at::cuda::getCurrentDeviceProperties()->multiProcessorCount, stream()), "kv8_qkv");
 }
 void kv_gather(at::Tensor k, at::Tensor v, const at::Tensor& cache, const at::Tensor& slots) {
   TORCH_CHECK(k.dim() == 3 && k.is_contiguous() && v.is_contiguous() && v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type() &&
