@@ -32,8 +32,8 @@
 // the CTA's work, where one fence serves both of its cut items.  Every wait is bounded; on time-out the status word is
 // set and the CTA unwinds.
 // Measured, us (bf16, caches larger than L2; floor = bytes at 6.56 TB/s): 16 requests of 4096 tokens, 32 / 8 heads of 128: 33 (21); 64 of them 94
-// (85); 48 of up to 8192, 32 / 4 heads: 63 (42); 16 / 2 heads of 256, 16 x 4096: 27 (11); 64 / 8 heads of 64, 16 x 4096: 38 (11), of
-// two tokens 61.  The first version, a thread per row of the tile with all its scores: 37 for the first of these.  On the CUDA cores: 344.
+// to 101 (85); 48 of up to 8192, 32 / 4 heads: 63 (42); 16 / 2 heads of 256, 16 x 4096: 25 (11); 64 / 8 heads of 64, 16 x 4096: 41 (11), of
+// two tokens 65.  The first version, a thread per row of the tile with all its scores: 37 for the first of these.  On the CUDA cores: 344.
 #include <cuda.h>
 #include <math.h>
 
@@ -50,7 +50,8 @@ constexpr int kM = 128;          // rows of 128 bytes in a tile
 constexpr int kRows = 16;        // query rows, zero padded
 constexpr int kMaxB = 2048;      // requests a launch
 // A cut this close to an item's end moves there (tiles; CTAs of one tile keep theirs): one tile costs less than a merge of 16 rows.  us without
-// and with, 12 requests of 600 tokens, 8 heads of 128: 16 rows 26.5 and 21.8, 8 rows 18.1 and 15.7, 4 rows 14.3 and 13.1; of 2000: 37.6 and 38.0.
+// and with, 12 requests of 600 tokens, 8 heads of 128: 16 rows 26.0 and 23.2, 8 rows 18.3 and 16.6, 4 rows 14.6 and 13.2; of 2000, 16 rows: 39.7 and
+// 40.8.
 constexpr int kSnap = 1;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -95,9 +96,14 @@ template <> struct Pieces<__half> {
 template <typename T, int D, int NR> struct Layout {
   using G = Geo<D>;
   static constexpr int P = Pieces<T>::q, W = Pieces<T>::w;
-  // Groups of four softmax warps: heads of 64 a group for the even and one for the odd keys; 16 query rows in halves, and 8 where keys are
-  // halved already.  us with 8 rows in one group and in two, 16 requests of 4096 tokens: heads of 128 30.0 and 31.0, heads of 64 54.0 and 46.7.
-  static constexpr int kKeyGroups = G::kPack, kRowGroups = NR == 16 || (NR == 8 && G::kPack == 2) ? 2 : 1, kGroups = kKeyGroups * kRowGroups;
+  // Groups of four softmax warps: heads of 64 a group for the even and one for the odd keys; 16 query rows in halves.  8 rows in halves where
+  // one CTA an SM fits anyway (heads of 256), and where a row of heads of 64 brings many instructions (fp16's pieces), which two groups overlap
+  // better than two CTAs.  us with 8 rows in one group and in two, 16 requests of 4096 tokens / 128 of 1000: heads of 256 bf16 28.0 and 25.3 / 40.6
+  // and 36.1, fp16 30.5 and 27.4 / 43.7 and 38.1; heads of 64 bf16 40.8 and 41.4 / 77.2 and 81.8, fp16 49.3 and 45.5 / 100.0 and 91.7; heads of 128
+  // bf16 29.2 and 29.7 / (64 of 4096) 61.1 and 62.8.
+  static constexpr int kKeyGroups = G::kPack;
+  static constexpr int kRowGroups = NR == 16 || (NR == 8 && (D == 256 || (D == 64 && !Pieces<T>::kE5))) ? 2 : 1;
+  static constexpr int kGroups = kKeyGroups * kRowGroups;
   static constexpr int kSoft = 128 * kGroups, kThreads = 64 + kSoft;
   static constexpr int kCtas = D == 256 || kGroups == 4 ? 1 : 2;        // an SM at most: shared memory, registers
   static constexpr int kRowsOf = NR / kRowGroups;                       // query rows of a thread
