@@ -3,9 +3,11 @@
 //
 // What bounds it is reading the cache, D + 4 bytes a row, so nothing is converted on the way: codes go from memory to shared memory to
 // the tensor core as e4m3 operands, and the numbers that have more digits are taken apart instead.
-//   * Queries: q times a power of two that puts the row's largest element in (128, 256] is the sum of e4m3 pieces, each the rounded rest
-//     of those in front of it.  A piece has four significant bits and rests are signed, so two pieces hold the 8 bits of bf16 and three the
-//     11 of fp16 exactly, down to 2^-18 of the row's largest element.  All pieces add into one accumulator.
+//   * Queries: q times a power of two that puts the row's largest element in (2^14, 2^15] (fp16: half of that) is the sum of three pieces, each
+//     the rounded rest of those in front of it.  An e5m2 piece has three significant bits, an e4m3 piece four, and rests are signed, so three
+//     e5m2 pieces hold the 8 bits of bf16 exactly, off by 2^-32 of the row's largest element for the smallest ones, and two of them with one of
+//     e4m3 the 11 bits of fp16, off by 2^-24: no more than fp32 sums with the largest element are.  All pieces add into one accumulator.
+//     (Two and three e4m3 pieces, off by 2^-18, made rows with one element 2^11 times the others wrong by up to 5 %.)
 //   * Weights: exp2(s - m) * v_scale * 2^lift, m the largest s + log2(v_scale) that the row has seen, so that neither a heavy key with a small
 //     value nor a light or hidden one with a large value takes the others' digits.  In fp16 and then in three pieces; each rest is multiplied
 //     up so that weights far below the largest keep theirs, and every piece has accumulator columns of its own.  The many keys behind one that
@@ -79,17 +81,21 @@ template <int D> struct Geo {
   static constexpr int kOp = kBlk * kM * 128;          // codes of K or V of a tile
   static constexpr int kNS = kRows * kPack;            // columns of S^T
 };
-// Pieces of a query (q) and of a weight (w; the rest times kStep from one to the next).  The running maximum moves when a score exceeds it by
+// Pieces of a query (q; of those scaled to at most kTop) and of a weight (w; the rest times kStep from one to the next).  The running maximum moves when a score exceeds it by
 // more than kSlack (log2): weights stay below 2^(kLift + kSlack).
 template <typename T> struct Pieces;
 template <> struct Pieces<__nv_bfloat16> {
-  static constexpr int q = 2, w = 3;
+  static constexpr int q = 3, w = 3;
   static constexpr bool kE5 = true;
+  static constexpr float kTop = 32768.f;
+  __host__ __device__ static constexpr bool q_e5(int) { return true; }
   static constexpr float kStep = 8.f, kLift = 7.f, kSlack = 8.f;
 };
 template <> struct Pieces<__half> {
   static constexpr int q = 3, w = 3;
   static constexpr bool kE5 = false;
+  static constexpr float kTop = 16384.f;
+  __host__ __device__ static constexpr bool q_e5(int piece) { return piece < 2; }
   static constexpr float kStep = 32.f, kLift = 5.f, kSlack = 3.f;
 };
 
@@ -114,7 +120,7 @@ template <typename T, int D, int NR> struct Layout {
   static constexpr int kTmem = kCols <= 64 ? 64 : kCols <= 128 ? 128 : 256;
   static constexpr int kScales = G::kKeys * 4;
   // barriers, factors, flags, exchange buffers
-  static constexpr int kMisc = 4096 + (D == 64 ? kRows * 64 * 4 : 0);      // 2 KB of it for up to 16 softmax warps
+  static constexpr int kMisc = 2048 + (D == 64 ? kRows * 64 * 4 : 0);
   static size_t smem(int slots, int B) {
     return 1024 + (size_t)slots * (G::kOp + kScales) + kQ + 2 * kP + kMisc + (size_t)(B + 1) * 4;
   }
@@ -141,18 +147,6 @@ __device__ __forceinline__ void tmem_st_rows(uint32_t taddr, const uint32_t (&r)
 __device__ __forceinline__ void tmem_st_rows(uint32_t taddr, const uint32_t (&r)[4]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
 }
-__device__ __forceinline__ uint16_t f16x2_to_e4m3x2(__half2 v) {
-  uint16_t r;
-  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(*reinterpret_cast<const uint32_t*>(&v)));
-  return r;
-}
-__device__ __forceinline__ uint16_t f16x2_to_e5m2x2(__half2 v) {
-  uint16_t r;
-  asm("cvt.rn.satfinite.e5m2x2.f16x2 %0, %1;" : "=h"(r) : "r"(*reinterpret_cast<const uint32_t*>(&v)));
-  return r;
-}
-// an e5m2 number is the upper byte of the same fp16 number
-__device__ __forceinline__ uint32_t e5m2x2_to_f16x2(uint16_t v) { return __byte_perm(v, 0, 0x1404); }
 // 2^x, results below 2^-126 as zero, which is far below what a weight's pieces hold
 __device__ __forceinline__ float fast_exp2(float x) {
   float r;
@@ -409,7 +403,8 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
     // ------------------------------------------------------------------ MMA issuer
     if (p.early_meta) griddep_wait();        // as the queries' warps do: the limit of the waits below is for this kernel's own work alone
     if (elect_one() && n_tiles > 0) {
-      constexpr uint32_t idesc_s = umma_idesc(kM, kNS, 0, 0, 0, 0);     // A = K (K-major), B = Q^T (K-major)
+      // A = K (e4m3, K-major), B = a piece of Q^T (K-major)
+      constexpr uint32_t idesc_s[2] = {umma_idesc(kM, kNS, 0, 0, 0, 0), umma_idesc(kM, kNS, 0, 1, 0, 0)};
       constexpr uint32_t idesc_o = umma_idesc(kM, kNO, 0, Pc::kE5 ? 1 : 0, 1, 0);     // A = V (e4m3, MN-major), B = P (K-major)
       const uint32_t tS = tmem_base, tO = tmem_base + 2 * kNS;
       const uint32_t q_addr = smem_u32(sQ), p_addr = smem_u32(sP), kv_addr = smem_u32(smem);
@@ -439,7 +434,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
           for (int c = 0; c < P * kBlk * 4; ++c) {
             const int piece = c / (kBlk * 4), b = (c / 4) % kBlk, k = c % 4;
             umma_f8(tS + (next_s & 1) * kNS, umma_desc_k_sw128(k_at + b * (kM * 128) + k * 32),
-                    umma_desc_k_sw128(q_at + (piece * kBlk + b) * (kNS * 128) + k * 32), idesc_s, c > 0 ? 1u : 0u);
+                    umma_desc_k_sw128(q_at + (piece * kBlk + b) * (kNS * 128) + k * 32), idesc_s[Pc::q_e5(piece)], c > 0 ? 1u : 0u);
           }
           umma_commit(&s_full[next_s & 1]);
           umma_commit(&kv_empty[ks]);
@@ -528,10 +523,10 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
         for (int o = kLanes / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
         // infinities, NaN, and what is too large for its scale to be a number: NaN
         const bool bad = amax == INFINITY;
-        const float top = bad ? 1.f : pow2_ceil(fmaxf(amax, 1e-30f)), up = 256.f * pow2_inv(top);
+        const float top = bad ? 1.f : pow2_ceil(fmaxf(amax, 1e-30f)), up = Pc::kTop * pow2_inv(top);
         if (row >= NR) continue;       // whole warps, or the same lanes of every exchange above
-        if (d == 0) sFactor[(item & 1) * kRows + row] = bad ? __uint_as_float(0x7fffffffu) : top * (1.f / 256.f) * p.scale_log2;
-        __half2 rest[4];               // at most 256: fp16 holds it
+        if (d == 0) sFactor[(item & 1) * kRows + row] = bad ? __uint_as_float(0x7fffffffu) : top * (1.f / Pc::kTop) * p.scale_log2;
+        __half2 rest[4];               // fp16 holds numbers up to kTop
 #pragma unroll
         for (int j = 0; j < 4; ++j) rest[j] = bad ? __float2half2_rn(0.f) : __floats2half2_rn(v[2 * j] * up, v[2 * j + 1] * up);
 #pragma unroll
@@ -539,8 +534,8 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
           uint16_t e[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            e[j] = f16x2_to_e4m3x2(rest[j]);
-            if (c + 1 < P) rest[j] = __hsub2(rest[j], as_half2(e4m3x2_to_f16x2(e[j])));
+            e[j] = Pc::q_e5(c) ? f16x2_to_e5m2x2(rest[j]) : f16x2_to_e4m3x2(rest[j]);
+            if (c + 1 < P) rest[j] = __hsub2(rest[j], as_half2(Pc::q_e5(c) ? e5m2x2_to_f16x2(e[j]) : e4m3x2_to_f16x2(e[j])));
           }
           const uint2 w = make_uint2(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16);
 #pragma unroll

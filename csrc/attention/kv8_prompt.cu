@@ -4,14 +4,15 @@
 // Per 128-key tile and 128-row query tile
 //     S[128 rows, 128 keys]  = Q . K_tile^T                 e4m3: codes as cached, queries in pieces
 //     O[128 rows, D dims]   += P[128 rows, 128 keys] . V    fp16, P in TMEM over the columns of S
-// Queries are sums of e4m3 pieces as in kv8_decode.cu (two hold bf16 exactly, three fp16), so K is an operand as it comes from memory; its
-// scales are multiplied onto the scores.  Two pieces at twice the rate of a 16-bit product cost what that would.  V and P go the other
+// Queries are sums of three 8-bit pieces as in kv8_decode.cu, so K is an operand as it comes from memory; its scales are multiplied onto the
+// scores.  Three pieces at twice the rate of a 16-bit product cost one and a half times what that would.  V and P go the other
 // way: pieces of P would have to be made by the softmax warps, which have no time left, so four warps widen V to fp16 between the TMA's
 // buffer and the tensor core's.  Every stored value is an exact fp16 number (common/kv8.cuh): its scale is gone then, and P rounds to 11 bits.
-// What bounds it: per tile the tensor core needs 1024 cycles, the special-function units as many (128 x 128 exponentials at 16 a cycle),
-// shared memory a little more for two tiles than both (1216 a tile: operands, TMA, widening, scales).
-// Measured, us, beside the kernel that widens first (kv8_wide.cu), 32 / 8 heads of 128: 17 new tokens (one tile) behind 16000: 37 and 52; 60 (two): 52
-// and 63; 128 (four): 95 and 91; 300 (ten): 313 and 233; 12 x 30 tokens without context: 12 and 16.  So it takes up to two tiles.
+// What bounds it: per tile the tensor core needs 1280 cycles, the special-function units 1024 (128 x 128 exponentials at 16 a cycle), shared
+// memory more than either (operands, TMA, widening, scales).
+// Measured, us, beside the kernel that widens first (kv8_wide.cu), 32 / 8 heads of 128 behind 16000 tokens: one tile 44 and 58, two 57 and 65, four 100
+// and 92, ten 328 and 235; 12 requests without context, one tile 12 and 14.  So it takes up to two tiles.  (Two pieces, which hold fewer digits:
+// 43, 53, 94, 305.)
 //
 // A row is (token, head of a group): a tile holds 128 / g tokens of all g heads of one key / value head, so that a few new tokens fill it,
 // and K and V are read and converted once for the group.  A persistent CTA works on two tiles ("streams") of consecutive tokens that read
@@ -32,20 +33,26 @@ constexpr int kThreads = 4 * 128;
 // 65536, and the split takes 128 x (64 + 192 + 192 + 64) = 65536.
 constexpr int kRegsFew = 64, kRegsSoft = 192;
 constexpr int kVStages = 4;                              // V pages as operands
-constexpr int kRing = 4;                                 // K scales and valid masks: one more than the K stages
+constexpr int kRing = 4;                                 // K scales and valid masks: more than the K stages
 
 template <typename T> struct Pieces;
-template <> struct Pieces<__nv_bfloat16> { static constexpr int n = 2; };
-template <> struct Pieces<__half> { static constexpr int n = 3; };
+template <> struct Pieces<__nv_bfloat16> {
+  static constexpr float kTop = 32768.f;
+  __host__ __device__ static constexpr bool e5(int) { return true; }
+};
+template <> struct Pieces<__half> {
+  static constexpr float kTop = 16384.f;
+  __host__ __device__ static constexpr bool e5(int piece) { return piece < 2; }
+};
 
 template <typename T, int D> struct Cfg {
-  static constexpr int P = Pieces<T>::n;
+  static constexpr int P = 3;
   static constexpr int kPiece = kTile * D;             // 128 rows of D e4m3 bytes
   static constexpr int kQ = P * kPiece;                // a stream's queries; in 16 bits (2 * kPiece) until they are taken apart
-  static constexpr int kKStages = 3 - (P == 3 && D == 128), kK = kTile * D;
+  static constexpr int kKStages = D == 128 ? 2 : 3, kK = kTile * D;
   static constexpr int kB = D / 64;                    // 64-dim blocks of a 16-bit row
   static constexpr int kV = kB * kPage * 128;
-  static constexpr int kRaw = P == 3 && D == 128 ? 3 : 4, kCodes = kPage * D;      // V pages as codes
+  static constexpr int kRaw = D == 128 ? 3 : 4, kCodes = kPage * D;      // V pages as codes
   static constexpr size_t kSmem =
       1024 + 2 * kQ + kKStages * kK + kVStages * kV + kRaw * (kCodes + kPage * 4) + kRing * kTile * 4 + 512;
   static_assert(kSmem <= 227 * 1024 && kKStages < kRing);
@@ -287,7 +294,8 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
     if (elect_one()) {
-      constexpr uint32_t idesc_s = umma_idesc(kTile, kTile, 0, 0, 0, 0);   // A = Q, B = K tile, both e4m3 and K-major
+      // A = a piece of Q, B = K tile (e4m3), both K-major
+      constexpr uint32_t idesc_s[2] = {umma_idesc(kTile, kTile, 0, 0, 0, 0), umma_idesc(kTile, kTile, 1, 0, 0, 0)};
       constexpr uint32_t idesc_o = umma_idesc(kTile, D, 0, 0, 0, 1);       // A = P (TMEM), B = V tile (MN-major), fp16
       int kc = 0, vc = 0, qc[2] = {0, 0}, tc[2] = {0, 0};   // consumed so far; tc: tiles of each stream whose P has been awaited
       bool ok = true;
@@ -301,7 +309,7 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 #pragma unroll
           for (int c = 0; c < C::P * (D / 32); ++c)
             umma_f8(tmem_base + s * kTile, desc_rows<D>(q_addr + c / (D / 32) * C::kPiece + c % (D / 32) * 32),
-                    desc_rows<D>(k_addr + c % (D / 32) * 32), idesc_s, c > 0 ? 1u : 0u);
+                    desc_rows<D>(k_addr + c % (D / 32) * 32), idesc_s[Pieces<T>::e5(c / (D / 32))], c > 0 ? 1u : 0u);
           umma_commit(&s_full[s]);
           const bool last = s == 1 || j >= it.n[1];
           if (last) {
@@ -456,13 +464,13 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         const uint32_t t16 = max(top & 0xffffu, top >> 16);
         const float amax = to_f(__builtin_bit_cast(T, (uint16_t)t16));
         const bool bad = !row_ok || !(amax <= 8.5e37f);
-        const float up2 = pow2_ceil(bad ? 1.f : fmaxf(amax, 1e-30f)), up = 256.f * pow2_inv(up2);
+        const float up2 = pow2_ceil(bad ? 1.f : fmaxf(amax, 1e-30f)), up = Pieces<T>::kTop * pow2_inv(up2);
         const __half2 instead = __float2half2_rn(row_ok ? __uint_as_float(0x7fffffffu) : 0.f);      // of the elements of a bad row
-        sc = up2 * (1.f / 256.f) * p.scale_log2;
+        sc = up2 * (1.f / Pieces<T>::kTop) * p.scale_log2;
         if (bar_red_or(1 + s, 128, late)) { fail = true; break; }     // also: rows of pieces and of queries overlap
 #pragma unroll
         for (int c = 0; c < D / 16; ++c) {
-          __half2 rest[8];                   // 16 elements, scaled: at most 256, fp16 holds them
+          __half2 rest[8];                   // 16 elements, scaled: at most kTop, fp16 holds them
           const uint32_t in[8] = {x[2 * c].x, x[2 * c].y, x[2 * c].z, x[2 * c].w, x[2 * c + 1].x, x[2 * c + 1].y, x[2 * c + 1].z, x[2 * c + 1].w};
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
@@ -474,10 +482,12 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             uint32_t y[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              const uint16_t a = f16x2_to_e4m3x2(rest[2 * j]), b = f16x2_to_e4m3x2(rest[2 * j + 1]);
+              constexpr auto e5 = Pieces<T>::e5;
+              const uint16_t a = e5(k) ? f16x2_to_e5m2x2(rest[2 * j]) : f16x2_to_e4m3x2(rest[2 * j]);
+              const uint16_t b = e5(k) ? f16x2_to_e5m2x2(rest[2 * j + 1]) : f16x2_to_e4m3x2(rest[2 * j + 1]);
               y[j] = a | (uint32_t)b << 16;
               if (k + 1 < C::P) {
-                const uint32_t ua = e4m3x2_to_f16x2(a), ub = e4m3x2_to_f16x2(b);
+                const uint32_t ua = e5(k) ? e5m2x2_to_f16x2(a) : e4m3x2_to_f16x2(a), ub = e5(k) ? e5m2x2_to_f16x2(b) : e4m3x2_to_f16x2(b);
                 rest[2 * j] = __hsub2(rest[2 * j], *reinterpret_cast<const __half2*>(&ua));
                 rest[2 * j + 1] = __hsub2(rest[2 * j + 1], *reinterpret_cast<const __half2*>(&ub));
               }

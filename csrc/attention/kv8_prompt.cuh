@@ -105,11 +105,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
-__device__ __forceinline__ uint16_t f16x2_to_e4m3x2(__half2 v) {
-  uint16_t r;
-  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(*reinterpret_cast<const uint32_t*>(&v)));
-  return r;
-}
 // 2^x on the special-function unit (-inf -> 0)
 __device__ __forceinline__ float ex2_approx(float x) {
   float y;

@@ -55,6 +55,18 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint16_t c) {
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(c));
   return r;
 }
+// and back, rounded; e5m2 numbers are the upper bytes of fp16 numbers
+__device__ __forceinline__ uint16_t f16x2_to_e4m3x2(__half2 v) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(*reinterpret_cast<const uint32_t*>(&v)));
+  return r;
+}
+__device__ __forceinline__ uint16_t f16x2_to_e5m2x2(__half2 v) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e5m2x2.f16x2 %0, %1;" : "=h"(r) : "r"(*reinterpret_cast<const uint32_t*>(&v)));
+  return r;
+}
+__device__ __forceinline__ uint32_t e5m2x2_to_f16x2(uint16_t v) { return __byte_perm(v, 0, 0x1404); }
 __device__ __forceinline__ float2 e4m3x2_to_float2(uint16_t c) {
   const uint32_t r = e4m3x2_to_f16x2(c);
   return __half22float2(*reinterpret_cast<const __half2*>(&r));

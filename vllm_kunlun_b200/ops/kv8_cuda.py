@@ -46,10 +46,10 @@ def _attend(out, q, kv_cache, block_tables, seq_lens, query_start_loc, scale, ma
             return
         if D in (64, 128, 256) and group <= 128 and scale > 0:
             # widened once for all query tiles where more than one pair of them (128 // group tokens each) reads the same keys.
-            # us widened inside and first, one request behind 16000 tokens, by tiles: 32 / 8 heads of 128: one 39 / 57, two 52 / 65, three
-            # 68 / 76, four 93 / 93, six 118 / 110, ten 305 / 235; 64 / 8 heads of 64: 35 / 37, 46 / 43, 59 / 52, 79 / 66, 101 / 79, 267 / 189.
-            # 40 requests behind 1000: 88 / 121, 111 / 138, 168 / 177, 182 / 190, 260 / 246, 437 / 362; heads of 64: 65 / 69, 92 / 90,
-            # 138 / 119, 155 / 129, 218 / 169, 349 / 258.  Heads of 256 have no kernel that widens inside.
+            # us widened inside and first, one request behind 16000 tokens, by tiles: 32 / 8 heads of 128: one 44 / 58, two 57 / 65, three
+            # 74 / 76, four 100 / 92, six 127 / 110, ten 328 / 235; 64 / 8 heads of 64: 36 / 41, 48 / 44, 61 / 53, 80 / 66, 102 / 79, 269 / 188.
+            # 40 requests behind 1000: 96 / 120, 117 / 138, 176 / 176, 188 / 188, 270 / 245, 451 / 382; heads of 64: 67 / 68, 95 / 90,
+            # 143 / 119, 160 / 129, 227 / 169, 364 / 258.  Heads of 256 have no kernel that widens inside.
             wide = D == 256 or max_query_len > 2 * (128 // group)
             _ext.C().kv8_prompt(out, q, kv_cache, block_tables, seq_lens, query_start_loc, sinks, max_query_len, max_seq_len, window,
                                 scale, wide, SCRATCH)
